@@ -314,6 +314,94 @@ int nxt_paged_attention_fp8_append_ex(
     int *device_status,
     nxt_stream_t stream);
 
+/* ── extension: 4-bit KV cache ──────────────────────────────────────────
+ * E2M1 codes with one E4M3 scale per 16 channels of a token and one fp32
+ * scale per pool: value = code * scale * pool_scale, 4.5 bits per element.
+ *   t = x / pool_scale in fp32 (NaN counts as 0),
+ *   scale = E4M3(max |t| over the 16 channels / 6), nearest even, at most 448,
+ *   code  = E2M1(t / scale), nearest even, at most 6 (0 when scale is 0).
+ * head_size is a multiple of 16 up to 256, block_size a multiple of 16.
+ * Pools are bytes: page p of KV head h starts at p * kv_block_stride +
+ * h * kv_head_stride (strides in bytes, multiples of 16; pools start on
+ * 16-byte boundaries) and holds block_size / 16 tiles of 9 * head_size bytes,
+ * one per 16 tokens:
+ *   K: 16 rows of head_size / 2 code bytes, then scales [16][head_size / 16];
+ *      a row is, for t = 0..3, for j = 0..head_size / 16 - 1, the codes of
+ *      channels 16 j + 4 t .. 16 j + 4 t + 3 (two per byte, low nibble first);
+ *   V: 16 rows of code bytes in channel order, then scales
+ *      [head_size / 16][16 tokens].
+ * Writing a token touches its own codes and scales only. Query, rows and
+ * output are fp16. */
+
+/* Stores token t's rows (fp16 key/value [num_tokens][num_kv_heads][head_size]
+ * at token_stride elements) at slot slot_mapping[t]; a negative slot, or one
+ * past the pools when num_blocks > 0, skips the token. The slots of one call
+ * are distinct. */
+int nxt_reshape_and_cache_q4(
+    const void *key, const void *value,
+    void *key_cache, void *value_cache,
+    const int64_t *slot_mapping, int num_tokens,
+    int num_kv_heads, int head_size, int block_size,
+    float k_scale, float v_scale,
+    int64_t kv_block_stride, int64_t kv_head_stride, int64_t token_stride,
+    int64_t num_blocks,
+    nxt_stream_t stream);
+
+/* Reads rows back: row t of key/value (fp16, token_stride elements) receives
+ * the values at slot slot_mapping[t], rounded to fp16 and at most its largest
+ * finite value; a slot that the write would skip gives a row of zeros. Slots may repeat. */
+int nxt_read_cache_q4(
+    void *key, void *value,
+    const void *key_cache, const void *value_cache,
+    const int64_t *slot_mapping, int num_tokens,
+    int num_kv_heads, int head_size, int block_size,
+    float k_scale, float v_scale,
+    int64_t kv_block_stride, int64_t kv_head_stride, int64_t token_stride,
+    int64_t num_blocks,
+    nxt_stream_t stream);
+
+/* Paged decode attention over 4-bit pools: the result of
+ * nxt_paged_attention_ex over the dequantised cache, for any number of query
+ * heads per KV head. Masking, clamping, status bits and workspace as there; a
+ * caller-owned workspace needs nxt_paged_attention_q4_workspace_size bytes.
+ * The library's own workspace is one per (device, stream): graphs captured on
+ * one stream and replayed at the same time need workspaces of their own. */
+int nxt_paged_attention_q4_ex(
+    void *out, const void *query,
+    const void *key_cache, const void *value_cache,
+    const int *block_tables, const int *seq_lens,
+    int num_seqs, int num_heads, int head_size,
+    int num_kv_heads, float scale,
+    int max_num_blocks_per_seq, int block_size,
+    float k_scale, float v_scale,
+    int64_t kv_block_stride, int64_t kv_head_stride,
+    int64_t num_blocks,
+    void *workspace, size_t workspace_bytes,
+    int *device_status,
+    nxt_stream_t stream);
+
+size_t nxt_paged_attention_q4_workspace_size(int num_seqs, int num_heads, int head_size,
+                                             int num_kv_heads, int max_num_blocks_per_seq,
+                                             int block_size);
+
+/* Decode step: stores new_key/new_value (fp16 [num_seqs][num_kv_heads]
+ * [head_size], one new token per sequence) at slot_mapping[b] as
+ * nxt_reshape_and_cache_q4 does, then attends over seq_lens (which already
+ * count the new token) with the library's own workspace. */
+int nxt_paged_attention_q4_append_ex(
+    void *out, const void *query,
+    void *key_cache, void *value_cache,
+    const int *block_tables, const int *seq_lens,
+    const void *new_key, const void *new_value, const int64_t *slot_mapping,
+    int num_seqs, int num_heads, int head_size,
+    int num_kv_heads, float scale,
+    int max_num_blocks_per_seq, int block_size,
+    float k_scale, float v_scale,
+    int64_t kv_block_stride, int64_t kv_head_stride,
+    int64_t num_blocks,
+    int *device_status,
+    nxt_stream_t stream);
+
 /* ── extension: block-table builder ─────────────────────────────────────
  * The glue between a continuous-batching scheduler and these kernels (the
  * reference's scheduler, src/core/scheduler.c:278-440, stops at the list of

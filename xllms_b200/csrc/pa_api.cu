@@ -14,6 +14,7 @@
 #include <thread>
 #include <functional>
 #include <utility>
+#include <vector>
 
 #include "operator_api.h"
 #include "pa_host.h"
@@ -60,6 +61,11 @@ struct Workspace {
 };
 // Keyed by (device, stream) so calls on different streams never share partials.
 std::map<std::pair<int, uintptr_t>, Workspace> g_ws;
+
+// Scratch of the 4-bit and sparse entry points (acquire_scratch).
+std::mutex g_scratch_mu;
+std::map<std::pair<int, uintptr_t>, Workspace> g_scratch;
+std::vector<std::pair<int, void*>> g_scratch_old;  // outgrown buffers, by device
 
 int map_cuda(cudaError_t e) { return e == cudaSuccess ? NXT_PA_OK : NXT_PA_ECUDA; }
 
@@ -118,6 +124,51 @@ int sm_count_of(int dev) {
     d.probed = true;
   }
   return d.sm_count;
+}
+
+int status_word(int dev, int** out) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  DeviceState* d = nullptr;
+  const int rc = device_state_locked(dev, &d);
+  if (rc == NXT_PA_OK) *out = d->status;
+  return rc;
+}
+
+int acquire_scratch(int dev, cudaStream_t st, size_t bytes, void** out,
+                    std::unique_lock<std::mutex>& lk) {
+  if (dev < 0 || dev >= kMaxDevices) return NXT_PA_EINVAL;
+  lk = std::unique_lock<std::mutex>(g_scratch_mu);
+  Workspace& w = g_scratch[{dev, stream_key(st)}];
+  if (w.bytes < bytes) {
+    // at least doubled, so that what is kept of old buffers stays below the newest
+    const size_t want = std::max(bytes, 2 * w.bytes);
+    void* p = nullptr;
+    if (cudaMalloc(&p, want) != cudaSuccess) {
+      cudaGetLastError();
+      return NXT_PA_ENOMEM;
+    }
+    if (w.ptr) g_scratch_old.emplace_back(dev, w.ptr);
+    w.ptr = p;
+    w.bytes = want;
+  }
+  *out = w.ptr;
+  return NXT_PA_OK;
+}
+
+int release_scratch() {
+  std::lock_guard<std::mutex> lk(g_scratch_mu);
+  int prev = 0;
+  const bool have_prev = cudaGetDevice(&prev) == cudaSuccess;
+  int rc = NXT_PA_OK;
+  auto drop = [&rc](int dev, void* p) {
+    if (p && (cudaSetDevice(dev) != cudaSuccess || cudaFree(p) != cudaSuccess)) rc = NXT_PA_ECUDA;
+  };
+  for (auto& kv : g_scratch) drop(kv.first.first, kv.second.ptr);
+  for (auto& o : g_scratch_old) drop(o.first, o.second);
+  g_scratch.clear();
+  g_scratch_old.clear();
+  if (have_prev) cudaSetDevice(prev);
+  return rc;
 }
 
 // Sharded calls on several GPUs: 1 = every output row is stored (to every
@@ -639,10 +690,10 @@ int nxt_paged_attention_device_status(int clear) {
 }
 
 int nxt_paged_attention_release_workspaces(void) {
+  int rc = release_scratch();
   std::lock_guard<std::mutex> lk(g_mu);
   int prev = 0;
   const bool have_prev = cudaGetDevice(&prev) == cudaSuccess;
-  int rc = NXT_PA_OK;
   for (auto& kv : g_ws) {
     if (!kv.second.ptr) continue;
     if (cudaSetDevice(kv.first.first) != cudaSuccess || cudaFree(kv.second.ptr) != cudaSuccess)

@@ -3,7 +3,10 @@
 #pragma once
 
 #include <cuda.h>
+#include <cuda_runtime.h>
 #include <stddef.h>
+
+#include <mutex>
 
 namespace xpa {
 namespace host {
@@ -58,6 +61,19 @@ bool fast_layout_ok(const void* k, const void* v, int D, int Hkv, long long kbs,
 int check_args(const void* out, const void* q, const void* k, const void* v, const int* bt,
                const int* sl, int B, int Hq, int D, int Hkv, int max_blocks, int bs, int ds,
                long long kbs, long long khs);
+
+// The library status word of device `dev` (the current device).
+int status_word(int dev, int** out);
+
+// Library-owned scratch of the 4-bit and sparse entry points, one buffer per
+// (device, stream). `lk` holds the pool's lock on return: keep it until the
+// call's kernels are enqueued, so that no other thread on the same stream can
+// hand out the buffer in between. A buffer that has to grow is replaced, and
+// the old one kept until release_scratch(), since a captured graph may still
+// name it. EINVAL / ENOMEM / OK.
+int acquire_scratch(int dev, cudaStream_t st, size_t bytes, void** out,
+                    std::unique_lock<std::mutex>& lk);
+int release_scratch();
 
 }  // namespace host
 }  // namespace xpa

@@ -19,6 +19,7 @@ the native kernels.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from typing import Optional, Union
@@ -547,6 +548,199 @@ def paged_attention_fp8_append(query, key_cache, value_cache, block_tables, seq_
         _ptr(device_status), _stream_ptr(stream))
     if rc != _native.NXT_PA_OK:
         raise PagedAttentionError(rc, "nxt_paged_attention_fp8_append_ex")
+    return out
+
+
+# ── 4-bit KV cache ─────────────────────────────────────────────────────────
+@contextlib.contextmanager
+def _launching(like, stream):
+    """Makes `like`'s device current and yields the stream pointer to launch
+    on; tensors made inside belong to that stream, so that the allocator gives
+    their memory to no one else while the kernels run."""
+    import torch
+    with torch.cuda.device(like.device):
+        if stream is None:
+            yield torch.cuda.current_stream().cuda_stream
+            return
+        st = torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream
+        with torch.cuda.stream(st):
+            yield st.cuda_stream
+
+
+def q4_pool_shape(num_blocks, num_kv_heads, block_size, head_size):
+    """Shape of a 4-bit K or V pool (uint8): [num_blocks, Hkv, block_size / 16,
+    9 * head_size], one row of bytes per 16 tokens (include/operator_api.h)."""
+    if block_size <= 0 or block_size % 16 or head_size <= 0 or head_size % 16 or head_size > 256:
+        raise PagedAttentionError(_native.NXT_PA_EINVAL, "q4_pool_shape: block_size and head_size "
+                                  "must be multiples of 16, head_size at most 256")
+    return (num_blocks, num_kv_heads, block_size // 16, 9 * head_size)
+
+
+def _check_q4_pools(where, key_cache, value_cache, like):
+    """(num_blocks, Hkv, block_size, head_size) of two 4-bit pools."""
+    import torch
+    for c in (key_cache, value_cache):
+        if (c.dim() != 4 or c.dtype != torch.uint8 or c.shape[3] % 144 or not c.shape[3]
+                or c.shape[3] > 9 * 256 or tuple(c.shape) != tuple(key_cache.shape)
+                or not c.is_contiguous() or not c.is_cuda or c.device != like.device):
+            raise PagedAttentionError(
+                _native.NXT_PA_EINVAL, f"{where}: 4-bit pools must be contiguous uint8 [num_blocks, "
+                "Hkv, block_size / 16, 9 * head_size] on the rows' device")
+    nb, hkv, spp, tile = key_cache.shape
+    return nb, hkv, 16 * spp, tile // 9
+
+
+def _q4_strides(hkv, bs, d):
+    return hkv * bs * d * 9 // 16, bs * d * 9 // 16
+
+
+def _check_rows(where, key, value, slots, heads, dim):
+    import torch
+    if (key.dim() != 3 or tuple(key.shape[1:]) != (heads, dim) or key.shape != value.shape
+            or key.dtype != torch.float16 or value.dtype != torch.float16
+            or (key.shape[0] and (key.stride(2) != 1 or (heads > 1 and key.stride(1) != dim)
+                                  or (key.shape[0] > 1 and key.stride(0) < heads * dim)
+                                  or key.stride() != value.stride()))
+            or not key.is_cuda or value.device != key.device
+            or not _index_ok(slots, key.shape[0], key)):
+        raise PagedAttentionError(_native.NXT_PA_EINVAL, f"{where}: rows must be fp16 [T, Hkv, D] "
+                                  "with dense heads and slot_mapping int64 [T], on one device")
+    return key.stride(0) if key.shape[0] > 1 else heads * dim
+
+
+def reshape_and_cache_q4(key, value, key_cache, value_cache, slot_mapping, k_scale, v_scale,
+                         stream=None) -> None:
+    """Quantise fp16 key/value [T, Hkv, D] into 4-bit pools (q4_pool_shape) at
+    slot_mapping[t] (int64; negative or past the pools: skipped; distinct)."""
+    nb, hkv, bs, d = _check_q4_pools("reshape_and_cache_q4", key_cache, value_cache, key)
+    ts = _check_rows("reshape_and_cache_q4", key, value, slot_mapping, hkv, d)
+    with _launching(key, stream) as st:
+        rc = _native.xpa().nxt_reshape_and_cache_q4(
+            _ptr(key), _ptr(value), _ptr(key_cache), _ptr(value_cache), _ptr(slot_mapping),
+            key.shape[0], hkv, d, bs, float(k_scale), float(v_scale), *_q4_strides(hkv, bs, d),
+            ts, nb, st)
+    if rc != _native.NXT_PA_OK:
+        raise PagedAttentionError(rc, "nxt_reshape_and_cache_q4")
+
+
+def read_cache_q4(key_cache, value_cache, slot_mapping, k_scale, v_scale, *, key=None, value=None,
+                  stream=None):
+    """The rows that 4-bit pools hold at slot_mapping[t], as fp16 key and value
+    [T, Hkv, D]; rows of negative slots, or slots past the pools, are zero."""
+    import torch
+    nb, hkv, bs, d = _check_q4_pools("read_cache_q4", key_cache, value_cache, key_cache)
+    with _launching(key_cache, stream) as st:
+        shape = (slot_mapping.numel(), hkv, d)
+        if key is None:
+            key = torch.empty(shape, dtype=torch.float16, device=key_cache.device)
+        if value is None:
+            value = (torch.empty(shape, dtype=torch.float16, device=key_cache.device)
+                     if key.is_contiguous() else torch.empty_strided(
+                         shape, key.stride(), dtype=torch.float16, device=key_cache.device))
+        if key.dim() != 3 or key.shape[0] != slot_mapping.numel():
+            raise PagedAttentionError(_native.NXT_PA_EINVAL, "read_cache_q4: rows")
+        ts = _check_rows("read_cache_q4", key, value, slot_mapping, hkv, d)
+        if key.device != key_cache.device:
+            raise PagedAttentionError(_native.NXT_PA_EINVAL, "read_cache_q4: devices")
+        rc = _native.xpa().nxt_read_cache_q4(
+            _ptr(key), _ptr(value), _ptr(key_cache), _ptr(value_cache), _ptr(slot_mapping),
+            key.shape[0], hkv, d, bs, float(k_scale), float(v_scale), *_q4_strides(hkv, bs, d),
+            ts, nb, st)
+    if rc != _native.NXT_PA_OK:
+        raise PagedAttentionError(rc, "nxt_read_cache_q4")
+    return key, value
+
+
+def _check_q4_attention(where, query, key_cache, value_cache, block_tables, seq_lens, out):
+    import torch
+
+    def bad(msg):
+        raise PagedAttentionError(_native.NXT_PA_EINVAL, f"{where}: {msg}")
+    if query.dim() != 3 or query.dtype != torch.float16 or not query.is_contiguous():
+        bad("query must be contiguous fp16 [B, Hq, D]")
+    if not query.is_cuda:
+        bad("every tensor must be on the query's CUDA device")
+    nb, hkv, bs, d = _check_q4_pools(where, key_cache, value_cache, query)
+    if query.shape[2] != d:
+        bad("head size of query and pools")
+    _check_tables(bad, query, block_tables, seq_lens, out)
+    return nb, hkv, bs, d
+
+
+def _check_tables(bad, query, block_tables, seq_lens, out):
+    import torch
+    B = query.shape[0]
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] < B:
+        bad("block_tables must be int32 [B, max_blocks]")
+    if seq_lens.dtype != torch.int32 or seq_lens.numel() < B:
+        bad("seq_lens must be int32 [B]")
+    if out is not None and (tuple(out.shape) != tuple(query.shape) or out.dtype != query.dtype):
+        bad("out must have the query's shape and dtype")
+    for t in (block_tables, seq_lens) + (() if out is None else (out,)):
+        if not t.is_contiguous():
+            bad("non-contiguous input")
+        if t.device != query.device:
+            bad("every tensor must be on the query's CUDA device")
+
+
+def paged_attention_q4(query, key_cache, value_cache, block_tables, seq_lens, k_scale, v_scale, *,
+                       scale=None, out=None, num_blocks=None, workspace=None, device_status=None,
+                       stream=None):
+    """Decode attention over 4-bit pools (q4_pool_shape); query and output fp16
+    [B, Hq, D], any number of query heads per KV head."""
+    import torch
+    nb, hkv, bs, d = _check_q4_attention("paged_attention_q4", query, key_cache, value_cache,
+                                         block_tables, seq_lens, out)
+    B, Hq, _ = query.shape
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    with _launching(query, stream) as st:
+        if out is None:
+            out = torch.empty_like(query)
+        rc = _native.xpa().nxt_paged_attention_q4_ex(
+            _ptr(out), _ptr(query), _ptr(key_cache), _ptr(value_cache), _ptr(block_tables),
+            _ptr(seq_lens), B, Hq, d, hkv, 1.0 / math.sqrt(d) if scale is None else float(scale),
+            block_tables.shape[1], bs, float(k_scale), float(v_scale), *_q4_strides(hkv, bs, d),
+            nb if num_blocks is None else int(num_blocks), _ptr(workspace), ws_bytes,
+            _ptr(device_status), st)
+    if rc != _native.NXT_PA_OK:
+        raise PagedAttentionError(rc, "nxt_paged_attention_q4_ex")
+    return out
+
+
+def q4_workspace_size(num_seqs, num_heads, head_size, num_kv_heads, max_num_blocks_per_seq,
+                      block_size=16) -> int:
+    """Workspace bytes of a paged_attention_q4 call on the current device."""
+    return int(_native.xpa().nxt_paged_attention_q4_workspace_size(
+        num_seqs, num_heads, head_size, num_kv_heads, max_num_blocks_per_seq, block_size))
+
+
+def paged_attention_q4_append(query, key_cache, value_cache, block_tables, seq_lens, new_key,
+                              new_value, slot_mapping, k_scale, v_scale, *, scale=None, out=None,
+                              num_blocks=None, device_status=None, stream=None):
+    """One decode step on 4-bit pools: new_key/new_value (fp16 [B, Hkv, D]) are
+    stored at slot_mapping[b] and included in the attention (seq_lens count
+    them)."""
+    import torch
+    where = "paged_attention_q4_append"
+    nb, hkv, bs, d = _check_q4_attention(where, query, key_cache, value_cache, block_tables,
+                                         seq_lens, out)
+    B, Hq, _ = query.shape
+    _check_rows(where, new_key, new_value, slot_mapping, hkv, d)
+    if (new_key.shape[0] != B or not new_key.is_contiguous() or not new_value.is_contiguous()
+            or new_key.device != query.device):
+        raise PagedAttentionError(_native.NXT_PA_EINVAL, f"{where}: new rows must be contiguous "
+                                  "[B, Hkv, D] on the query's device")
+    with _launching(query, stream) as st:
+        if out is None:
+            out = torch.empty_like(query)
+        rc = _native.xpa().nxt_paged_attention_q4_append_ex(
+            _ptr(out), _ptr(query), _ptr(key_cache), _ptr(value_cache), _ptr(block_tables),
+            _ptr(seq_lens), _ptr(new_key), _ptr(new_value), _ptr(slot_mapping), B, Hq, d, hkv,
+            1.0 / math.sqrt(d) if scale is None else float(scale), block_tables.shape[1], bs,
+            float(k_scale), float(v_scale), *_q4_strides(hkv, bs, d),
+            nb if num_blocks is None else int(num_blocks), _ptr(device_status), st)
+    if rc != _native.NXT_PA_OK:
+        raise PagedAttentionError(rc, "nxt_paged_attention_q4_append_ex")
     return out
 
 
