@@ -402,6 +402,114 @@ int nxt_paged_attention_q4_append_ex(
     int *device_status,
     nxt_stream_t stream);
 
+/* ── extension: page bounds and sparse decode attention ─────────────────
+ * For long contexts: attention over the max_pages pages of a sequence that
+ * score best against its query, chosen per KV head. A page is scored by its
+ * bounds, the lowest and highest key per channel:
+ *   score = max over the KV head's query heads q of
+ *           sum_d max(q_d * lo_d, q_d * hi_d),
+ * which no q . k of the page exceeds (of q . k times the sign of `scale`). The
+ * first sink_pages and the last recent_pages pages of a sequence are always
+ * kept, the rest of max_pages goes to the best others, in the exact order of
+ * the scores, ties to the earlier page. A sequence of at most max_pages pages
+ * keeps them all, and the result is then nxt_paged_attention_ex's. Pages that
+ * the table does not name validly are never kept (NXT_PA_DEV_BAD_PAGE).
+ *
+ * bounds: [num_blocks][num_kv_heads][2][head_size] (lowest, then highest) in
+ * the query's type, one entry per physical page. NaN keys count as 0 there,
+ * infinite ones as the largest finite value; queries likewise in the scores.
+ *
+ * Sizes: sink_pages >= 0, recent_pages >= 1, sink_pages + recent_pages <=
+ * max_pages, max_pages * block_size an int. With several KV heads the pools'
+ * kv_block_stride is a multiple of kv_head_stride. */
+
+/* Writes the bounds of the pages that hold the last num_new_tokens tokens of
+ * each sequence (0: of all its pages), over their valid tokens. To call after
+ * the tokens are stored: with the number of tokens added since the last call,
+ * or more. dtype_size 2 or 4. */
+int nxt_page_bounds(
+    void *bounds, const void *key_cache,
+    const int *block_tables, const int *seq_lens,
+    int num_seqs, int num_kv_heads, int head_size,
+    int max_num_blocks_per_seq, int block_size, int dtype_size,
+    int64_t kv_block_stride, int64_t kv_head_stride,
+    int64_t num_blocks, int num_new_tokens,
+    int *device_status,
+    nxt_stream_t stream);
+
+/* The same from 4-bit keys (the values nxt_read_cache_q4 returns); the bounds
+ * are fp16. */
+int nxt_page_bounds_q4(
+    void *bounds, const void *key_cache,
+    const int *block_tables, const int *seq_lens,
+    int num_seqs, int num_kv_heads, int head_size,
+    int max_num_blocks_per_seq, int block_size, float k_scale,
+    int64_t kv_block_stride, int64_t kv_head_stride,
+    int64_t num_blocks, int num_new_tokens,
+    int *device_status,
+    nxt_stream_t stream);
+
+/* The selection alone, for any attention call over these pools:
+ *   sel_tables [num_seqs * num_kv_heads][max_pages]: the kept pages of row
+ *     b * num_kv_heads + h in order, as page * (kv_block_stride /
+ *     kv_head_stride) + h (as page with one KV head), -1 past the last;
+ *   sel_lens [num_seqs * num_kv_heads]: tokens in them;
+ *   sel_pages (may be NULL) [num_seqs * num_kv_heads][max_pages]: their
+ *     indices within the sequence, -1 past the last.
+ * An attention call then takes num_seqs * num_kv_heads sequences with
+ * num_heads / num_kv_heads query heads and one KV head each, sel_tables,
+ * sel_lens, max_pages table entries, and kv_head_stride as block stride. */
+int nxt_select_pages(
+    int *sel_tables, int *sel_lens, int *sel_pages,
+    const void *query, const void *bounds,
+    const int *block_tables, const int *seq_lens,
+    int num_seqs, int num_heads, int head_size,
+    int num_kv_heads, float scale,
+    int max_num_blocks_per_seq, int block_size, int dtype_size,
+    int64_t kv_block_stride, int64_t kv_head_stride,
+    int64_t num_blocks,
+    int max_pages, int sink_pages, int recent_pages,
+    void *workspace, size_t workspace_bytes,
+    int *device_status,
+    nxt_stream_t stream);
+
+/* Selection and attention in one call. sel_pages as above (may be NULL);
+ * workspace and device_status as for nxt_paged_attention_ex. */
+int nxt_paged_attention_sparse_ex(
+    void *out, const void *query,
+    const void *key_cache, const void *value_cache, const void *bounds,
+    const int *block_tables, const int *seq_lens, int *sel_pages,
+    int num_seqs, int num_heads, int head_size,
+    int num_kv_heads, float scale,
+    int max_num_blocks_per_seq, int block_size, int dtype_size,
+    int64_t kv_block_stride, int64_t kv_head_stride,
+    int64_t num_blocks,
+    int max_pages, int sink_pages, int recent_pages,
+    void *workspace, size_t workspace_bytes,
+    int *device_status,
+    nxt_stream_t stream);
+
+/* The same over 4-bit pools. */
+int nxt_paged_attention_q4_sparse_ex(
+    void *out, const void *query,
+    const void *key_cache, const void *value_cache, const void *bounds,
+    const int *block_tables, const int *seq_lens, int *sel_pages,
+    int num_seqs, int num_heads, int head_size,
+    int num_kv_heads, float scale,
+    int max_num_blocks_per_seq, int block_size,
+    float k_scale, float v_scale,
+    int64_t kv_block_stride, int64_t kv_head_stride,
+    int64_t num_blocks,
+    int max_pages, int sink_pages, int recent_pages,
+    void *workspace, size_t workspace_bytes,
+    int *device_status,
+    nxt_stream_t stream);
+
+/* Workspace bytes that suffice for the three calls above with these sizes. */
+size_t nxt_paged_attention_sparse_workspace_size(
+    int num_seqs, int num_heads, int head_size, int num_kv_heads,
+    int max_num_blocks_per_seq, int block_size, int dtype_size, int max_pages);
+
 /* ── extension: block-table builder ─────────────────────────────────────
  * The glue between a continuous-batching scheduler and these kernels (the
  * reference's scheduler, src/core/scheduler.c:278-440, stops at the list of

@@ -117,6 +117,25 @@ SIGNATURES = {
         _I,
         [_VP, _CVP, _VP, _VP, _IP, _IP, _CVP, _CVP, _VP, _I, _I, _I, _I, _F, _I, _I, _F, _F,
          _I64, _I64, _I64, _VP, _VP]),
+    "nxt_page_bounds": (
+        _I,
+        [_VP, _CVP, _IP, _IP, _I, _I, _I, _I, _I, _I, _I64, _I64, _I64, _I, _VP, _VP]),
+    "nxt_page_bounds_q4": (
+        _I,
+        [_VP, _CVP, _IP, _IP, _I, _I, _I, _I, _I, _F, _I64, _I64, _I64, _I, _VP, _VP]),
+    "nxt_select_pages": (
+        _I,
+        [_IP, _IP, _IP, _CVP, _CVP, _IP, _IP, _I, _I, _I, _I, _F, _I, _I, _I, _I64, _I64, _I64,
+         _I, _I, _I, _VP, _SZ, _VP, _VP]),
+    "nxt_paged_attention_sparse_ex": (
+        _I,
+        [_VP, _CVP, _CVP, _CVP, _CVP, _IP, _IP, _IP, _I, _I, _I, _I, _F, _I, _I, _I, _I64, _I64,
+         _I64, _I, _I, _I, _VP, _SZ, _VP, _VP]),
+    "nxt_paged_attention_q4_sparse_ex": (
+        _I,
+        [_VP, _CVP, _CVP, _CVP, _CVP, _IP, _IP, _IP, _I, _I, _I, _I, _F, _I, _I, _F, _F, _I64,
+         _I64, _I64, _I, _I, _I, _VP, _SZ, _VP, _VP]),
+    "nxt_paged_attention_sparse_workspace_size": (_SZ, [_I, _I, _I, _I, _I, _I, _I, _I]),
     "nxt_reshape_and_cache": (
         _I, [_CVP, _CVP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I64, _I64, _I64, _VP]),
     "nxt_paged_attention_append_ex": (

@@ -1,0 +1,61 @@
+// pa_sparse.h — host-side launchers of the page bounds and page selection
+// kernels (pa_sparse.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "pa_device.cuh"
+
+namespace xpa {
+
+// Element type of the cache the bounds are taken from.
+constexpr int kBoundsF16 = 0;
+constexpr int kBoundsF32 = 1;
+constexpr int kBoundsQ4 = 2;  // 4-bit keys; the bounds are fp16
+
+struct BoundsParams {
+  void* bounds;  // [num_blocks][Hkv][2][D]: lowest, then highest key per channel
+  const void* key_cache;
+  const int* block_tables;
+  const int* seq_lens;
+  int* status;
+  long long kv_block_stride, kv_head_stride;  // elements (4-bit: bytes)
+  long long num_blocks;
+  int B, Hkv, D, max_blocks, block_size;
+  int num_new;        // > 0: only pages that hold one of the last num_new tokens
+  int pages_per_seq;  // pages of a sequence that may be due
+  int kind;
+  int vec;            // every key row and bounds row starts on a 16-byte boundary
+  float k_scale;      // 4-bit
+};
+
+cudaError_t launch_bounds(const BoundsParams& p, cudaStream_t st);
+
+struct SelectParams {
+  const void* q;       // [B][Hq][D]
+  const void* bounds;  // [num_blocks][Hkv][2][D]
+  const int* block_tables;
+  const int* seq_lens;
+  int* status;
+  int* sel_tables;  // [B * Hkv][keep] page * head_pages + kv head
+  int* sel_lens;    // [B * Hkv] tokens kept
+  int* sel_pages;   // [B * Hkv][keep] page index within the sequence, -1 past the last; or null
+  // workspace
+  unsigned* keys;         // [B * Hkv][max_blocks] ordered scores, 0: page not eligible
+  float* absmax;          // [B * Hkv][chunks] largest |bound| seen by the score kernel's CTAs
+  unsigned* near_page;    // [B * Hkv][max_blocks] pages too near the border for fp32
+  unsigned long long* near_key;  // [B * Hkv][max_blocks] their scores in 64 bits
+  long long num_blocks;
+  long long head_pages;  // kv_block_stride / kv_head_stride
+  int B, Hq, Hkv, D, GS, max_blocks, block_size;
+  int keep, sink, recent;
+  int chunks;  // score CTAs per row
+  float sign;  // of the score scale: -1, 0 or 1
+  int vec;     // fp16, D % 8 == 0, q and bounds on 16-byte boundaries
+};
+
+constexpr int kScoreChunk = 256;  // pages per score CTA
+
+cudaError_t launch_select(const SelectParams& p, int dtype_size, cudaStream_t st);
+
+}  // namespace xpa

@@ -1,0 +1,318 @@
+// pa_sparse_api.cu — C ABI of page bounds and sparse decode attention
+// (include/operator_api.h). Attention over the kept pages is the framework's
+// own decode attention on per-head pages: page p of KV head h is page
+// p * (kv_block_stride / kv_head_stride) + h of a pool with one KV head.
+#include <climits>
+#include <cmath>
+
+#include "operator_api.h"
+#include "pa_host.h"
+#include "pa_sparse.h"
+
+using namespace xpa::host;
+
+namespace {
+
+int map_cuda(cudaError_t e) { return e == cudaSuccess ? NXT_PA_OK : NXT_PA_ECUDA; }
+
+bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int bounds_call(void* bounds, const void* key_cache, const int* bt, const int* sl, int B, int Hkv,
+                int D, int max_blocks, int bs, int kind, float k_scale, int64_t kbs, int64_t khs,
+                int64_t num_blocks, int num_new, int* dev_status, cudaStream_t st) {
+  const bool q4 = kind == xpa::kBoundsQ4;
+  if (B < 0 || num_new < 0) return NXT_PA_EINVAL;
+  if (B == 0) return NXT_PA_OK;
+  if (!bounds || !key_cache || !bt || !sl) return NXT_PA_EINVAL;
+  if (Hkv <= 0 || D <= 0 || D > 256 || bs <= 0 || max_blocks < 0 || kbs < 0 || khs < 0)
+    return NXT_PA_EINVAL;
+  const unsigned es = kind == xpa::kBoundsF32 ? 4 : 2;
+  if (!aligned(bounds, es)) return NXT_PA_EINVAL;
+  if (q4) {
+    if (D % 16 || bs % 16 || kbs % 16 || khs % 16 || !aligned(key_cache, 16) ||
+        !(k_scale > 0.f) || !std::isfinite(k_scale))
+      return NXT_PA_EINVAL;
+  } else if (!aligned(key_cache, es)) {
+    return NXT_PA_EINVAL;
+  }
+  if (max_blocks == 0) return NXT_PA_OK;
+  xpa::BoundsParams p{};
+  p.bounds = bounds;
+  p.key_cache = key_cache;
+  p.block_tables = bt;
+  p.seq_lens = sl;
+  p.kv_block_stride = kbs;
+  p.kv_head_stride = khs;
+  p.num_blocks = num_blocks;
+  p.B = B;
+  p.Hkv = Hkv;
+  p.D = D;
+  p.max_blocks = max_blocks;
+  p.block_size = bs;
+  p.num_new = num_new;
+  // the last num_new tokens lie in at most this many pages
+  p.pages_per_seq = max_blocks;
+  if (num_new > 0 && (num_new - 1) / bs + 2 < max_blocks) p.pages_per_seq = (num_new - 1) / bs + 2;
+  p.kind = kind;
+  p.k_scale = k_scale;
+  if (!q4) {
+    p.vec = aligned(key_cache, 16) && aligned(bounds, 16) && (D * es) % 16 == 0 &&
+            (kbs * es) % 16 == 0 && (khs * es) % 16 == 0;
+  }
+  if ((long long)B * Hkv > INT_MAX || (long long)B * Hkv * p.pages_per_seq / 4 >= INT_MAX)
+    return NXT_PA_EINVAL;
+  p.status = dev_status;
+  if (!p.status) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return NXT_PA_ECUDA;
+    const int rc = status_word(dev, &p.status);
+    if (rc != NXT_PA_OK) return rc;
+  }
+  return map_cuda(xpa::launch_bounds(p, st));
+}
+
+// One sparse call. Exactly one of the attention forms is asked for, or none
+// (selection alone, into the caller's arrays).
+struct SparseCall {
+  // selection
+  const void *q, *bounds;
+  const int *bt, *sl;
+  int* sel_pages;
+  int B, Hq, D, Hkv;
+  float scale;
+  int max_blocks, bs, ds;
+  int64_t kbs, khs, num_blocks;
+  int keep, sink, recent;
+  // attention
+  void* out = nullptr;
+  const void *k = nullptr, *v = nullptr;
+  bool q4 = false;
+  float k_scale = 1.f, v_scale = 1.f;
+};
+
+// Workspace: scores and near pages of the selection, the kept pages' tables,
+// the attention's partials, each from a 256-byte boundary.
+struct Layout {
+  size_t keys, absmax, near_page, near_key, tables, lens, part, total;
+  size_t part_bytes;
+  int chunks;
+};
+
+Layout layout_of(long long rows, int GS, int D, int max_blocks, int bs, int ds, int keep, bool q4,
+                 bool attention) {
+  Layout l{};
+  size_t at = 0;
+  auto take = [&at](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  l.chunks = ceil_div(max_blocks, xpa::kScoreChunk);
+  const size_t scored = max_blocks > keep ? (size_t)rows * max_blocks : 0;
+  l.keys = take(scored * sizeof(unsigned));
+  l.absmax = take((size_t)rows * l.chunks * sizeof(float));
+  l.near_page = take(scored * sizeof(unsigned));
+  l.near_key = take(scored * sizeof(unsigned long long));
+  if (attention) {
+    l.tables = take((size_t)rows * keep * sizeof(int));
+    l.lens = take((size_t)rows * sizeof(int));
+    l.part_bytes = q4 ? nxt_paged_attention_q4_workspace_size((int)rows, GS, D, 1, keep, bs)
+                      : nxt_paged_attention_workspace_size((int)rows, GS, D, 1, keep, bs, ds);
+    l.part = take(l.part_bytes);
+  }
+  l.total = at;
+  return l;
+}
+
+int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, size_t ws_bytes,
+                int* dev_status, cudaStream_t st) {
+  const bool attention = c.out || c.k;
+  int rc;
+  if (attention) {
+    rc = check_args(c.out, c.q, c.k, c.v, c.bt, c.sl, c.B, c.Hq, c.D, c.Hkv, c.max_blocks, c.bs,
+                    c.ds, c.kbs, c.khs);
+  } else {
+    rc = check_args(c.q, c.q, c.q, c.q, c.bt, c.sl, c.B, c.Hq, c.D, c.Hkv, c.max_blocks, c.bs,
+                    c.ds, c.kbs, c.khs);
+    if (rc == NXT_PA_OK && c.B > 0 && (!sel_tables || !sel_lens)) rc = NXT_PA_EINVAL;
+  }
+  if (rc != NXT_PA_OK || c.B == 0) return rc;
+  if (!c.bounds || !aligned(c.bounds, c.ds) || !aligned(c.q, c.ds)) return NXT_PA_EINVAL;
+  if (c.sink < 0 || c.recent < 1 || c.keep < 1 || (long long)c.sink + c.recent > c.keep ||
+      (long long)c.keep * c.bs > INT_MAX)
+    return NXT_PA_EINVAL;
+  if (std::isnan(c.scale)) return NXT_PA_EINVAL;
+  if (c.Hkv > 1 && (c.khs <= 0 || c.kbs % c.khs || c.kbs / c.khs < c.Hkv)) return NXT_PA_EINVAL;
+  if (c.q4 && (c.D % 16 || c.bs % 16 || !(c.k_scale > 0.f) || !(c.v_scale > 0.f) ||
+               !std::isfinite(c.k_scale) || !std::isfinite(c.v_scale) || !aligned(c.k, 16) ||
+               !aligned(c.v, 16) || c.kbs % 16 || c.khs % 16 || !aligned(c.out, 2)))
+    return NXT_PA_EINVAL;
+  if (ws && !workspace_aligned(ws)) return NXT_PA_EINVAL;
+  const long long rows = (long long)c.B * c.Hkv;
+  const int GS = c.Hq / c.Hkv;
+  if (rows * ceil_div(c.max_blocks, xpa::kScoreChunk) > INT_MAX || rows * GS > INT_MAX ||
+      rows * c.keep > INT_MAX)
+    return NXT_PA_EINVAL;
+  const long long head_pages = c.Hkv > 1 ? c.kbs / c.khs : 1;
+  const int64_t page_stride = c.Hkv > 1 ? c.khs : c.kbs;
+
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return NXT_PA_ECUDA;
+  int* status = dev_status;
+  if (!status) {
+    rc = status_word(dev, &status);
+    if (rc != NXT_PA_OK) return rc;
+  }
+  const Layout l =
+      layout_of(rows, GS, c.D, c.max_blocks, c.bs, c.ds, c.keep, c.q4, attention);
+  std::unique_lock<std::mutex> lk;
+  if (ws) {
+    if (ws_bytes < l.total) return NXT_PA_EWORKSPACE;
+  } else if (l.total > 0) {
+    rc = acquire_scratch(dev, st, l.total, &ws, lk);
+    if (rc != NXT_PA_OK) return rc;
+  }
+  char* base = static_cast<char*>(ws);
+  xpa::SelectParams p{};
+  p.q = c.q;
+  p.bounds = c.bounds;
+  p.block_tables = c.bt;
+  p.seq_lens = c.sl;
+  p.status = status;
+  p.sel_tables = attention ? reinterpret_cast<int*>(base + l.tables) : sel_tables;
+  p.sel_lens = attention ? reinterpret_cast<int*>(base + l.lens) : sel_lens;
+  p.sel_pages = c.sel_pages;
+  p.keys = reinterpret_cast<unsigned*>(base + l.keys);
+  p.absmax = reinterpret_cast<float*>(base + l.absmax);
+  p.near_page = reinterpret_cast<unsigned*>(base + l.near_page);
+  p.near_key = reinterpret_cast<unsigned long long*>(base + l.near_key);
+  p.num_blocks = c.num_blocks;
+  p.head_pages = head_pages;
+  p.B = c.B;
+  p.Hq = c.Hq;
+  p.Hkv = c.Hkv;
+  p.D = c.D;
+  p.GS = GS;
+  p.max_blocks = c.max_blocks;
+  p.block_size = c.bs;
+  p.keep = c.keep;
+  p.sink = c.sink;
+  p.recent = c.recent;
+  p.chunks = l.chunks;
+  p.sign = c.scale > 0.f ? 1.f : c.scale < 0.f ? -1.f : 0.f;
+  p.vec = c.ds == 2 && c.D % 8 == 0 && aligned(c.q, 16) && aligned(c.bounds, 16);
+  const cudaError_t e = xpa::launch_select(p, c.ds, st);
+  if (e != cudaSuccess) return map_cuda(e);
+  if (!attention) return NXT_PA_OK;
+
+  int64_t nb = c.num_blocks > 0 ? c.num_blocks : -1;
+  if (nb > 0) nb = nb > INT_MAX / head_pages ? INT_MAX : nb * head_pages;
+  void* part = l.part_bytes ? base + l.part : nullptr;
+  if (c.q4)
+    return nxt_paged_attention_q4_ex(c.out, c.q, c.k, c.v, p.sel_tables, p.sel_lens, (int)rows,
+                                     GS, c.D, 1, c.scale, c.keep, c.bs, c.k_scale,
+                                     c.v_scale, page_stride, c.khs, nb, part, l.part_bytes, status,
+                                     st);
+  return nxt_paged_attention_ex(c.out, c.q, c.k, c.v, p.sel_tables, p.sel_lens, (int)rows, GS, c.D,
+                                1, c.scale, c.keep, c.bs, c.ds, page_stride, c.khs, nb, part,
+                                l.part_bytes, status, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int nxt_page_bounds(void* bounds, const void* key_cache, const int* block_tables,
+                    const int* seq_lens, int num_seqs, int num_kv_heads, int head_size,
+                    int max_num_blocks_per_seq, int block_size, int dtype_size,
+                    int64_t kv_block_stride, int64_t kv_head_stride, int64_t num_blocks,
+                    int num_new_tokens, int* device_status, nxt_stream_t stream) {
+  if (dtype_size != 2 && dtype_size != 4) return NXT_PA_EINVAL;
+  return bounds_call(bounds, key_cache, block_tables, seq_lens, num_seqs, num_kv_heads, head_size,
+                     max_num_blocks_per_seq, block_size,
+                     dtype_size == 4 ? xpa::kBoundsF32 : xpa::kBoundsF16, 1.f, kv_block_stride,
+                     kv_head_stride, num_blocks, num_new_tokens, device_status,
+                     static_cast<cudaStream_t>(stream));
+}
+
+int nxt_page_bounds_q4(void* bounds, const void* key_cache, const int* block_tables,
+                       const int* seq_lens, int num_seqs, int num_kv_heads, int head_size,
+                       int max_num_blocks_per_seq, int block_size, float k_scale,
+                       int64_t kv_block_stride, int64_t kv_head_stride, int64_t num_blocks,
+                       int num_new_tokens, int* device_status, nxt_stream_t stream) {
+  return bounds_call(bounds, key_cache, block_tables, seq_lens, num_seqs, num_kv_heads, head_size,
+                     max_num_blocks_per_seq, block_size, xpa::kBoundsQ4, k_scale, kv_block_stride,
+                     kv_head_stride, num_blocks, num_new_tokens, device_status,
+                     static_cast<cudaStream_t>(stream));
+}
+
+int nxt_select_pages(int* sel_tables, int* sel_lens, int* sel_pages, const void* query,
+                     const void* bounds, const int* block_tables, const int* seq_lens,
+                     int num_seqs, int num_heads, int head_size, int num_kv_heads, float scale,
+                     int max_num_blocks_per_seq, int block_size, int dtype_size,
+                     int64_t kv_block_stride, int64_t kv_head_stride, int64_t num_blocks,
+                     int max_pages, int sink_pages, int recent_pages, void* workspace,
+                     size_t workspace_bytes, int* device_status, nxt_stream_t stream) {
+  SparseCall c{query, bounds, block_tables, seq_lens, sel_pages, num_seqs, num_heads, head_size,
+               num_kv_heads, scale, max_num_blocks_per_seq, block_size, dtype_size,
+               kv_block_stride, kv_head_stride, num_blocks, max_pages, sink_pages, recent_pages};
+  return sparse_call(c, sel_tables, sel_lens, workspace, workspace_bytes, device_status,
+                     static_cast<cudaStream_t>(stream));
+}
+
+int nxt_paged_attention_sparse_ex(void* out, const void* query, const void* key_cache,
+                                  const void* value_cache, const void* bounds,
+                                  const int* block_tables, const int* seq_lens, int* sel_pages,
+                                  int num_seqs, int num_heads, int head_size, int num_kv_heads,
+                                  float scale, int max_num_blocks_per_seq, int block_size,
+                                  int dtype_size, int64_t kv_block_stride, int64_t kv_head_stride,
+                                  int64_t num_blocks, int max_pages, int sink_pages,
+                                  int recent_pages, void* workspace, size_t workspace_bytes,
+                                  int* device_status, nxt_stream_t stream) {
+  SparseCall c{query, bounds, block_tables, seq_lens, sel_pages, num_seqs, num_heads, head_size,
+               num_kv_heads, scale, max_num_blocks_per_seq, block_size, dtype_size,
+               kv_block_stride, kv_head_stride, num_blocks, max_pages, sink_pages, recent_pages,
+               out, key_cache, value_cache};
+  if (num_seqs > 0 && (!out || !key_cache || !value_cache)) return NXT_PA_EINVAL;
+  return sparse_call(c, nullptr, nullptr, workspace, workspace_bytes, device_status,
+                     static_cast<cudaStream_t>(stream));
+}
+
+int nxt_paged_attention_q4_sparse_ex(void* out, const void* query, const void* key_cache,
+                                     const void* value_cache, const void* bounds,
+                                     const int* block_tables, const int* seq_lens, int* sel_pages,
+                                     int num_seqs, int num_heads, int head_size, int num_kv_heads,
+                                     float scale, int max_num_blocks_per_seq, int block_size,
+                                     float k_scale, float v_scale, int64_t kv_block_stride,
+                                     int64_t kv_head_stride, int64_t num_blocks, int max_pages,
+                                     int sink_pages, int recent_pages, void* workspace,
+                                     size_t workspace_bytes, int* device_status,
+                                     nxt_stream_t stream) {
+  SparseCall c{query, bounds, block_tables, seq_lens, sel_pages, num_seqs, num_heads, head_size,
+               num_kv_heads, scale, max_num_blocks_per_seq, block_size, 2, kv_block_stride,
+               kv_head_stride, num_blocks, max_pages, sink_pages, recent_pages, out, key_cache,
+               value_cache, true, k_scale, v_scale};
+  if (num_seqs > 0 && (!out || !key_cache || !value_cache)) return NXT_PA_EINVAL;
+  return sparse_call(c, nullptr, nullptr, workspace, workspace_bytes, device_status,
+                     static_cast<cudaStream_t>(stream));
+}
+
+size_t nxt_paged_attention_sparse_workspace_size(int num_seqs, int num_heads, int head_size,
+                                                 int num_kv_heads, int max_num_blocks_per_seq,
+                                                 int block_size, int dtype_size, int max_pages) {
+  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_size <= 0 || block_size <= 0 ||
+      max_pages <= 0 || max_num_blocks_per_seq < 0)
+    return 0;
+  const long long rows = (long long)num_seqs * num_kv_heads;
+  if (rows > INT_MAX) return 0;
+  const int GS = num_heads / num_kv_heads;
+  const size_t plain = layout_of(rows, GS, head_size, max_num_blocks_per_seq, block_size,
+                                 dtype_size, max_pages, false, true)
+                           .total;
+  const size_t q4 = layout_of(rows, GS, head_size, max_num_blocks_per_seq, block_size, dtype_size,
+                              max_pages, true, true)
+                        .total;
+  return plain > q4 ? plain : q4;
+}
+
+}  // extern "C"

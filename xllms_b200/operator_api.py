@@ -744,6 +744,147 @@ def paged_attention_q4_append(query, key_cache, value_cache, block_tables, seq_l
     return out
 
 
+# ── page bounds and sparse attention ───────────────────────────────────────
+def _check_bounds(bad, bounds, num_blocks, hkv, d, dtype, like):
+    if (tuple(bounds.shape) != (num_blocks, hkv, 2, d) or bounds.dtype != dtype
+            or not bounds.is_contiguous() or bounds.device != like.device):
+        bad("bounds must be contiguous [num_blocks, Hkv, 2, D] beside the pools")
+
+
+def page_bounds(key_cache, block_tables, seq_lens, bounds, *, num_new_tokens=0, k_scale=None,
+                num_blocks=None, device_status=None, stream=None):
+    """Writes into `bounds` [num_blocks, Hkv, 2, D] the lowest and highest key
+    per channel of the pages that hold the last num_new_tokens tokens of each
+    sequence (0: of all its pages), over their valid tokens. key_cache is an
+    fp16 or fp32 pool [num_blocks, Hkv, P, D] (bounds of its type) or, with
+    k_scale, a 4-bit pool (q4_pool_shape; bounds fp16). Returns `bounds`."""
+    import torch
+
+    def bad(msg):
+        raise PagedAttentionError(_native.NXT_PA_EINVAL, f"page_bounds: {msg}")
+    if not key_cache.is_cuda or key_cache.dim() != 4 or not key_cache.is_contiguous():
+        bad("the pool must be a contiguous 4-D CUDA tensor")
+    if seq_lens.dim() != 1:
+        bad("seq_lens must be int32 [B]")
+    if k_scale is None:
+        ds = _dtype_size(key_cache)
+        nb, hkv, bs, d = key_cache.shape
+        strides, dtype, kind = (hkv * bs * d, bs * d), key_cache.dtype, ds
+    else:
+        nb, hkv, bs, d = _check_q4_pools("page_bounds", key_cache, key_cache, key_cache)
+        strides, dtype, kind = _q4_strides(hkv, bs, d), torch.float16, float(k_scale)
+    _check_bounds(bad, bounds, nb, hkv, d, dtype, key_cache)
+    B = seq_lens.numel()
+    if (block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] < B
+            or seq_lens.dtype != torch.int32 or not block_tables.is_contiguous()
+            or not seq_lens.is_contiguous() or block_tables.device != key_cache.device
+            or seq_lens.device != key_cache.device):
+        bad("block_tables must be int32 [B, max_blocks] and seq_lens int32 [B], beside the pool")
+    name = "nxt_page_bounds" if k_scale is None else "nxt_page_bounds_q4"
+    with _launching(key_cache, stream) as st:
+        rc = getattr(_native.xpa(), name)(
+            _ptr(bounds), _ptr(key_cache), _ptr(block_tables), _ptr(seq_lens), B, hkv, d,
+            block_tables.shape[1], bs, kind, *strides,
+            nb if num_blocks is None else int(num_blocks), int(num_new_tokens),
+            _ptr(device_status), st)
+    if rc != _native.NXT_PA_OK:
+        raise PagedAttentionError(rc, name)
+    return bounds
+
+
+def _check_sparse(where, query, key_cache, value_cache, bounds, block_tables, seq_lens, out,
+                  selected, max_pages, q4):
+    """(num_blocks, Hkv, page size, strides) of a sparse call's pools."""
+    import torch
+
+    def bad(msg):
+        raise PagedAttentionError(_native.NXT_PA_EINVAL, f"{where}: {msg}")
+    if q4:
+        nb, hkv, bs, d = _check_q4_attention(where, query, key_cache, value_cache, block_tables,
+                                             seq_lens, out)
+        strides = _q4_strides(hkv, bs, d)
+    else:
+        _check_attention_inputs(where, query, key_cache, value_cache, block_tables, seq_lens, out)
+        nb, hkv, bs, d = key_cache.shape
+        strides = (hkv * bs * d, bs * d)
+    _check_bounds(bad, bounds, nb, hkv, d, query.dtype, query)
+    if selected is not None and (
+            selected.dtype != torch.int32 or not selected.is_contiguous()
+            or tuple(selected.shape) != (query.shape[0], hkv, max_pages)
+            or selected.device != query.device):
+        bad("selected must be contiguous int32 [B, Hkv, max_pages] on the query's device")
+    return nb, hkv, bs, strides
+
+
+def select_pages(query, key_cache, bounds, block_tables, seq_lens, max_pages, *, sink_pages=0,
+                 recent_pages=1, scale=None, num_blocks=None, device_status=None, stream=None):
+    """The pages that sparse attention keeps: (tables int32 [B * Hkv,
+    max_pages], lens int32 [B * Hkv], pages int32 [B, Hkv, max_pages]). With
+    key_cache.view(NB * Hkv, 1, P, D), query.view(B * Hkv, G, D), tables and
+    lens are the inputs of any attention call over the pool."""
+    import torch
+    nb, hkv, bs, strides = _check_sparse("select_pages", query, key_cache, key_cache, bounds,
+                                         block_tables, seq_lens, None, None, max_pages, False)
+    B, Hq, d = query.shape
+    with _launching(query, stream) as st:
+        new = lambda *s: torch.empty(s, dtype=torch.int32, device=query.device)
+        tables, lens = new(B * hkv, int(max_pages)), new(B * hkv)
+        pages = new(B, hkv, int(max_pages))
+        rc = _native.xpa().nxt_select_pages(
+            _ptr(tables), _ptr(lens), _ptr(pages), _ptr(query), _ptr(bounds), _ptr(block_tables),
+            _ptr(seq_lens), B, Hq, d, hkv, 1.0 / math.sqrt(d) if scale is None else float(scale),
+            block_tables.shape[1], bs, _dtype_size(query), *strides,
+            nb if num_blocks is None else int(num_blocks), int(max_pages), int(sink_pages),
+            int(recent_pages), None, 0, _ptr(device_status), st)
+    if rc != _native.NXT_PA_OK:
+        raise PagedAttentionError(rc, "nxt_select_pages")
+    return tables, lens, pages
+
+
+def paged_attention_sparse(query, key_cache, value_cache, bounds, block_tables, seq_lens,
+                           max_pages, *, sink_pages=0, recent_pages=1, k_scale=None, v_scale=None,
+                           scale=None, out=None, selected=None, num_blocks=None, workspace=None,
+                           device_status=None, stream=None):
+    """Decode attention over at most max_pages pages per sequence and KV head:
+    the first sink_pages, the last recent_pages and the best of the others by
+    their bounds (page_bounds). Pools as for paged_attention, or 4-bit ones
+    with k_scale and v_scale. ``selected`` (int32 [B, Hkv, max_pages]) receives
+    the kept pages' indices within each sequence, -1 past the last."""
+    import torch
+    q4 = k_scale is not None
+    if q4 != (v_scale is not None):
+        raise PagedAttentionError(_native.NXT_PA_EINVAL,
+                                  "paged_attention_sparse: k_scale and v_scale go together")
+    nb, hkv, bs, strides = _check_sparse(
+        "paged_attention_sparse", query, key_cache, value_cache, bounds, block_tables, seq_lens,
+        out, selected, max_pages, q4)
+    B, Hq, d = query.shape
+    name = "nxt_paged_attention_q4_sparse_ex" if q4 else "nxt_paged_attention_sparse_ex"
+    kind = (float(k_scale), float(v_scale)) if q4 else (_dtype_size(query),)
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    with _launching(query, stream) as st:
+        if out is None:
+            out = torch.empty_like(query)
+        rc = getattr(_native.xpa(), name)(
+            _ptr(out), _ptr(query), _ptr(key_cache), _ptr(value_cache), _ptr(bounds),
+            _ptr(block_tables), _ptr(seq_lens), _ptr(selected), B, Hq, d, hkv,
+            1.0 / math.sqrt(d) if scale is None else float(scale), block_tables.shape[1], bs,
+            *kind, *strides, nb if num_blocks is None else int(num_blocks), int(max_pages),
+            int(sink_pages), int(recent_pages), _ptr(workspace), ws_bytes, _ptr(device_status),
+            st)
+    if rc != _native.NXT_PA_OK:
+        raise PagedAttentionError(rc, name)
+    return out
+
+
+def sparse_workspace_size(num_seqs, num_heads, head_size, num_kv_heads, max_num_blocks_per_seq,
+                          max_pages, block_size=16, dtype_size=2) -> int:
+    """Workspace bytes of a paged_attention_sparse call on the current device."""
+    return int(_native.xpa().nxt_paged_attention_sparse_workspace_size(
+        num_seqs, num_heads, head_size, num_kv_heads, max_num_blocks_per_seq, block_size,
+        dtype_size, max_pages))
+
+
 # ── block-table builder ────────────────────────────────────────────────────
 class BlockTables:
     """One decode step's kernel inputs on the device, built by
