@@ -322,8 +322,8 @@ int nxt_paged_attention_fp8_append_ex(
  *   code  = E2M1(t / scale), nearest even, at most 6 (0 when scale is 0).
  * head_size is a multiple of 16 up to 256, block_size a multiple of 16.
  * Pools are bytes: page p of KV head h starts at p * kv_block_stride +
- * h * kv_head_stride (strides in bytes, multiples of 16; pools start on
- * 16-byte boundaries) and holds block_size / 16 tiles of 9 * head_size bytes,
+ * h * kv_head_stride (strides in bytes, multiples of 16, kv_block_stride
+ * below 2^31; pools start on 16-byte boundaries) and holds block_size / 16 tiles of 9 * head_size bytes,
  * one per 16 tokens:
  *   K: 16 rows of head_size / 2 code bytes, then scales [16][head_size / 16];
  *      a row is, for t = 0..3, for j = 0..head_size / 16 - 1, the codes of

@@ -1,6 +1,6 @@
 // pa_q4.cu — 4-bit KV cache: rows written and read back by slot, and paged
 // decode attention over it. Format and tile layout: pa_q4.cuh.
-#include <algorithm>
+#include <type_traits>
 #include <utility>
 
 #include "pa_q4.cuh"
@@ -184,112 +184,164 @@ struct Q4Cfg {
   static constexpr size_t kSmem = kRingBytes > kMergeBytes ? kRingBytes : kMergeBytes;
 };
 
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t r;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(a));
-  return r;
-}
+// Shared-memory reads and copies at compile-time offsets from one register.
+template <int OFF>
 __device__ __forceinline__ uint32_t lds16(uint32_t a) {
   uint16_t r;
-  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(r) : "r"(a));
+  asm volatile("ld.shared.b16 %0, [%1+%2];" : "=h"(r) : "r"(a), "n"(OFF));
   return r;
 }
+template <int OFF>
 __device__ __forceinline__ uint32_t lds8(uint32_t a) {
   uint32_t r;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(r) : "r"(a));
+  asm volatile("ld.shared.u8 %0, [%1+%2];" : "=r"(r) : "r"(a), "n"(OFF));
   return r;
 }
-template <int N>
+template <int N, int OFF>
 __device__ __forceinline__ void lds_words(uint32_t a, uint32_t* r) {
   if constexpr (N == 1) {
-    r[0] = lds32(a);
+    asm volatile("ld.shared.b32 %0, [%1+%2];" : "=r"(r[0]) : "r"(a), "n"(OFF));
   } else if constexpr (N == 2) {
-    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(a));
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2+%3];"
+                 : "=r"(r[0]), "=r"(r[1])
+                 : "r"(a), "n"(OFF));
   } else {
     static_assert(N == 4, "1, 2 or 4 words");
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4+%5];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(a));
+                 : "r"(a), "n"(OFF));
   }
 }
+template <int DST, int SRC>
+__device__ __forceinline__ void cp_async16_at(uint32_t dst, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0+%2], [%1+%3], 16;" ::"r"(dst), "l"(src), "n"(DST),
+               "n"(SRC)
+               : "memory");
+}
 
-// Where a tile's pieces sit in a ring stage, and one lane's reads of them.
+// Where a tile's pieces sit in a ring stage, and one lane's copies and reads
+// of them; S0 is the stage's byte offset in the warp's ring.
 // EXACT (D = 64 W, W = 1, 2, 4): rows are placed and chunks swizzled so that
 // every read below is conflict-free; K row r's place is its S^T row, V row
 // 4 t + k's place is 4 k + t. Otherwise a tile is copied as it is.
 template <int W, bool EXACT>
 struct Q4Stage {
-  int D;            // head size
-  int lane, g, t;
-  uint32_t kd[W], vd[W];  // EXACT: this lane's copy destinations in a stage
+  static constexpr int DD = 64 * W;
+  int D, lane, g, t;
+  // sources in page 0; EXACT: this lane's first chunk of each piece
+  const uint8_t *ksrc, *vsrc, *ssrc;
+  uint32_t ring;               // the warp's ring
+  uint32_t kd, sd, vd[W];      // EXACT: copy destinations in stage 0
+  uint32_t ka[2], ksa, va, vsa;  // read addresses in stage 0
 
-  __device__ __forceinline__ Q4Stage(int D_, int lane_) : D(D_), lane(lane_) {
+  __device__ __forceinline__ Q4Stage(int D_, int lane_, const uint8_t* k, const uint8_t* v,
+                                     uint32_t ring_)
+      : D(D_), lane(lane_), ksrc(k), vsrc(v), ssrc(k), ring(ring_) {
     g = lane >> 2;
     t = lane & 3;
+    const int tok = 4 * (g >> 1) + (g & 1);  // sigma(g); sigma(g + 8) is + 2
     if constexpr (EXACT) {
       constexpr int CPR = 2 * W;  // 16-byte chunks per row
+      ksrc = k + lane * 16;
+      vsrc = v + lane * 16;
+      // both tiles' scales: D / 16 chunks each, lanes 0.. and 16..
+      const int sc = lane & 15;
+      ssrc = (lane < 16 ? k : v) + 8 * DD + sc * 16;
+      sd = ring + 16 * DD + (lane >> 4) * DD + sc * 16;
 #pragma unroll
-      for (int k = 0; k < W; ++k) {
-        const int x = lane + 32 * k, r = x / CPR, c = x % CPR;
+      for (int i = 0; i < W; ++i) {
+        const int x = lane + 32 * i, r = x / CPR, c = x % CPR;
         const int kp = 2 * (r >> 2) + (r & 1) + 8 * ((r >> 1) & 1);
         const int vp = 4 * (r & 3) + (r >> 2);
         int ck = c, cv = c;
         if (W == 4) ck = c ^ (kp & 1);
         if (W == 2) cv = c ^ (2 * ((vp >> 1) & 1));
         if (W == 4) cv = c ^ (2 * (vp & 3));
-        kd[k] = (uint32_t)(kp * 32 * W + ck * 16);
-        vd[k] = (uint32_t)(8 * 64 * W + vp * 32 * W + cv * 16);
+        // 32 chunks further on is a whole number of token groups: the K place
+        // moves by a constant
+        if (i == 0) kd = ring + (uint32_t)(kp * 32 * W + ck * 16);
+        vd[i] = ring + (uint32_t)(8 * DD + vp * 32 * W + cv * 16);
       }
+      const uint32_t row = ring + g * 32 * W;
+      ka[0] = ka[1] = row + t * 8 * W;
+      if (W == 4) {
+        ka[0] = row + (((2 * t) ^ (g & 1)) << 4);
+        ka[1] = row + (((2 * t + 1) ^ (g & 1)) << 4);
+      }
+      ksa = ring + 16 * DD + tok * 4 * W;
+      va = ring + 8 * DD + t * 32 * W;
+      if (W == 1) va += 4 * g;
+      if (W == 2) va += (((g >> 1) ^ (t & 2)) << 4) + (g & 1) * 8;
+      if (W == 4) va += (g ^ (2 * t)) << 4;
+      vsa = ring + 17 * DD + 4 * t + (g * W >> 1) * 16;
+    } else {
+      ka[0] = ka[1] = ring + tok * (D / 2) + t * (D / 8);
+      ksa = ring + 8 * D + tok * (D / 16);
+      va = ring + 9 * D;
+      vsa = ring + 17 * D + 4 * t;
     }
   }
 
-  // Issues the copies of one K and one V tile into the stage at `st`.
-  __device__ __forceinline__ void copy(uint32_t st, const uint8_t* k, const uint8_t* v) const {
+  // Issues the copies of the K and V tiles of page e, `sub` bytes into it.
+  template <int S0>
+  __device__ __forceinline__ void copy(int e, int page_bytes, int sub) const {
     if constexpr (EXACT) {
-      constexpr int DD = 64 * W;
-#pragma unroll
-      for (int i = 0; i < W; ++i) cp_async16(st + kd[i], k + (lane + 32 * i) * 16);
-#pragma unroll
-      for (int i = 0; i < W; ++i) cp_async16(st + vd[i], v + (lane + 32 * i) * 16);
-      // both tiles' scales: D / 16 chunks each, lanes 0.. and 16..
-      const int c = lane & 15;
-      if (c < 4 * W)
-        cp_async16(st + 16 * DD + (lane >> 4) * DD + c * 16,
-                   (lane < 16 ? k : v) + 8 * DD + c * 16);
+      // rows per 32 chunks: 16 / W; their K places are 2 * (16 / W) / 4 apart
+      constexpr int kStep = W == 1 ? 0 : (16 / W / 4) * 2 * 32 * W;
+      const uint8_t* k = ksrc + (long long)e * page_bytes + sub;
+      const uint8_t* v = vsrc + (long long)e * page_bytes + sub;
+      const uint8_t* s = ssrc + (long long)e * page_bytes + sub;
+      cp_async16_at<S0, 0>(kd, k);
+      if constexpr (W >= 2) cp_async16_at<S0 + kStep, 512>(kd, k);
+      if constexpr (W == 4) {
+        cp_async16_at<S0 + 2 * kStep, 1024>(kd, k);
+        cp_async16_at<S0 + 3 * kStep, 1536>(kd, k);
+      }
+      cp_async16_at<S0, 0>(vd[0], v);
+      if constexpr (W >= 2) cp_async16_at<S0, 512>(vd[1], v);
+      if constexpr (W == 4) {
+        cp_async16_at<S0, 1024>(vd[2], v);
+        cp_async16_at<S0, 1536>(vd[3], v);
+      }
+      if (W == 4 || (lane & 15) < 4 * W) cp_async16_at<S0, 0>(sd, s);
     } else {
+      const long long off = (long long)e * page_bytes + sub;
       const int n = 9 * D / 16;
       for (int x = lane; x < n; x += 32) {
-        cp_async16(st + x * 16, k + x * 16);
-        cp_async16(st + 9 * D + x * 16, v + x * 16);
+        cp_async16_at<S0, 0>(ring + x * 16, ksrc + off + x * 16);
+        cp_async16_at<S0, 0>(ring + 9 * D + x * 16, vsrc + off + x * 16);
       }
     }
   }
 
   // K codes and scales of S^T rows g (r = 0) and g + 8 (r = 1): word i of kw
   // is groups 2 i, 2 i + 1; byte j of ks is group j's scale.
-  __device__ __forceinline__ void load_k(uint32_t st, uint32_t (&kw)[2][2 * W],
-                                         uint32_t (&ks)[2][W]) const {
-    const int tok = 4 * (g >> 1) + (g & 1);  // sigma(g); sigma(g + 8) is + 2
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      if constexpr (EXACT) {
-        const uint32_t row = st + (g + 8 * r) * 32 * W;
-        if constexpr (W == 1) lds_words<2>(row + t * 8, kw[r]);
-        if constexpr (W == 2) lds_words<4>(row + t * 16, kw[r]);
-        if constexpr (W == 4) {
-          lds_words<4>(row + (((2 * t) ^ (g & 1)) << 4), kw[r]);
-          lds_words<4>(row + (((2 * t + 1) ^ (g & 1)) << 4), kw[r] + 4);
-        }
-        lds_words<W>(st + 16 * 64 * W + (tok + 2 * r) * 4 * W, ks[r]);
+  template <int S0>
+  __device__ __forceinline__ void load_k(uint32_t (&kw)[2][2 * W], uint32_t (&ks)[2][W]) const {
+    if constexpr (EXACT) {
+      constexpr int kRows = 8 * 32 * W;
+      if constexpr (W == 4) {
+        lds_words<4, S0>(ka[0], kw[0]);
+        lds_words<4, S0>(ka[1], kw[0] + 4);
+        lds_words<4, S0 + kRows>(ka[0], kw[1]);
+        lds_words<4, S0 + kRows>(ka[1], kw[1] + 4);
       } else {
-        const int NG = D / 16;
-        const uint32_t row = st + (tok + 2 * r) * (D / 2) + t * (2 * NG);
-        const uint32_t sc = st + 8 * D + (tok + 2 * r) * NG;
+        lds_words<2 * W, S0>(ka[0], kw[0]);
+        lds_words<2 * W, S0 + kRows>(ka[0], kw[1]);
+      }
+      lds_words<W, S0>(ksa, ks[0]);
+      lds_words<W, S0 + 8 * W>(ksa, ks[1]);
+    } else {
+      const int NG = D / 16;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t row = ka[0] + 2 * r * (D / 2);
+        const uint32_t sc = ksa + 2 * r * NG;
 #pragma unroll
         for (int i = 0; i < 2 * W; ++i) {
           uint32_t lo = 0, hi = 0;
-          if (2 * i < NG) lo = lds16(row + 4 * i);
-          if (2 * i + 1 < NG) hi = lds16(row + 4 * i + 2);
+          if (2 * i < NG) lo = lds16<S0>(row + 4 * i);
+          if (2 * i + 1 < NG) hi = lds16<S0>(row + 4 * i + 2);
           kw[r][i] = lo | (hi << 16);
         }
 #pragma unroll
@@ -297,7 +349,7 @@ struct Q4Stage {
           uint32_t s = 0;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (4 * i + j < NG) s |= lds8(sc + 4 * i + j) << (8 * j);
+            if (4 * i + j < NG) s |= lds8<S0>(sc + 4 * i + j) << (8 * j);
           ks[r][i] = s;
         }
       }
@@ -306,39 +358,58 @@ struct Q4Stage {
 
   // V codes of tokens 4 t + k: word w is channels 8 (g W + w) .. + 7; vs[w]
   // holds the four tokens' scales of those channels.
-  __device__ __forceinline__ void load_v(uint32_t st, uint32_t (&vw)[4][W],
-                                         uint32_t (&vs)[W]) const {
+  template <int S0>
+  __device__ __forceinline__ void load_v(uint32_t (&vw)[4][W], uint32_t (&vs)[W]) const {
     if constexpr (EXACT) {
-      const uint32_t base = st + 8 * 64 * W;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t row = base + (4 * k + t) * 32 * W;
-        if constexpr (W == 1) lds_words<1>(row + 4 * g, vw[k]);
-        if constexpr (W == 2)
-          lds_words<2>(row + (((g >> 1) ^ (t & 2)) << 4) + (g & 1) * 8, vw[k]);
-        if constexpr (W == 4) lds_words<4>(row + ((g ^ (2 * t)) << 4), vw[k]);
-      }
-      const uint32_t sc = st + 17 * 64 * W + 4 * t;
-      if constexpr (W == 1) vs[0] = lds32(sc + (g >> 1) * 16);
-      if constexpr (W == 2) vs[0] = vs[1] = lds32(sc + g * 16);
+      constexpr int kRows = 4 * 32 * W;
+      lds_words<W, S0>(va, vw[0]);
+      lds_words<W, S0 + kRows>(va, vw[1]);
+      lds_words<W, S0 + 2 * kRows>(va, vw[2]);
+      lds_words<W, S0 + 3 * kRows>(va, vw[3]);
+      lds_words<1, S0>(vsa, vs);
+      if constexpr (W == 2) vs[1] = vs[0];
       if constexpr (W == 4) {
-        vs[0] = vs[1] = lds32(sc + 2 * g * 16);
-        vs[2] = vs[3] = lds32(sc + (2 * g + 1) * 16);
+        vs[1] = vs[0];
+        lds_words<1, S0 + 16>(vsa, vs + 2);
+        vs[3] = vs[2];
       }
     } else {
-      const uint32_t base = st + 9 * D;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         const int at = g * W + w;
         const bool in = at < D / 8;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          vw[k][w] = in ? lds32(base + (4 * t + k) * (D / 2) + at * 4) : 0u;
-        vs[w] = in ? lds32(base + 8 * D + (at >> 1) * 16 + 4 * t) : 0u;
+        for (int k = 0; k < 4; ++k) {
+          vw[k][w] = 0u;
+          if (in) lds_words<1, S0>(va + (4 * t + k) * (D / 2) + at * 4, &vw[k][w]);
+        }
+        vs[w] = 0u;
+        if (in) lds_words<1, S0>(vsa + (at >> 1) * 16, &vs[w]);
       }
     }
   }
 };
+
+// f(0), f(1), ..., f(N - 1) with compile-time arguments, until one is false.
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ bool each_stage(F&& f) {
+  if constexpr (I < N) {
+    if (!f(std::integral_constant<int, I>{})) return false;
+    return each_stage<N, I + 1>(static_cast<F&&>(f));
+  }
+  return true;
+}
+
+// D = A . B, fp16 inputs, fp32 result.
+__device__ __forceinline__ void mma_f16_16816_zero(float (&d)[4], uint32_t a0, uint32_t a1,
+                                                   uint32_t a2, uint32_t a3, uint32_t b0,
+                                                   uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7},"
+      " {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 
 template <int W, int NT, bool EXACT, int NW, int STAGES, int MINB>
 __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
@@ -363,7 +434,12 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const Q4Stage<W, EXACT> sg(D, lane);
+
+  // Scores are handled as q . k times a positive factor: its sign goes into Q
+  // (a factor of 0 is a Q of 0).
+  const float sl = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+  const float sign = p.scale_log2 > 0.f ? 1.f : p.scale_log2 < 0.f ? -1.f : 0.f;
+  const float slack = fminf(kRaise / sl, 1e30f);  // kRaise in units of q . k
 
   // ── Q fragments: head g of tile nt, channels 16 j + 4 t .. + 3 ──────────
   uint32_t qf[4 * W][NT][2];
@@ -386,6 +462,10 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
             u.y = s[2] | ((uint32_t)s[3] << 16);
           }
         }
+        if (sign <= 0.f) {
+          u.x = h2_mul(u.x, pack_half2(sign, sign));
+          u.y = h2_mul(u.y, pack_half2(sign, sign));
+        }
         qf[j][nt][0] = u.x;
         qf[j][nt][1] = u.y;
       }
@@ -394,43 +474,48 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
 
   // ── this warp's tiles: j = warp, warp + NW, ... of the item ─────────────
   const int spp = p.block_size >> 4;  // tiles per page
+  const int page_bytes = (int)p.kv_block_stride;
   const long long tok_end = min((long long)it.L, (long long)it.page_end * p.block_size);
   const int tok_begin = it.page_begin * p.block_size;
   const int tiles = (int)((tok_end - tok_begin + 15) >> 4);
   const int n = tiles > warp ? (tiles - warp + NW - 1) / NW : 0;
-  const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + (long long)it.kvh * p.kv_head_stride;
-  const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + (long long)it.kvh * p.kv_head_stride;
+  const long long head_off = (long long)it.kvh * p.kv_head_stride;
+  const Q4Stage<W, EXACT> sg(D, lane, static_cast<const uint8_t*>(p.k) + head_off,
+                             static_cast<const uint8_t*>(p.v) + head_off,
+                             smem_u32(smem) + warp * (STAGES * C::kStageBytes));
   const int* table = p.block_tables + (long long)it.b * p.max_blocks + it.page_begin;
-  const uint32_t ring = smem_u32(smem) + warp * (STAGES * C::kStageBytes);
+  auto entry_ok = [&](int e) { return e >= 0 && (p.num_blocks <= 0 || e < p.num_blocks); };
 
-  long long ent = -1;   // lane l: pool offset of this warp's tile (i & ~31) + l, -1: none
-  uint32_t live = 0;    // bit s: stage s holds a tile to compute
-  auto issue = [&](int i, int s) {
+  int ent = -1, sub = 0;  // lane l: page and offset in it of tile (i & ~31) + l; -1: none
+  bool masked = false;    // a page of this warp's is masked
+  auto issue = [&](int i, auto stage) {
     if (i < n) {
       if ((i & 31) == 0) {
-        ent = -1;
+        bool bad = false;
         if (i + lane < n) {
           const int j = warp + (i + lane) * NW;
-          const int page = j / spp;
-          const int e = __ldg(table + page);
-          if (e < 0 || (p.num_blocks > 0 && e >= p.num_blocks))
+          const int page = spp == 1 ? j : j / spp;
+          sub = (j - page * spp) * (9 * D);
+          ent = __ldg(table + page);
+          bad = !entry_ok(ent);
+          if (bad) {
+            ent = -1;
             raise_status(p, kDevBadPage);
-          else
-            ent = (long long)e * p.kv_block_stride + (long long)(j - page * spp) * (9 * D);
+          }
         }
+        masked |= __any_sync(0xffffffffu, bad);
       }
-      const long long off = __shfl_sync(0xffffffffu, ent, i & 31);
-      live &= ~(1u << s);
-      if (off >= 0) {
-        live |= 1u << s;
-        sg.copy(ring + s * C::kStageBytes, kbase + off, vbase + off);
-      }
+      const int e = __shfl_sync(0xffffffffu, ent, i & 31);
+      const int in = spp > 1 ? __shfl_sync(0xffffffffu, sub, i & 31) : 0;
+      if (e >= 0) sg.template copy<decltype(stage)::value * C::kStageBytes>(e, page_bytes, in);
     }
     cp_async_commit();
   };
 
   float o[4 * W][NT][4] = {};
-  float m[NT][2], moff[NT][2], l[NT][2];  // heads 2 t, 2 t + 1 of each tile
+  // Heads 2 t, 2 t + 1 of each tile: the reference point m in units of q . k
+  // and the same less kShift in the exp2 domain, and the weights' sum.
+  float m[NT][2], moff[NT][2], l[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -440,61 +525,63 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
       l[nt][c] = 0.f;
     }
 
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) issue(s, s);
-  int stage = 0;
-  for (int i = 0; i < n; ++i) {
+  // One tile, the warp's i-th, from ring stage `stage`; false after the last.
+  int left = (int)(tok_end - tok_begin) - warp * 16;  // tokens from this tile on
+  auto step = [&](int i, auto stage) {
+    constexpr int S = decltype(stage)::value, S0 = S * C::kStageBytes;
+    if (i >= n) return false;
     cp_async_wait<STAGES - 2>();
-    __syncwarp();  // every lane's copies of this stage are in; the next one is free
-    const int prev = stage == 0 ? STAGES - 1 : stage - 1;
-    issue(i + STAGES - 1, prev);
-    const uint32_t st = ring + stage * C::kStageBytes;
-    const bool compute = (live >> stage) & 1u;
-    stage = stage + 1 == STAGES ? 0 : stage + 1;
-    if (!compute) continue;  // warp-uniform
-    // tokens of this tile, sigma(g) and sigma(g + 8) of this lane's S^T rows
-    const int left = (int)(tok_end - tok_begin) - (warp + i * NW) * 16;
+    __syncwarp();  // every lane's copies of this stage are in; the one before is free
+    issue(i + STAGES - 1, std::integral_constant<int, (S + STAGES - 1) % STAGES>{});
+    const int here = left;
+    left -= 16 * NW;
+    if (masked && !entry_ok(__ldg(table + (warp + i * NW) / spp))) return true;  // warp-uniform
 
-    // ── S^T = K . Q^T ─────────────────────────────────────────────────────
+    // ── S^T = K . Q^T, a channel group's scale applied to its sums ────────
     float x[NT][4] = {};
     {
       uint32_t kw[2][2 * W], ks[2][W];
-      sg.load_k(st, kw, ks);
+      sg.template load_k<S0>(kw, ks);
 #pragma unroll
       for (int i2 = 0; i2 < 2 * W; ++i2) {
         if (!EXACT && 2 * i2 >= NG) break;
         uint32_t a[2][4];
+        float2 sc[2];  // groups 2 i2 and 2 i2 + 1 of rows g and g + 8
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint32_t s2 = fp8x2_to_h2<kKvE4M3>(ks[r][i2 >> 1] >> (16 * (i2 & 1)));
-          const uint32_t sl = h2_low2(s2), sh = h2_high2(s2);
+          sc[r] = unpack_half2(fp8x2_to_h2<kKvE4M3>(ks[r][i2 >> 1] >> (16 * (i2 & 1))));
           q4x8_to_h2(kw[r][i2], a[r]);
-          a[r][0] = h2_mul(a[r][0], sl);
-          a[r][1] = h2_mul(a[r][1], sl);
-          a[r][2] = h2_mul(a[r][2], sh);
-          a[r][3] = h2_mul(a[r][3], sh);
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma_f16_16816(x[nt], a[0][0], a[1][0], a[0][1], a[1][1], qf[2 * i2][nt][0],
-                        qf[2 * i2][nt][1]);
-          mma_f16_16816(x[nt], a[0][2], a[1][2], a[0][3], a[1][3], qf[2 * i2 + 1][nt][0],
-                        qf[2 * i2 + 1][nt][1]);
+          float y[4], z[4];
+          mma_f16_16816_zero(y, a[0][0], a[1][0], a[0][1], a[1][1], qf[2 * i2][nt][0],
+                             qf[2 * i2][nt][1]);
+          mma_f16_16816_zero(z, a[0][2], a[1][2], a[0][3], a[1][3], qf[2 * i2 + 1][nt][0],
+                             qf[2 * i2 + 1][nt][1]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            x[nt][c] = fmaf(y[c], sc[c >> 1].x, x[nt][c]);
+            x[nt][c] = fmaf(z[c], sc[c >> 1].y, x[nt][c]);
+          }
         }
       }
     }
 
     // ── softmax step ──────────────────────────────────────────────────────
-    const int tok = 4 * (g >> 1) + (g & 1);
-    const bool v0 = tok < left, v1 = tok + 2 < left;
+    if (here < 16) {  // tokens sigma(g) and sigma(g + 8) of the last tile
+      const int tok = 4 * (g >> 1) + (g & 1);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (tok >= here) x[nt][0] = x[nt][1] = -INFINITY;
+        if (tok + 2 >= here) x[nt][2] = x[nt][3] = -INFINITY;
+      }
+    }
     bool raise = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        x[nt][c] = ((c & 2) ? v1 : v0) ? x[nt][c] * p.scale_log2 : -INFINITY;
-      raise |= fmaxf(x[nt][0], x[nt][2]) > m[nt][0] + kRaise;
-      raise |= fmaxf(x[nt][1], x[nt][3]) > m[nt][1] + kRaise;
+      raise |= fmaxf(x[nt][0], x[nt][2]) > m[nt][0] + slack;
+      raise |= fmaxf(x[nt][1], x[nt][3]) > m[nt][1] + slack;
     }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -503,12 +590,11 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
         for (int c = 0; c < 2; ++c) {
           float mx = fmaxf(x[nt][c], x[nt][c + 2]);
 #pragma unroll
-          for (int off = 4; off < 32; off <<= 1)
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+          for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
           mx = fmaxf(mx, m[nt][c]);
-          const float f = m[nt][c] == -INFINITY ? 0.f : ex2(m[nt][c] - mx);
+          const float f = m[nt][c] == -INFINITY ? 0.f : ex2((m[nt][c] - mx) * sl);
           m[nt][c] = mx;
-          moff[nt][c] = mx == -INFINITY ? 0.f : mx - kShift;
+          moff[nt][c] = mx == -INFINITY ? 0.f : fmaf(mx, sl, -kShift);
           l[nt][c] *= f;
 #pragma unroll
           for (int mt = 0; mt < 4 * W; ++mt) {
@@ -520,13 +606,10 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
     uint32_t ph[NT][2], pl[NT][2];  // P^T fragments, hi and lo
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float e[4], lo[4];
+      float e[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        // a masked score is -inf and its weight 2^-inf = 0, whatever moff is
-        e[c] = ex2(x[nt][c] - moff[nt][c & 1]);
-        lo[c] = e[c];
-      }
+      for (int c = 0; c < 4; ++c)  // a masked score is -inf and its weight 0, whatever moff is
+        e[c] = ex2(fmaf(x[nt][c], sl, -moff[nt][c & 1]));
       l[nt][0] += e[0] + e[2];
       l[nt][1] += e[1] + e[3];
 #pragma unroll
@@ -534,17 +617,17 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
         const uint32_t hi = pack_half2(e[2 * r], e[2 * r + 1]);
         const float2 hf = unpack_half2(hi);
         ph[nt][r] = movmatrix_trans(hi);
-        pl[nt][r] = movmatrix_trans(pack_half2(lo[2 * r] - hf.x, lo[2 * r + 1] - hf.y));
+        pl[nt][r] = movmatrix_trans(pack_half2(e[2 * r] - hf.x, e[2 * r + 1] - hf.y));
       }
     }
 
     // ── O^T += V^T . P^T ──────────────────────────────────────────────────
     {
       uint32_t vw[4][W], vs[W];
-      sg.load_v(st, vw, vs);
+      sg.template load_v<S0>(vw, vs);
       uint32_t keep = 0xffffffffu;  // scales of tokens past the end: 0, their V counts as 0
-      if (left < 16) {
-        const int nv = left - 4 * t;  // valid tokens among this lane's four
+      if (here < 16) {
+        const int nv = here - 4 * t;  // valid tokens among this lane's four
         keep = nv >= 4 ? 0xffffffffu : nv <= 0 ? 0u : (1u << (8 * nv)) - 1u;
       }
 #pragma unroll
@@ -574,7 +657,14 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
         }
       }
     }
-  }
+    return true;
+  };
+  each_stage<STAGES - 1>([&](auto s) {
+    issue(decltype(s)::value, s);
+    return true;
+  });
+  for (int i = 0; each_stage<STAGES>([&](auto s) { return step(i + decltype(s)::value, s); });)
+    i += STAGES;
   cp_async_wait<0>();
   __syncthreads();  // the rings become merge space
 
@@ -596,7 +686,8 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
       if (g == 0) {
-        sml[(warp * C::kHeads + head) * 2] = m[nt][c];
+        // any common offset of the reference points leaves the merges as they are
+        sml[(warp * C::kHeads + head) * 2] = m[nt][c] == -INFINITY ? -INFINITY : moff[nt][c];
         sml[(warp * C::kHeads + head) * 2 + 1] = s;
       }
     }

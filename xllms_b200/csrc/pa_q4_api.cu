@@ -1,5 +1,6 @@
 // pa_q4_api.cu — C ABI of the 4-bit KV cache (include/operator_api.h): argument
 // checks, launch planning and workspaces.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -24,7 +25,8 @@ int check_pools(const void* k, const void* v, int Hkv, int D, int bs, float ks, 
   if (!k || !v || !aligned(k, 16) || !aligned(v, 16)) return NXT_PA_EINVAL;
   if (Hkv <= 0 || D <= 0 || D > 256 || D % 16 || bs <= 0 || bs % 16) return NXT_PA_EINVAL;
   if (!scale_ok(ks) || !scale_ok(vs)) return NXT_PA_EINVAL;
-  if (kbs < 0 || khs < 0 || kbs % 16 || khs % 16) return NXT_PA_EINVAL;
+  // a page's bytes are an int: the kernels multiply page ids by them in one step
+  if (kbs < 0 || kbs > INT_MAX || khs < 0 || kbs % 16 || khs % 16) return NXT_PA_EINVAL;
   return NXT_PA_OK;
 }
 
@@ -58,13 +60,27 @@ int rows_call(bool write, void* key, void* value, void* kc, void* vc, const int6
   return map_cuda(write ? xpa::launch_q4_write(a, st) : xpa::launch_q4_read(a, st));
 }
 
-// Partitions of a 4-bit call: planned in 16-token tiles like the pages of a
-// one-byte cache, then rounded to whole pages.
+// Partitions of a 4-bit call, in 16-token tiles rounded to whole pages: at
+// most XPA_Q4_PART_TILES, halved while the grid would hold fewer than
+// XPA_Q4_ITEMS_PER_SM items per SM, but not below XPA_Q4_MIN_TILES.
+#ifndef XPA_Q4_PART_TILES
+#define XPA_Q4_PART_TILES 128
+#endif
+#ifndef XPA_Q4_ITEMS_PER_SM
+#define XPA_Q4_ITEMS_PER_SM 12
+#endif
+#ifndef XPA_Q4_MIN_TILES
+#define XPA_Q4_MIN_TILES 8
+#endif
 Plan q4_plan(int B, int Hq, int D, int Hkv, int max_blocks, int bs, int nsm) {
   const int spp = bs / 16;
-  const long long tiles = (long long)max_blocks * spp;
-  Plan pl = make_plan(B, Hq, D, Hkv, tiles > INT_MAX / 2 ? INT_MAX / 2 : (int)tiles, nsm, 1);
-  pl.part_pages = pl.part_pages / spp > 0 ? pl.part_pages / spp : 1;
+  const long long tiles = std::max(1LL, (long long)max_blocks * spp);
+  const long long rows = (long long)B * Hkv, want = (long long)XPA_Q4_ITEMS_PER_SM * nsm;
+  long long pt = XPA_Q4_PART_TILES;
+  while (pt > XPA_Q4_MIN_TILES && rows * ceil_div(tiles, pt) < want) pt >>= 1;
+  while (ceil_div(tiles, pt) > 8192) pt <<= 1;
+  Plan pl;
+  pl.part_pages = (int)std::max(1LL, pt / spp);
   pl.max_parts = ceil_div(max_blocks > 0 ? max_blocks : 1, pl.part_pages);
   pl.ws_bytes = pl.max_parts > 1 ? partial_bytes((long long)B * Hq * pl.max_parts, D) : 0;
   return pl;
