@@ -90,9 +90,12 @@ def attention(q, k, v, tables, lens, scale, num_blocks=None):
     kernel's arithmetic may be off by, element by element:
       scores are fp32 sums of exact products, D / 16 matrix steps of at most
       2^-22 of the sum of the terms' magnitudes each, plus the scaling's and
-      the exponential's few units: a weight is off by exp(2 ds) - 1 at most,
-      weights keep 22 bits, their products and sums are fp32 (2^-22 a step and
-      a tile), and the output is rounded to fp16 once (half a step: 2^-11)."""
+      the exponential's few units: a weight is off by exp(2 ds) - 1 at most;
+      a weight is then rounded to fp16 (half a step: 2^-11 of it; where that is
+      below fp16's normal range, half of 2^-24, 2^-32 of the largest weight,
+      since the largest is at least 2^7), their products and sums are fp32
+      (2^-22 a step and a tile), and the output is rounded to fp16 once
+      (2^-11)."""
     q = q.astype(np.float64)
     B, Hq, D = q.shape
     nb, hkv, bs, _ = k.shape
@@ -116,5 +119,7 @@ def attention(q, k, v, tables, lens, scale, num_blocks=None):
                 p /= p.sum()
                 ds = (D / 16 + 4) * 2.0 ** -22 * mag.max() + 2.0 ** -20
                 out[b, x] = p @ vv
-                bound[b, x] = (p @ np.abs(vv)) * (np.expm1(2 * ds) + (n / 16 + 16) * 2.0 ** -22)
+                bound[b, x] = (p @ np.abs(vv)) * (
+                np.expm1(2 * ds) + 2.0 ** -11 + (n / 16 + 16) * 2.0 ** -22)
+            bound[b, x] += 2.0 ** -32 * p.max() * np.abs(vv).sum(0)
     return out, bound + 2.0 ** -11 * np.abs(out) + 2.0 ** -24

@@ -1,5 +1,7 @@
 // pa_q4.cu — 4-bit KV cache: rows written and read back by slot, and paged
 // decode attention over it. Format and tile layout: pa_q4.cuh.
+#include <algorithm>
+#include <numeric>
 #include <type_traits>
 #include <utility>
 
@@ -156,7 +158,7 @@ __global__ void __launch_bounds__(128) pa_q4_read_kernel(const Q4RowsParams a) {
 //
 // Per tile, with mma.sync m16n8k16 (fp16 in, fp32 sums):
 //   S^T(16 tokens x 8 heads)  = K . Q^T      K as A, D / 16 steps
-//   O^T(D x 8 heads)         += V^T . P^T    V as A, D / 16 row tiles, P = hi + lo
+//   O^T(D x 8 heads)         += V^T . P^T    V as A, D / 16 row tiles
 // Token order: row r of S^T (and k index r of P^T) is token sigma(r) with
 // sigma(2 t) = 4 t, sigma(2 t + 1) = 4 t + 1, sigma(8 + 2 t) = 4 t + 2,
 // sigma(9 + 2 t) = 4 t + 3, so a lane's four V tokens are 4 t .. 4 t + 3 and
@@ -165,18 +167,22 @@ __global__ void __launch_bounds__(128) pa_q4_read_kernel(const Q4RowsParams a) {
 // row tile 4 w + i holds channels 8 (g W + w) + 2 i (row g) and + 1 (row g + 8).
 //
 // Softmax: scores live in the exp2 domain. The reference point m of a head
-// moves only when a score exceeds it by more than 8, so most tiles need one
-// vote and no shuffles; p <= 2^15 with the shift of 7 that keeps small
-// weights above fp16's subnormals. P = hi + lo in fp16 keeps 22 bits.
+// moves only when a score exceeds it by more than 8, so most steps need one
+// vote and no shuffles. The weights p = 2^(x - m + 7) <= 2^15 go into the
+// product as fp16, their sum is of the fp32 values: a weight keeps 11 bits
+// (2^-11 relative at most, next to codes of 1 mantissa bit) down to 2^-21 of
+// the largest and 2^-32 of it absolutely below. A second fp16 term for the
+// rest of p would cost a ninth of the kernel's time.
 // ════════════════════════════════════════════════════════════════════════
 constexpr float kRaise = 8.f;  // log2 units a score may exceed m by
 constexpr float kShift = 7.f;  // p = 2^(x - m + kShift) <= 2^15
 
-template <int W, int NT, bool EXACT, int NW, int STAGES>
+template <int W, int NT, bool EXACT, int NW, int STAGES, int U>
 struct Q4Cfg {
   static constexpr int kDMax = 64 * W;
   static constexpr int kHeads = 8 * NT;
-  static constexpr int kStageBytes = 18 * kDMax;  // one K and one V tile
+  static constexpr int kTileBytes = 18 * kDMax;   // one K and one V tile
+  static constexpr int kStageBytes = U * kTileBytes;
   static constexpr int kRow = kDMax + 4;          // merge rows, floats
   static constexpr size_t kMergeBytes =
       (size_t)NW * kHeads * kRow * sizeof(float) + (size_t)NW * kHeads * 2 * sizeof(float);
@@ -226,7 +232,6 @@ __device__ __forceinline__ void cp_async16_at(uint32_t dst, const uint8_t* src) 
 // 4 t + k's place is 4 k + t. Otherwise a tile is copied as it is.
 template <int W, bool EXACT>
 struct Q4Stage {
-  static constexpr int DD = 64 * W;
   int D, lane, g, t;
   // sources in page 0; EXACT: this lane's first chunk of each piece
   const uint8_t *ksrc, *vsrc, *ssrc;
@@ -241,6 +246,7 @@ struct Q4Stage {
     t = lane & 3;
     const int tok = 4 * (g >> 1) + (g & 1);  // sigma(g); sigma(g + 8) is + 2
     if constexpr (EXACT) {
+      constexpr int DD = 64 * W;
       constexpr int CPR = 2 * W;  // 16-byte chunks per row
       ksrc = k + lane * 16;
       vsrc = v + lane * 16;
@@ -282,15 +288,15 @@ struct Q4Stage {
     }
   }
 
-  // Issues the copies of the K and V tiles of page e, `sub` bytes into it.
+  // Issues the copies of the K and V tiles that start `at` units into the pools.
   template <int S0>
-  __device__ __forceinline__ void copy(int e, int page_bytes, int sub) const {
+  __device__ __forceinline__ void copy(unsigned at, unsigned unit) const {
     if constexpr (EXACT) {
       // rows per 32 chunks: 16 / W; their K places are 2 * (16 / W) / 4 apart
       constexpr int kStep = W == 1 ? 0 : (16 / W / 4) * 2 * 32 * W;
-      const uint8_t* k = ksrc + (long long)e * page_bytes + sub;
-      const uint8_t* v = vsrc + (long long)e * page_bytes + sub;
-      const uint8_t* s = ssrc + (long long)e * page_bytes + sub;
+      const uint8_t* k = ksrc + (unsigned long long)at * unit;
+      const uint8_t* v = vsrc + (unsigned long long)at * unit;
+      const uint8_t* s = ssrc + (unsigned long long)at * unit;
       cp_async16_at<S0, 0>(kd, k);
       if constexpr (W >= 2) cp_async16_at<S0 + kStep, 512>(kd, k);
       if constexpr (W == 4) {
@@ -305,7 +311,7 @@ struct Q4Stage {
       }
       if (W == 4 || (lane & 15) < 4 * W) cp_async16_at<S0, 0>(sd, s);
     } else {
-      const long long off = (long long)e * page_bytes + sub;
+      const unsigned long long off = (unsigned long long)at * unit;
       const int n = 9 * D / 16;
       for (int x = lane; x < n; x += 32) {
         cp_async16_at<S0, 0>(ring + x * 16, ksrc + off + x * 16);
@@ -400,20 +406,40 @@ __device__ __forceinline__ bool each_stage(F&& f) {
   return true;
 }
 
-// D = A . B, fp16 inputs, fp32 result.
-__device__ __forceinline__ void mma_f16_16816_zero(float (&d)[4], uint32_t a0, uint32_t a1,
-                                                   uint32_t a2, uint32_t a3, uint32_t b0,
-                                                   uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7},"
-      " {%8, %9}, {%10, %10, %10, %10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+// Addresses of one call: a tile starts at a whole number of units in its pool.
+struct Q4Units {
+  unsigned unit, page_units, tile_units;  // bytes; units per page, per tile
+  int page_limit;   // page ids below this are in the pools
+  int head_chunks;  // CTAs per group of query heads
+};
+
+constexpr int kGridY = 32768;
+
+// Partition blockIdx.x of row (sequence, KV head).
+__device__ __forceinline__ ItemKind q4_item(const Params& p, int row, Item& it) {
+  it.part = blockIdx.x;
+  it.b = row / p.Hkv;
+  it.kvh = row - it.b * p.Hkv;
+  int L = __ldg(p.seq_lens + it.b);
+  const long long cap = (long long)p.max_blocks * p.block_size;
+  if (L < 0 || L > cap) {
+    if (it.part == 0 && it.kvh == 0 && threadIdx.x == 0) raise_status(p, kDevSeqClamped);
+    L = L < 0 ? 0 : (int)cap;
+  }
+  it.L = L;
+  it.slot0 = 0;
+  const long long part_tokens = (long long)p.part_pages * p.block_size;
+  it.direct = L <= part_tokens;
+  if (L == 0) return it.part == 0 ? kItemZero : kItemNone;
+  if (it.part * part_tokens >= L) return kItemNone;
+  it.page_begin = it.part * p.part_pages;
+  it.page_end = it.page_begin + p.part_pages;
+  return kItemWork;
 }
 
-template <int W, int NT, bool EXACT, int NW, int STAGES, int MINB>
-__global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
-  using C = Q4Cfg<W, NT, EXACT, NW, STAGES>;
+template <int W, int NT, bool EXACT, int NW, int STAGES, int U, int MINB>
+__global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, const Q4Units q) {
+  using C = Q4Cfg<W, NT, EXACT, NW, STAGES, U>;
   extern __shared__ __align__(128) uint8_t smem[];
   // Every CTA waits for the kernel before this one (which may be this call's
   // append); the merge may be scheduled from here on and waits for this grid.
@@ -422,9 +448,13 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
   const int D = EXACT ? C::kDMax : p.D;
   const int NG = D / 16;
   Item it;
-  const ItemKind kind = decode_item(p, blockIdx.x, it);
+  // grid: x = partition, y and z = (sequence, KV head, head chunk)
+  const int col = blockIdx.y + blockIdx.z * kGridY;
+  if (col >= p.B * p.Hkv * q.head_chunks) return;
+  const int row = q.head_chunks == 1 ? col : col / q.head_chunks;
+  const ItemKind kind = q4_item(p, row, it);
   if (kind == kItemNone) return;
-  const int h0 = blockIdx.y * C::kHeads;
+  const int h0 = (col - row * q.head_chunks) * C::kHeads;
   const int nh = min(p.GS - h0, C::kHeads);
   const long long row0 = (long long)it.b * p.Hq + (long long)it.kvh * p.GS + h0;
   if (kind == kItemZero) {
@@ -444,20 +474,20 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
   // ── Q fragments: head g of tile nt, channels 16 j + 4 t .. + 3 ──────────
   uint32_t qf[4 * W][NT][2];
   {
-    const __half* q = static_cast<const __half*>(p.q);
-    const bool al = (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
+    const __half* query = static_cast<const __half*>(p.q);
+    const bool al = (reinterpret_cast<uintptr_t>(query) & 7u) == 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const bool head = nt * 8 + g < nh;
-      const __half* row = q + (row0 + nt * 8 + g) * D + 4 * t;
+      const __half* src = query + (row0 + nt * 8 + g) * D + 4 * t;
 #pragma unroll
       for (int j = 0; j < 4 * W; ++j) {
         uint2 u = make_uint2(0u, 0u);
         if (head && j < NG) {
           if (al) {
-            u = __ldg(reinterpret_cast<const uint2*>(row + 16 * j));
+            u = __ldg(reinterpret_cast<const uint2*>(src + 16 * j));
           } else {
-            const unsigned short* s = reinterpret_cast<const unsigned short*>(row + 16 * j);
+            const unsigned short* s = reinterpret_cast<const unsigned short*>(src + 16 * j);
             u.x = s[0] | ((uint32_t)s[1] << 16);
             u.y = s[2] | ((uint32_t)s[3] << 16);
           }
@@ -472,42 +502,51 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
     }
   }
 
-  // ── this warp's tiles: j = warp, warp + NW, ... of the item ─────────────
+  // ── this warp's steps of U tiles: i = warp, warp + NW, ... of the item ──
   const int spp = p.block_size >> 4;  // tiles per page
-  const int page_bytes = (int)p.kv_block_stride;
   const long long tok_end = min((long long)it.L, (long long)it.page_end * p.block_size);
   const int tok_begin = it.page_begin * p.block_size;
   const int tiles = (int)((tok_end - tok_begin + 15) >> 4);
-  const int n = tiles > warp ? (tiles - warp + NW - 1) / NW : 0;
+  const int steps = (tiles + U - 1) / U;
+  const int n = steps > warp ? (steps - warp + NW - 1) / NW : 0;
   const long long head_off = (long long)it.kvh * p.kv_head_stride;
   const Q4Stage<W, EXACT> sg(D, lane, static_cast<const uint8_t*>(p.k) + head_off,
                              static_cast<const uint8_t*>(p.v) + head_off,
                              smem_u32(smem) + warp * (STAGES * C::kStageBytes));
   const int* table = p.block_tables + (long long)it.b * p.max_blocks + it.page_begin;
-  auto entry_ok = [&](int e) { return e >= 0 && (p.num_blocks <= 0 || e < p.num_blocks); };
+  auto entry_ok = [&](int e) { return e >= 0 && e < q.page_limit; };
 
-  int ent = -1, sub = 0;  // lane l: page and offset in it of tile (i & ~31) + l; -1: none
-  bool masked = false;    // a page of this warp's is masked
+  constexpr int kBatch = 32 / U;
+  constexpr unsigned kNone = 0xffffffffu;
+  // lane l: where tile l % U of step i - i % kBatch + l / U starts, in units
+  unsigned ent = kNone;
+  bool masked = false;  // a page of this warp's is masked
+  auto tile_page = [&](int i, int u) { return (U * (warp + i * NW) + u) / spp; };
   auto issue = [&](int i, auto stage) {
+    constexpr int S0 = decltype(stage)::value * C::kStageBytes;
     if (i < n) {
-      if ((i & 31) == 0) {
+      if (i % kBatch == 0) {
         bool bad = false;
-        if (i + lane < n) {
-          const int j = warp + (i + lane) * NW;
+        const int j = U * (warp + (i + lane / U) * NW) + lane % U;
+        ent = kNone;
+        if (j < tiles) {
           const int page = spp == 1 ? j : j / spp;
-          sub = (j - page * spp) * (9 * D);
-          ent = __ldg(table + page);
-          bad = !entry_ok(ent);
-          if (bad) {
-            ent = -1;
+          const int e = __ldg(table + page);
+          bad = !entry_ok(e);
+          if (bad)
             raise_status(p, kDevBadPage);
-          }
+          else
+            ent = (unsigned)e * q.page_units + (unsigned)(j - page * spp) * q.tile_units;
         }
         masked |= __any_sync(0xffffffffu, bad);
       }
-      const int e = __shfl_sync(0xffffffffu, ent, i & 31);
-      const int in = spp > 1 ? __shfl_sync(0xffffffffu, sub, i & 31) : 0;
-      if (e >= 0) sg.template copy<decltype(stage)::value * C::kStageBytes>(e, page_bytes, in);
+      const int l = U * (i % kBatch);
+      each_stage<U>([&](auto u) {
+        constexpr int T0 = S0 + decltype(u)::value * C::kTileBytes;
+        const unsigned at = __shfl_sync(0xffffffffu, ent, l + decltype(u)::value);
+        if (at != kNone) sg.template copy<T0>(at, q.unit);
+        return true;
+      });
     }
     cp_async_commit();
   };
@@ -525,70 +564,90 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
       l[nt][c] = 0.f;
     }
 
-  // One tile, the warp's i-th, from ring stage `stage`; false after the last.
-  int left = (int)(tok_end - tok_begin) - warp * 16;  // tokens from this tile on
+  // The warp's i-th step, from ring stage `stage`; false after the last.
+  int left = (int)(tok_end - tok_begin) - warp * (16 * U);  // tokens from this step on
   auto step = [&](int i, auto stage) {
     constexpr int S = decltype(stage)::value, S0 = S * C::kStageBytes;
     if (i >= n) return false;
     cp_async_wait<STAGES - 2>();
     __syncwarp();  // every lane's copies of this stage are in; the one before is free
     issue(i + STAGES - 1, std::integral_constant<int, (S + STAGES - 1) % STAGES>{});
-    const int here = left;
-    left -= 16 * NW;
-    if (masked && !entry_ok(__ldg(table + (warp + i * NW) / spp))) return true;  // warp-uniform
+    int here[U];  // valid tokens of each tile, when below 16
+#pragma unroll
+    for (int u = 0; u < U; ++u) here[u] = left - 16 * u;
+    left -= 16 * U * NW;
+    if (masked) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (here[u] > 0 && !entry_ok(__ldg(table + tile_page(i, u)))) here[u] = 0;
+    }
+    const bool partial = here[0] < 16 || here[U - 1] < 16;
 
-    // ── S^T = K . Q^T, a channel group's scale applied to its sums ────────
-    float x[NT][4] = {};
+    // ── S^T = K . Q^T ─────────────────────────────────────────────────────
+    float x[U][NT][4] = {};
     {
-      uint32_t kw[2][2 * W], ks[2][W];
-      sg.template load_k<S0>(kw, ks);
+      uint32_t kw[U][2][2 * W], ks[U][2][W];
+      each_stage<U>([&](auto u) {
+        constexpr int V = decltype(u)::value;
+        sg.template load_k<S0 + V * C::kTileBytes>(kw[V], ks[V]);
+        return true;
+      });
 #pragma unroll
       for (int i2 = 0; i2 < 2 * W; ++i2) {
         if (!EXACT && 2 * i2 >= NG) break;
-        uint32_t a[2][4];
-        float2 sc[2];  // groups 2 i2 and 2 i2 + 1 of rows g and g + 8
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          sc[r] = unpack_half2(fp8x2_to_h2<kKvE4M3>(ks[r][i2 >> 1] >> (16 * (i2 & 1))));
-          q4x8_to_h2(kw[r][i2], a[r]);
-        }
+        for (int u = 0; u < U; ++u) {
+          uint32_t a[2][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float y[4], z[4];
-          mma_f16_16816_zero(y, a[0][0], a[1][0], a[0][1], a[1][1], qf[2 * i2][nt][0],
-                             qf[2 * i2][nt][1]);
-          mma_f16_16816_zero(z, a[0][2], a[1][2], a[0][3], a[1][3], qf[2 * i2 + 1][nt][0],
-                             qf[2 * i2 + 1][nt][1]);
+          for (int r = 0; r < 2; ++r) {
+            // scales of groups 2 i2 and 2 i2 + 1
+            const uint32_t s2 = fp8x2_to_h2<kKvE4M3>(ks[u][r][i2 >> 1] >> (16 * (i2 & 1)));
+            q4x8_to_h2(kw[u][r][i2], a[r]);
+            a[r][0] = h2_mul_low(a[r][0], s2);
+            a[r][1] = h2_mul_low(a[r][1], s2);
+            a[r][2] = h2_mul_high(a[r][2], s2);
+            a[r][3] = h2_mul_high(a[r][3], s2);
+          }
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            x[nt][c] = fmaf(y[c], sc[c >> 1].x, x[nt][c]);
-            x[nt][c] = fmaf(z[c], sc[c >> 1].y, x[nt][c]);
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_f16_16816(x[u][nt], a[0][0], a[1][0], a[0][1], a[1][1], qf[2 * i2][nt][0],
+                          qf[2 * i2][nt][1]);
+            mma_f16_16816(x[u][nt], a[0][2], a[1][2], a[0][3], a[1][3], qf[2 * i2 + 1][nt][0],
+                          qf[2 * i2 + 1][nt][1]);
           }
         }
       }
     }
 
     // ── softmax step ──────────────────────────────────────────────────────
-    if (here < 16) {  // tokens sigma(g) and sigma(g + 8) of the last tile
+    if (partial) {  // tokens sigma(g) and sigma(g + 8)
       const int tok = 4 * (g >> 1) + (g & 1);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (tok >= here) x[nt][0] = x[nt][1] = -INFINITY;
-        if (tok + 2 >= here) x[nt][2] = x[nt][3] = -INFINITY;
-      }
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (tok >= here[u]) x[u][nt][0] = x[u][nt][1] = -INFINITY;
+          if (tok + 2 >= here[u]) x[u][nt][2] = x[u][nt][3] = -INFINITY;
+        }
     }
+    auto top = [&](int nt, int c) {
+      float mx = fmaxf(x[0][nt][c], x[0][nt][c + 2]);
+#pragma unroll
+      for (int u = 1; u < U; ++u) mx = fmaxf(mx, fmaxf(x[u][nt][c], x[u][nt][c + 2]));
+      return mx;
+    };
     bool raise = false;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      raise |= fmaxf(x[nt][0], x[nt][2]) > m[nt][0] + slack;
-      raise |= fmaxf(x[nt][1], x[nt][3]) > m[nt][1] + slack;
-    }
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        raise |= top(nt, c) > m[nt][c] + slack;
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float mx = fmaxf(x[nt][c], x[nt][c + 2]);
+          float mx = top(nt, c);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
           mx = fmaxf(mx, m[nt][c]);
@@ -603,43 +662,51 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
           }
         }
     }
-    uint32_t ph[NT][2], pl[NT][2];  // P^T fragments, hi and lo
+    uint32_t pf[U][NT][2];  // P^T fragments
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float e[4];
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int c = 0; c < 4; ++c)  // a masked score is -inf and its weight 0, whatever moff is
-        e[c] = ex2(fmaf(x[nt][c], sl, -moff[nt][c & 1]));
-      l[nt][0] += e[0] + e[2];
-      l[nt][1] += e[1] + e[3];
+      for (int nt = 0; nt < NT; ++nt) {
+        float e[4];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint32_t hi = pack_half2(e[2 * r], e[2 * r + 1]);
-        const float2 hf = unpack_half2(hi);
-        ph[nt][r] = movmatrix_trans(hi);
-        pl[nt][r] = movmatrix_trans(pack_half2(e[2 * r] - hf.x, e[2 * r + 1] - hf.y));
+        for (int c = 0; c < 4; ++c)  // a masked score is -inf and its weight 0, whatever moff is
+          e[c] = ex2(fmaf(x[u][nt][c], sl, -moff[nt][c & 1]));
+        l[nt][0] += e[0] + e[2];
+        l[nt][1] += e[1] + e[3];
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          pf[u][nt][r] = movmatrix_trans(pack_half2(e[2 * r], e[2 * r + 1]));
       }
-    }
 
     // ── O^T += V^T . P^T ──────────────────────────────────────────────────
-    {
-      uint32_t vw[4][W], vs[W];
-      sg.template load_v<S0>(vw, vs);
-      uint32_t keep = 0xffffffffu;  // scales of tokens past the end: 0, their V counts as 0
-      if (here < 16) {
-        const int nv = here - 4 * t;  // valid tokens among this lane's four
-        keep = nv >= 4 ? 0xffffffffu : nv <= 0 ? 0u : (1u << (8 * nv)) - 1u;
+    // scales of tokens past the end become 0, so their V counts as 0
+    uint32_t keep[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      keep[u] = 0xffffffffu;
+      if (partial) {
+        const int nv = here[u] - 4 * t;  // valid tokens among this lane's four
+        keep[u] = nv >= 4 ? 0xffffffffu : nv <= 0 ? 0u : (1u << (8 * nv)) - 1u;
       }
+    }
+    uint32_t vw[U][4][W], vs[U][W];
+    each_stage<U>([&](auto u) {
+      constexpr int V = decltype(u)::value;
+      sg.template load_v<S0 + V * C::kTileBytes>(vw[V], vs[V]);
+      return true;
+    });
+#pragma unroll
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         if (!EXACT && w * 8 >= D) break;
-        const uint32_t sw = vs[w] & keep;
+        const uint32_t sw = vs[u][w] & keep[u];
         const uint32_t s01 = fp8x2_to_h2<kKvE4M3>(sw), s23 = fp8x2_to_h2<kKvE4M3>(sw >> 16);
         uint32_t a[4][4];  // [even 01, odd 01, even 23, odd 23][channel pair]
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           // nibbles of two tokens side by side: byte i = channels 2 i / 2 i + 1
-          const uint32_t w0 = vw[2 * k][w], w1 = vw[2 * k + 1][w];
+          const uint32_t w0 = vw[u][2 * k][w], w1 = vw[u][2 * k + 1][w];
           const uint32_t ev = (w0 & 0x0f0f0f0fu) | ((w1 << 4) & 0xf0f0f0f0u);
           const uint32_t od = ((w0 >> 4) & 0x0f0f0f0fu) | (w1 & 0xf0f0f0f0u);
           q4x8_to_h2(ev, a[2 * k]);
@@ -650,13 +717,10 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
           const uint32_t a0 = h2_mul(a[0][i2], s01), a1 = h2_mul(a[1][i2], s01);
           const uint32_t a2 = h2_mul(a[2][i2], s23), a3 = h2_mul(a[3][i2], s23);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_f16_16816(o[4 * w + i2][nt], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
-            mma_f16_16816(o[4 * w + i2][nt], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
-          }
+          for (int nt = 0; nt < NT; ++nt)
+            mma_f16_16816(o[4 * w + i2][nt], a0, a1, a2, a3, pf[u][nt][0], pf[u][nt][1]);
         }
       }
-    }
     return true;
   };
   each_stage<STAGES - 1>([&](auto s) {
@@ -705,9 +769,17 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
       // a warp without a score above -inf holds zeros, or NaN to pass on
       const float wt = mw == M ? 1.f : ex2(mw - M);
       den = fmaf(wt, sml[(w * C::kHeads + head) * 2 + 1], den);
-      const float* src = so + (size_t)(w * C::kHeads + head) * C::kRow + d0;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) num[k] = fmaf(wt, src[k], num[k]);
+      const float4* src =
+          reinterpret_cast<const float4*>(so + (size_t)(w * C::kHeads + head) * C::kRow + d0);
+      const float4 a = src[0], b = src[1];
+      num[0] = fmaf(wt, a.x, num[0]);
+      num[1] = fmaf(wt, a.y, num[1]);
+      num[2] = fmaf(wt, a.z, num[2]);
+      num[3] = fmaf(wt, a.w, num[3]);
+      num[4] = fmaf(wt, b.x, num[4]);
+      num[5] = fmaf(wt, b.y, num[5]);
+      num[6] = fmaf(wt, b.z, num[6]);
+      num[7] = fmaf(wt, b.w, num[7]);
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) num[k] *= p.v_scale;
@@ -722,13 +794,11 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p) {
       }
     } else {
       const long long pr = (row0 + head) * p.slots + it.slot0 + it.part;
-      float* dst = p.part_o + pr * D + d0;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) dst[k] = num[k];
-      if (d0 == 0) {
-        p.part_ml[2 * pr] = M;
-        p.part_ml[2 * pr + 1] = den;
-      }
+      // D is a multiple of 16: the partials' rows start on 16-byte boundaries
+      float4* dst = reinterpret_cast<float4*>(p.part_o + pr * D + d0);
+      dst[0] = make_float4(num[0], num[1], num[2], num[3]);
+      dst[1] = make_float4(num[4], num[5], num[6], num[7]);
+      if (d0 == 0) reinterpret_cast<float2*>(p.part_ml)[pr] = make_float2(M, den);
     }
   }
 }
@@ -753,8 +823,11 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t
 #ifndef XPA_Q4_WARPS
 #define XPA_Q4_WARPS 4
 #endif
+#ifndef XPA_Q4_TILES
+#define XPA_Q4_TILES 2
+#endif
 #ifndef XPA_Q4_STAGES
-#define XPA_Q4_STAGES 4
+#define XPA_Q4_STAGES 2
 #endif
 #ifndef XPA_Q4_MIN_CTAS
 #define XPA_Q4_MIN_CTAS 4
@@ -762,19 +835,34 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t
 
 template <int W, int NT, bool EXACT>
 cudaError_t launch_q4_t(const Params& p, cudaStream_t st) {
-  constexpr int NW = XPA_Q4_WARPS, STAGES = XPA_Q4_STAGES;
+  constexpr int NW = XPA_Q4_WARPS, STAGES = XPA_Q4_STAGES, U = XPA_Q4_TILES;
   constexpr int MINB = (EXACT && W <= 2 && NT == 1) ? XPA_Q4_MIN_CTAS : 1;
-  using C = Q4Cfg<W, NT, EXACT, NW, STAGES>;
-  auto kern = pa_q4_kernel<W, NT, EXACT, NW, STAGES, MINB>;
+  using C = Q4Cfg<W, NT, EXACT, NW, STAGES, U>;
+  auto kern = pa_q4_kernel<W, NT, EXACT, NW, STAGES, U, MINB>;
   cudaError_t e =
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
   if (e != cudaSuccess) return e;
   e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout,
                            (int)cudaSharedmemCarveoutMaxShared);
   if (e != cudaSuccess) return e;
-  const long long items = (long long)p.B * p.Hkv * p.max_parts;
-  const unsigned chunks = (unsigned)((p.GS + C::kHeads - 1) / C::kHeads);
-  return launch_pdl(kern, dim3((unsigned)items, chunks), NW * 32, C::kSmem, st, p);
+  // addresses in the largest unit that divides a page's and a tile's bytes
+  Q4Units q;
+  const unsigned tile = 9u * p.D, page = (unsigned)p.kv_block_stride;
+  q.unit = page ? std::gcd(page, tile) : tile;
+  q.page_units = page / q.unit;
+  q.tile_units = tile / q.unit;
+  // page ids whose addresses fit in 32 bits of units; the rest are masked
+  const unsigned spp = (unsigned)p.block_size / 16;
+  long long limit = 0x7fffffffLL;
+  if (q.page_units > 0)
+    limit = std::min(limit, (0xfffffffeLL - (long long)spp * q.tile_units) / q.page_units);
+  if (p.num_blocks > 0) limit = std::min(limit, p.num_blocks);
+  q.page_limit = (int)limit;
+  q.head_chunks = (p.GS + C::kHeads - 1) / C::kHeads;
+  const long long cols = (long long)p.B * p.Hkv * q.head_chunks;
+  const dim3 grid((unsigned)p.max_parts, (unsigned)std::min<long long>(cols, kGridY),
+                  (unsigned)((cols + kGridY - 1) / kGridY));
+  return launch_pdl(kern, grid, NW * 32, C::kSmem, st, p, q);
 }
 
 }  // namespace

@@ -55,8 +55,17 @@ __device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
       __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint32_t h2_low2(uint32_t a) { return __byte_perm(a, a, 0x1010); }
-__device__ __forceinline__ uint32_t h2_high2(uint32_t a) { return __byte_perm(a, a, 0x3232); }
+// a times the low / the high half of s (the multiply selects it: no extra step).
+__device__ __forceinline__ uint32_t h2_mul_low(uint32_t a, uint32_t s) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a),
+                            __low2half2(*reinterpret_cast<const __half2*>(&s)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t h2_mul_high(uint32_t a, uint32_t s) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a),
+                            __high2half2(*reinterpret_cast<const __half2*>(&s)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 
 // ── encoding ────────────────────────────────────────────────────────────
 // The E4M3 scale of a group whose largest |t| is amax.

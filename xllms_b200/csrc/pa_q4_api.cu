@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <numeric>
 
 #include "operator_api.h"
 #include "pa_host.h"
@@ -25,7 +26,6 @@ int check_pools(const void* k, const void* v, int Hkv, int D, int bs, float ks, 
   if (!k || !v || !aligned(k, 16) || !aligned(v, 16)) return NXT_PA_EINVAL;
   if (Hkv <= 0 || D <= 0 || D > 256 || D % 16 || bs <= 0 || bs % 16) return NXT_PA_EINVAL;
   if (!scale_ok(ks) || !scale_ok(vs)) return NXT_PA_EINVAL;
-  // a page's bytes are an int: the kernels multiply page ids by them in one step
   if (kbs < 0 || kbs > INT_MAX || khs < 0 || kbs % 16 || khs % 16) return NXT_PA_EINVAL;
   return NXT_PA_OK;
 }
@@ -100,10 +100,16 @@ int attention_call(void* out, const void* q, const void* k, const void* v, const
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return NXT_PA_ECUDA;
   const Plan pl = q4_plan(B, Hq, D, Hkv, max_blocks, bs, sm_count_of(dev));
-  // grid x: items; grid y: chunks of 8 query heads of a group
-  if ((long long)B * Hkv * pl.max_parts > INT_MAX || (long long)B * Hq > INT_MAX ||
-      ceil_div(Hq / Hkv, 8) > 65535)
+  // one CTA per partition and 8 query heads (16 of a larger group) at least
+  if ((long long)B * Hkv * pl.max_parts > INT_MAX || (long long)B * Hq > INT_MAX)
     return NXT_PA_EINVAL;
+  // the kernels address tiles by 32 bits of the largest unit that divides a
+  // page and a tile; pools that are known to be larger are refused
+  if (num_blocks > 0 && kbs > 0) {
+    const long long unit = std::gcd(kbs, 9LL * D);
+    if ((num_blocks - 1) * (kbs / unit) + (bs / 16) * (9LL * D / unit) > 0xfffffffeLL)
+      return NXT_PA_EINVAL;
+  }
   if (check_only) return NXT_PA_OK;
   int* status = dev_status;
   if (!status) {
