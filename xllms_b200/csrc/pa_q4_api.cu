@@ -67,7 +67,7 @@ int rows_call(bool write, void* key, void* value, void* kc, void* vc, const int6
 #define XPA_Q4_PART_TILES 128
 #endif
 #ifndef XPA_Q4_ITEMS_PER_SM
-#define XPA_Q4_ITEMS_PER_SM 12
+#define XPA_Q4_ITEMS_PER_SM 4
 #endif
 #ifndef XPA_Q4_MIN_TILES
 #define XPA_Q4_MIN_TILES 8

@@ -49,12 +49,19 @@ struct SelectParams {
   long long head_pages;  // kv_block_stride / kv_head_stride
   int B, Hq, Hkv, D, GS, max_blocks, block_size;
   int keep, sink, recent;
-  int chunks;  // score CTAs per row
+  int chunks, chunk_pages;  // score CTAs per row, pages of each
   float sign;  // of the score scale: -1, 0 or 1
   int vec;     // fp16, D % 8 == 0, q and bounds on 16-byte boundaries
 };
 
-constexpr int kScoreChunk = 256;  // pages per score CTA
+// Pages of one score CTA: 256 in the tensor-core kernel where that still fills
+// the GPU (four tiles of 16 pages a warp), else 64; 32 in the scalar one, whose
+// warps take a page at a time.
+inline int score_chunk_pages(long long rows, int max_blocks, bool vec, int sms) {
+  if (!vec) return 32;
+  return rows * ((max_blocks + 255) / 256) >= 4LL * sms ? 256 : 64;
+}
+constexpr int kMinScoreChunk = 32;
 
 cudaError_t launch_select(const SelectParams& p, int dtype_size, cudaStream_t st);
 

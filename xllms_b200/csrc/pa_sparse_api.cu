@@ -59,7 +59,7 @@ int bounds_call(void* bounds, const void* key_cache, const int* bt, const int* s
     p.vec = aligned(key_cache, 16) && aligned(bounds, 16) && (D * es) % 16 == 0 &&
             (kbs * es) % 16 == 0 && (khs * es) % 16 == 0;
   }
-  if ((long long)B * Hkv > INT_MAX || (long long)B * Hkv * p.pages_per_seq / 4 >= INT_MAX)
+  if ((long long)B * p.pages_per_seq > INT_MAX)
     return NXT_PA_EINVAL;
   p.status = dev_status;
   if (!p.status) {
@@ -90,16 +90,22 @@ struct SparseCall {
   float k_scale = 1.f, v_scale = 1.f;
 };
 
+// Items per SM below which the attention over the kept pages splits its rows
+// further. A row holds few pages here, so the partials of a finer split cost
+// more than an idle SM.
+#ifndef XPA_SPARSE_ITEMS_PER_SM
+#define XPA_SPARSE_ITEMS_PER_SM 8
+#endif
+
 // Workspace: scores and near pages of the selection, the kept pages' tables,
 // the attention's partials, each from a 256-byte boundary.
 struct Layout {
   size_t keys, absmax, near_page, near_key, tables, lens, part, total;
   size_t part_bytes;
-  int chunks;
 };
 
 Layout layout_of(long long rows, int GS, int D, int max_blocks, int bs, int ds, int keep, bool q4,
-                 bool attention) {
+                 bool attention, int sms) {
   Layout l{};
   size_t at = 0;
   auto take = [&at](size_t bytes) {
@@ -107,17 +113,16 @@ Layout layout_of(long long rows, int GS, int D, int max_blocks, int bs, int ds, 
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  l.chunks = ceil_div(max_blocks, xpa::kScoreChunk);
   const size_t scored = max_blocks > keep ? (size_t)rows * max_blocks : 0;
   l.keys = take(scored * sizeof(unsigned));
-  l.absmax = take((size_t)rows * l.chunks * sizeof(float));
+  l.absmax = take(scored ? (size_t)rows * ceil_div(max_blocks, xpa::kMinScoreChunk) * sizeof(float) : 0);
   l.near_page = take(scored * sizeof(unsigned));
   l.near_key = take(scored * sizeof(unsigned long long));
   if (attention) {
     l.tables = take((size_t)rows * keep * sizeof(int));
     l.lens = take((size_t)rows * sizeof(int));
     l.part_bytes = q4 ? nxt_paged_attention_q4_workspace_size((int)rows, GS, D, 1, keep, bs)
-                      : nxt_paged_attention_workspace_size((int)rows, GS, D, 1, keep, bs, ds);
+                      : make_plan((int)rows, GS, D, 1, keep, sms, ds, XPA_SPARSE_ITEMS_PER_SM).ws_bytes;
     l.part = take(l.part_bytes);
   }
   l.total = at;
@@ -150,7 +155,7 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
   if (ws && !workspace_aligned(ws)) return NXT_PA_EINVAL;
   const long long rows = (long long)c.B * c.Hkv;
   const int GS = c.Hq / c.Hkv;
-  if (rows * ceil_div(c.max_blocks, xpa::kScoreChunk) > INT_MAX || rows * GS > INT_MAX ||
+  if (rows * ceil_div(c.max_blocks, xpa::kMinScoreChunk) > INT_MAX || rows * GS > INT_MAX ||
       rows * c.keep > INT_MAX)
     return NXT_PA_EINVAL;
   const long long head_pages = c.Hkv > 1 ? c.kbs / c.khs : 1;
@@ -164,7 +169,8 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
     if (rc != NXT_PA_OK) return rc;
   }
   const Layout l =
-      layout_of(rows, GS, c.D, c.max_blocks, c.bs, c.ds, c.keep, c.q4, attention);
+      layout_of(rows, GS, c.D, c.max_blocks, c.bs, c.ds, c.keep, c.q4, attention,
+                sm_count_of(dev));
   std::unique_lock<std::mutex> lk;
   if (ws) {
     if (ws_bytes < l.total) return NXT_PA_EWORKSPACE;
@@ -198,9 +204,10 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
   p.keep = c.keep;
   p.sink = c.sink;
   p.recent = c.recent;
-  p.chunks = l.chunks;
   p.sign = c.scale > 0.f ? 1.f : c.scale < 0.f ? -1.f : 0.f;
   p.vec = c.ds == 2 && c.D % 8 == 0 && aligned(c.q, 16) && aligned(c.bounds, 16);
+  p.chunk_pages = xpa::score_chunk_pages(rows, c.max_blocks, p.vec, sm_count_of(dev));
+  p.chunks = ceil_div(c.max_blocks, p.chunk_pages);
   const cudaError_t e = xpa::launch_select(p, c.ds, st);
   if (e != cudaSuccess) return map_cuda(e);
   if (!attention) return NXT_PA_OK;
@@ -213,9 +220,9 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
                                      GS, c.D, 1, c.scale, c.keep, c.bs, c.k_scale,
                                      c.v_scale, page_stride, c.khs, nb, part, l.part_bytes, status,
                                      st);
-  return nxt_paged_attention_ex(c.out, c.q, c.k, c.v, p.sel_tables, p.sel_lens, (int)rows, GS, c.D,
-                                1, c.scale, c.keep, c.bs, c.ds, page_stride, c.khs, nb, part,
-                                l.part_bytes, status, st);
+  return attention_planned(c.out, c.q, c.k, c.v, p.sel_tables, p.sel_lens, (int)rows, GS, c.D, 1,
+                           c.scale, c.keep, c.bs, c.ds, page_stride, c.khs, nb, part, l.part_bytes,
+                           status, st, XPA_SPARSE_ITEMS_PER_SM);
 }
 
 }  // namespace
@@ -306,11 +313,14 @@ size_t nxt_paged_attention_sparse_workspace_size(int num_seqs, int num_heads, in
   const long long rows = (long long)num_seqs * num_kv_heads;
   if (rows > INT_MAX) return 0;
   const int GS = num_heads / num_kv_heads;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = -1;
+  const int sms = sm_count_of(dev);
   const size_t plain = layout_of(rows, GS, head_size, max_num_blocks_per_seq, block_size,
-                                 dtype_size, max_pages, false, true)
+                                 dtype_size, max_pages, false, true, sms)
                            .total;
   const size_t q4 = layout_of(rows, GS, head_size, max_num_blocks_per_seq, block_size, dtype_size,
-                              max_pages, true, true)
+                              max_pages, true, true, sms)
                         .total;
   return plain > q4 ? plain : q4;
 }
