@@ -7,6 +7,7 @@
 // no less than any q . k of the page; the score of a KV head is the largest
 // over its query heads. The best pages are kept, in the exact order of the
 // scores, ties to the earlier page.
+#include <algorithm>
 #include <cfloat>
 #include <climits>
 #include <utility>
@@ -296,126 +297,176 @@ __device__ __forceinline__ int table_entry(const SelectParams& p, int b, int at)
   return e;
 }
 
-// fp16 with 16-byte rows: 16 pages x 8 heads per warp step on mma.sync. The
-// work per page is 2 D bytes x 2 against 4 D flop per head, far below the
-// tensor ridge: bound by HBM. k index 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of the
-// two steps over channels 32 c .. + 31 are channels 32 c + 8 t .. + 7, so a
-// lane's share of a bounds row is one 16-byte load.
-// C: 32-channel blocks, ceil(D / 32) rounded up.
-template <int C>
-__global__ void __launch_bounds__(128) pa_score_mma_kernel(const SelectParams p) {
-  __shared__ float s_max[4];
+// fp16 with 16-byte rows: 16 pages x 8 heads per warp step on mma.sync, the
+// bounds [lo | hi] of a page as one row of 2 D values against [q^- | q^+], and
+// their magnitudes against each other for the error bound. The work per page
+// is 4 D bytes against 8 D flop per head, far below the tensor ridge: bound by
+// HBM, so each warp copies whole rows (4 D contiguous bytes) into a ring of two
+// tiles of its own with cp.async and scores the tile before meanwhile. Rows are
+// padded by 16 bytes to an odd number of 16-byte units, so ldmatrix reads eight
+// of them without a bank conflict. CTA = (sequence, W KV heads, chunk of pages):
+// its warps read the same pages side by side (all heads of a page are one run
+// of memory), each with its own KV head, and with a second set of tiles where
+// there are few heads.
+// S: steps of 16 values, 2 D <= 16 S; FULL: 2 D = 16 S.
+constexpr int kScoreWarps = 4;  // W: three CTAs per SM at D = 128, whose starts overlap
+inline size_t score_smem_bytes(int D) {
+  return (size_t)kScoreWarps * 2 * kScoreTile * (4 * D + 16);
+}
+
+template <int S, bool FULL>
+__global__ void __launch_bounds__(kScoreWarps * 32) pa_score_mma_kernel(const SelectParams p) {
+  extern __shared__ __align__(128) uint8_t smem[];
   pdl_wait_primary();
-  const int row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
-  const int b = row / p.Hkv, h = row - b * p.Hkv;
+  const int D = FULL ? 8 * S : p.D;
+  constexpr int NW = kScoreWarps;
+  const int groups = (p.Hkv + NW - 1) / NW;
+  const int chunk = blockIdx.x % p.chunks, col = blockIdx.x / p.chunks;
+  const int b = col / groups, first_head = (col - b * groups) * NW;
   const int L = clamped_len(p.seq_lens, b, p.max_blocks, p.block_size, nullptr, false);
   const int npages = (int)(((long long)L + p.block_size - 1) / p.block_size);
   const int page_end = min(npages, (chunk + 1) * p.chunk_pages);
   if (npages <= p.keep || chunk * p.chunk_pages >= npages) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const __half* bounds = static_cast<const __half*>(p.bounds) + (long long)h * 2 * p.D;
-  const long long page_stride = (long long)p.Hkv * 2 * p.D;
+  const int heads = min(p.Hkv - first_head, NW), sets = NW / heads;
+  const int set = warp / heads, h = first_head + warp - set * heads;
+  if (set >= sets) return;
+  const int row = b * p.Hkv + h;
+  const int row_bytes = 4 * D + 16, stage_bytes = kScoreTile * row_bytes;
+  const uint32_t ring = smem_u32(smem) + warp * 2 * stage_bytes;
+  const uint8_t* bounds = static_cast<const uint8_t*>(p.bounds) + (long long)h * 4 * D;
+  const unsigned page_bytes = (unsigned)p.Hkv * 4u * (unsigned)D;
   unsigned* keys = p.keys + (long long)row * p.max_blocks;
-  float big = 0.f;
+  float* magnitude = p.magnitude + (long long)row * p.tiles;
+  // lanes 0..15: the entries of the tile at `at`, -1 past the end
+  auto entries = [&](int at) {
+    return lane < kScoreTile && at + lane < page_end ? table_entry(p, b, at + lane) : -1;
+  };
+  // Copies a tile's rows; a page that is not there reads the first page's row
+  // and is dropped at the end.
+  auto issue = [&](int e, uint32_t st) {
+    if constexpr (FULL && S == 8) {  // 256-byte rows, two at a time
+      const uint8_t* src = bounds + (lane & 15) * 16;
+      const uint32_t dst = st + (lane >> 4) * row_bytes + (lane & 15) * 16;
+#pragma unroll
+      for (int r = 0; r < kScoreTile; r += 2) {
+        const int er = max(__shfl_sync(0xffffffffu, e, r + (lane >> 4)), 0);
+        cp_async16(dst + r * row_bytes, src + (unsigned long long)(unsigned)er * page_bytes);
+      }
+    } else if constexpr (FULL) {  // rows of one or more times 512 bytes
+      const uint8_t* src = bounds + lane * 16;
+      const uint32_t dst = st + lane * 16;
+#pragma unroll
+      for (int r = 0; r < kScoreTile; ++r) {
+        const int er = max(__shfl_sync(0xffffffffu, e, r), 0);
+        const uint8_t* from = src + (unsigned long long)(unsigned)er * page_bytes;
+#pragma unroll
+        for (int c = 0; c < S / 16; ++c)
+          cp_async16(dst + r * row_bytes + c * 512, from + c * 512);
+      }
+    } else {
+#pragma unroll 1
+      for (int r = 0; r < kScoreTile; ++r) {
+        const int er = max(__shfl_sync(0xffffffffu, e, r), 0);
+        const uint8_t* from = bounds + (unsigned long long)(unsigned)er * page_bytes;
+        for (int c = lane; c < D / 4; c += 32)
+          cp_async16(st + r * row_bytes + c * 16, from + c * 16);
+      }
+    }
+  };
+  // this lane's row and half in ldmatrix.x4: rows 0-7, 8-15, then the next 8 values
+  const uint32_t frag = (lane & 15) * row_bytes + (lane >> 4) * 16;
+  const int begin = chunk * p.chunk_pages + set * kScoreTile, stride = sets * kScoreTile;
+#pragma unroll 1
   for (int h0 = 0; h0 < p.GS; h0 += 8) {
-    // q^- and q^+ of head h0 + g, finite, times the sign of the score scale
-    uint32_t qn[C][4], qp[C][4];
+    int e = entries(begin);
+    if (begin < page_end) issue(e, ring);
+    cp_async_commit();
+    // head h0 + g: values 16 s + 2 t, + 1, + 8, + 9 of [q^- | q^+], finite,
+    // times the sign of the score scale
+    uint32_t qf[S][2];
     {
       const __half* q = static_cast<const __half*>(p.q) +
-                        ((long long)b * p.Hq + (long long)h * p.GS + h0 + g) * p.D + 8 * t;
+                        ((long long)b * p.Hq + (long long)h * p.GS + h0 + g) * D + 2 * t;
       const __half2 zero = __float2half2_rn(0.f), top = __float2half2_rn(65504.f);
       const __half2 sg = __float2half2_rn(p.sign);
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        uint4 u = make_uint4(0u, 0u, 0u, 0u);
-        if (h0 + g < p.GS && 32 * c + 8 * t < p.D)
-          u = __ldg(reinterpret_cast<const uint4*>(q + 32 * c));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      for (int s = 0; s < S; ++s)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          // max and min drop a NaN operand, so a NaN becomes 0 in both halves
-          const __half2 x = *reinterpret_cast<const __half2*>(&w[k]);
-          __half2 pos = __hmin2(__hmax2(x, zero), top);
-          __half2 neg = __hmax2(__hmin2(x, zero), __hneg2(top));
-          if (p.sign <= 0.f) {
-            const __half2 a = __hmul2(neg, sg), z = __hmul2(pos, sg);
-            pos = a;
-            neg = z;
+        for (int k = 0; k < 2; ++k) {
+          const int at = 16 * s + 8 * k;
+          const bool upper = at >= D;
+          qf[s][k] = 0u;
+          if (h0 + g < p.GS && (FULL || at < 2 * D)) {
+            // max and min drop a NaN operand, so a NaN becomes 0 in both halves
+            const __half2 x = __ldg(reinterpret_cast<const __half2*>(q + at - (upper ? D : 0)));
+            __half2 pos = __hmin2(__hmax2(x, zero), top);
+            __half2 neg = __hmax2(__hmin2(x, zero), __hneg2(top));
+            if (p.sign <= 0.f) {
+              const __half2 a = __hmul2(neg, sg), z = __hmul2(pos, sg);
+              pos = a;
+              neg = z;
+            }
+            const __half2 y = upper ? pos : neg;
+            qf[s][k] = *reinterpret_cast<const uint32_t*>(&y);
           }
-          qp[c][k] = *reinterpret_cast<const uint32_t*>(&pos);
-          qn[c][k] = *reinterpret_cast<const uint32_t*>(&neg);
         }
-      }
     }
-    // entries of this warp's next tile, read one tile ahead
-    int p0 = chunk * p.chunk_pages + warp * 16;
-    int next = lane < 16 && p0 + lane < page_end ? table_entry(p, b, p0 + lane) : -1;
-    for (; p0 < page_end; p0 += 64) {
-      const int e0 = __shfl_sync(0xffffffffu, next, g), e1 = __shfl_sync(0xffffffffu, next, g + 8);
-      next = lane < 16 && p0 + 64 + lane < page_end ? table_entry(p, b, p0 + 64 + lane) : -1;
-      const uint4 none = make_uint4(0u, 0u, 0u, 0u);
-      uint4 a[2][2][C];  // [lo, hi][row g, row g + 8][block]
+    uint32_t st = 0;
+#pragma unroll 1
+    for (int p0 = begin; p0 < page_end; p0 += stride) {
+      const int next = entries(p0 + stride);
+      if (p0 + stride < page_end) issue(next, ring + (st ^ stage_bytes));
+      cp_async_commit();
+      cp_async_wait<1>();
+      __syncwarp();
+      float x[2][4] = {}, y[2][4] = {};  // sums and sums of magnitudes, two chains each
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const bool in = 32 * c + 8 * t < p.D;
+      for (int s = 0; s < S; ++s) {
+        if (!FULL && 8 * s >= D) break;
+        uint32_t a[4], m[4];
+        ldsm_x4(ring + st + frag + s * 32, a[0], a[1], a[2], a[3]);
 #pragma unroll
-        for (int side = 0; side < 2; ++side) {
-          const long long off = (long long)side * p.D + 32 * c + 8 * t;
-          a[side][0][c] = in && e0 >= 0 ? __ldg(reinterpret_cast<const uint4*>(
-                                              bounds + e0 * page_stride + off))
-                                        : none;
-          a[side][1][c] = in && e1 >= 0 ? __ldg(reinterpret_cast<const uint4*>(
-                                              bounds + e1 * page_stride + off))
-                                        : none;
-        }
+        for (int k = 0; k < 4; ++k) m[k] = a[k] & 0x7fff7fffu;
+        mma_f16_16816(x[s & 1], a[0], a[1], a[2], a[3], qf[s][0], qf[s][1]);
+        mma_f16_16816(y[s & 1], m[0], m[1], m[2], m[3], qf[s][0] & 0x7fff7fffu,
+                      qf[s][1] & 0x7fff7fffu);
       }
-      float x[4] = {};
-      __half2 mx = __float2half2_rn(0.f);
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int side = 0; side < 2; ++side) {
-          const uint4 u = a[side][0][c], v = a[side][1][c];
-          const uint32_t* qq = side ? qp[c] : qn[c];
-          mma_f16_16816(x, u.x, v.x, u.y, v.y, qq[0], qq[1]);
-          mma_f16_16816(x, u.z, v.z, u.w, v.w, qq[2], qq[3]);
-          if (h0 == 0) {
-            const uint32_t all[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              mx = __hmax2(mx, __habs2(*reinterpret_cast<const __half2*>(&all[k])));
-          }
-        }
-      big = fmaxf(big, fmaxf(__low2float(mx), __high2float(mx)));
+      __syncwarp();  // the stage may be filled again
+      st ^= stage_bytes;
       // heads h0 + 2 t, + 1 of pages g and g + 8: the largest over the group
+      float most = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[0][k] += x[1][k];
+        most = fmaxf(most, y[0][k] + y[1][k]);
+      }
       const bool c0 = h0 + 2 * t < p.GS, c1 = h0 + 2 * t + 1 < p.GS;
-      float r0 = fmaxf(c0 ? x[0] : -INFINITY, c1 ? x[1] : -INFINITY);
-      float r1 = fmaxf(c0 ? x[2] : -INFINITY, c1 ? x[3] : -INFINITY);
-      r0 = fmaxf(r0, __shfl_xor_sync(0xffffffffu, r0, 1));
-      r1 = fmaxf(r1, __shfl_xor_sync(0xffffffffu, r1, 1));
-      r0 = fmaxf(r0, __shfl_xor_sync(0xffffffffu, r0, 2));
-      r1 = fmaxf(r1, __shfl_xor_sync(0xffffffffu, r1, 2));
-      if (t == 0) {
-        if (p0 + g < page_end) {
-          unsigned k = e0 < 0 ? 0u : key_of(r0);
-          if (h0 > 0) k = max(k, keys[p0 + g]);
-          keys[p0 + g] = k;
-        }
-        if (p0 + g + 8 < page_end) {
-          unsigned k = e1 < 0 ? 0u : key_of(r1);
-          if (h0 > 0) k = max(k, keys[p0 + g + 8]);
-          keys[p0 + g + 8] = k;
-        }
+      float s0 = fmaxf(c0 ? x[0][0] : -INFINITY, c1 ? x[0][1] : -INFINITY);
+      float s1 = fmaxf(c0 ? x[0][2] : -INFINITY, c1 ? x[0][3] : -INFINITY);
+      s0 = fmaxf(s0, __shfl_xor_sync(0xffffffffu, s0, 1));
+      s1 = fmaxf(s1, __shfl_xor_sync(0xffffffffu, s1, 1));
+      s0 = fmaxf(s0, __shfl_xor_sync(0xffffffffu, s0, 2));
+      s1 = fmaxf(s1, __shfl_xor_sync(0xffffffffu, s1, 2));
+      most = warp_max(most);
+      const int e0 = __shfl_sync(0xffffffffu, e, g), e1 = __shfl_sync(0xffffffffu, e, g + 8);
+      e = next;
+      // lane 0 of a quad stores page g, lane 1 page g + 8
+      if (t < 2 && p0 + g + 8 * t < page_end) {
+        unsigned k = (t ? e1 : e0) < 0 ? 0u : key_of(t ? s1 : s0);
+        unsigned* dst = keys + p0 + g + 8 * t;
+        if (h0 > 0) k = max(k, *dst);
+        *dst = k;
+      }
+      if (lane == 0) {
+        float* dst = magnitude + p0 / kScoreTile;
+        *dst = h0 > 0 ? fmaxf(*dst, most) : most;
       }
     }
+    cp_async_wait<0>();
+    __syncwarp();
   }
-  big = warp_max(big);
-  if (lane == 0) s_max[warp] = big;
-  __syncthreads();
-  if (threadIdx.x == 0)
-    p.absmax[(long long)row * p.chunks + chunk] =
-        fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
 }
 
 // Every other type and size: one warp per page, lanes across the channels.
@@ -440,43 +491,46 @@ __global__ void __launch_bounds__(128) pa_score_kernel(const SelectParams p) {
       const T* lo = static_cast<const T*>(p.bounds) + ((long long)e * p.Hkv + h) * 2 * p.D;
       float best = -INFINITY;
       for (int x = 0; x < p.GS; ++x) {
-        float s = 0.f;
+        float s = 0.f, m = 0.f;
         for (int d = lane; d < p.D; d += 32) {
           const float qd = p.sign * tame(to_float<T>(q[(long long)x * p.D + d]), top);
           const float l = to_float<T>(lo[d]), u = to_float<T>(lo[p.D + d]);
           s = fmaf(fmaxf(qd, 0.f), u, s);
           s = fmaf(fminf(qd, 0.f), l, s);
-          if (x == 0) big = fmaxf(big, fmaxf(fabsf(l), fabsf(u)));
+          m = fmaf(fabsf(qd), qd > 0.f ? fabsf(u) : fabsf(l), m);
         }
         best = fmaxf(best, warp_sum(s));
+        big = fmaxf(big, warp_sum(m));
       }
       key = key_of(best);
     }
     if (lane == 0) p.keys[(long long)row * p.max_blocks + at] = key;
   }
-  big = warp_max(big);
   if (lane == 0) s_max[warp] = big;
   __syncthreads();
   if (threadIdx.x == 0)
-    p.absmax[(long long)row * p.chunks + chunk] =
+    p.magnitude[(long long)row * p.tiles + chunk] =
         fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
 }
 
 // ════════════════════════════════════════════════════════════════════════
 // Selection, second kernel: one CTA per row.
-//   1. T = the r-th largest fp32 score, by bisection on the ordered keys
-//      (each step one count over the row and one barrier).
-//   2. A score is off by at most E, so T is within E of the true r-th
-//      largest: scores above T + 2 E are in, those below T - 2 E out. When
-//      more lie between than places are left, those few are scored again in
-//      64 bits (products of the operands are exact there) and the best taken,
-//      the earlier page on a tie.
+//   1. A histogram of the fp32 scores' ordered keys over their range finds the
+//      bin that holds the r-th largest.
+//   2. A score is off by at most E, so scores above the bin's end + 2 E are in
+//      and those below its start - 2 E are out. When more lie between than
+//      places are left, those few are scored again in 64 bits (products of the
+//      operands are exact there) and the best taken, the earlier page on a tie.
 //   3. The kept pages go out in order, as per-head page ids.
 // E: a tensor-core step of 16 products and its accumulator is taken to be off
-// by at most 2^-18 of the sum of their magnitudes, a scalar sum by less; with
-// up to 16 steps and that sum at most |q|_1 max |bound|, E = 2^-14 of the
-// latter covers both.
+// by at most 2^-18 of the sum of their magnitudes (17 terms cut at 2^-23 of the
+// largest), a scalar sum by less; over the at most 16 steps of a chain that is
+// 2^-14 of the sum of a score's terms' magnitudes, whose largest of the row the
+// score kernel has left.
+// A row is read once and the code runs through once: what counts is the latency
+// of its dozen barriers and of fetching the code, so loops stay loops.
 // ════════════════════════════════════════════════════════════════════════
+constexpr int kBins = 2048;
 constexpr int kNearCap = 1024;  // near pages that are ranked in shared memory
 
 template <int NT>
@@ -510,18 +564,22 @@ __device__ __forceinline__ K bisect(BlockCount<NT>& s, int& turn, K lo, K hi, in
   return lo;
 }
 
-// NT threads hold the first NT * KPT keys of the row in registers (thread t
-// the pages t, t + NT, ...); a longer row's others are read again each time.
-template <typename T, int NT, int KPT>
-__global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p) {
+// The row's keys stay in shared memory up to kSmemKeys pages (`smem_keys`),
+// longer rows are read again from the workspace.
+constexpr int kSmemKeys = 32768;
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p, int smem_keys) {
   constexpr int NWARP = NT / 32;
+  extern __shared__ unsigned s_keys[];
   __shared__ BlockCount<NT> s_cnt;
-  __shared__ float s_red[2][NWARP];
+  __shared__ float s_red[NWARP];
   __shared__ unsigned s_ends[2];
-  __shared__ int s_near;
+  __shared__ int s_near, s_bin;
   __shared__ unsigned s_near_page[kNearCap];
   __shared__ unsigned long long s_near_key[kNearCap];
-  __shared__ int s_count[KPT * NWARP];
+  __shared__ int s_count[NWARP];
+  __shared__ int s_bins[kBins];
   constexpr float top = sizeof(T) == 2 ? 65504.f : FLT_MAX;
   pdl_wait_primary();
   const int row = blockIdx.x;
@@ -531,41 +589,32 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p) 
                             h == 0 && tid == 0);
   const int n = (int)(((long long)L + p.block_size - 1) / p.block_size);
   const bool scored = n > p.keep;
-  unsigned* keys = p.keys + (long long)row * p.max_blocks;
+  // keys of the row's pages, 0: the table names no page there
+  unsigned* K = p.keys + (long long)row * p.max_blocks;
   const int first = p.sink, last = n - p.recent;  // [first, last): pages that compete
   unsigned take = 1u;  // a competing page with a key of at least this is kept
-  unsigned kr[KPT];    // 0: the table names no page there
-#pragma unroll
-  for (int i = 0; i < KPT; ++i) {
-    const int at = tid + i * NT;
-    kr[i] = 0u;
-    if (at < n) kr[i] = scored ? keys[at] : table_entry(p, b, at) >= 0;
-  }
   if (scored) {
     const int r = p.keep - p.sink - p.recent;
     int turn = 0;
     int mine = 0;
     unsigned kmin = 0xffffffffu, kmax = 0u;
-    // f(page, key) for the competing pages with a key
-    auto each = [&](auto f) {
-#pragma unroll
-      for (int i = 0; i < KPT; ++i) {
-        const int at = tid + i * NT;
-        if (at >= first && at < last && kr[i]) f(at, kr[i]);
+#pragma unroll 4
+    for (int at = tid; at < n; at += NT) {
+      const unsigned k = K[at];
+      if (n <= smem_keys) s_keys[at] = k;
+      if (k && at >= first && at < last) {
+        ++mine;
+        kmin = min(kmin, k);
+        kmax = max(kmax, k);
       }
-      for (int at = tid + KPT * NT; at < last; at += NT)
-        if (at >= first && keys[at]) f(at, keys[at]);
-    };
-    each([&](int, unsigned k) {
-      ++mine;
-      kmin = min(kmin, k);
-      kmax = max(kmax, k);
-    });
+    }
+    if (n <= smem_keys) K = s_keys;  // each thread goes on with the keys it copied
     if (tid == 0) {
       s_ends[0] = 0xffffffffu;
       s_ends[1] = 0u;
       s_near = 0;
     }
+    for (int i = tid; i < kBins; i += NT) s_bins[i] = 0;
     const int eligible = block_sum<NT>(s_cnt, mine, turn);
     if (r <= 0) {
       take = 0xffffffffu;  // no competing page fits; no key is this large
@@ -576,68 +625,101 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p) 
         atomicMin(&s_ends[0], kmin);
         atomicMax(&s_ends[1], kmax);
       }
-      // max |bound| of the row and max over heads of |q|_1
-      float big = 0.f, l1 = 0.f;
-      const int chunks = (n + p.chunk_pages - 1) / p.chunk_pages;
-      for (int i = tid; i < chunks; i += NT)
-        big = fmaxf(big, p.absmax[(long long)row * p.chunks + i]);
-      const T* q = static_cast<const T*>(p.q) + ((long long)b * p.Hq + (long long)h * p.GS) * p.D;
-      for (int x = warp; x < p.GS; x += NWARP) {
-        float s = 0.f;
-        for (int d = lane; d < p.D; d += 32)
-          s += fabsf(tame(to_float<T>(q[(long long)x * p.D + d]), top));
-        l1 = fmaxf(l1, warp_sum(s));
-      }
-      big = warp_max(big);
-      if (lane == 0) {
-        s_red[0][warp] = big;
-        s_red[1][warp] = l1;
+      // the largest sum of magnitudes of the row
+      float most = 0.f;
+      const int tiles = (n + p.tile_pages - 1) / p.tile_pages;
+      for (int i = tid; i < tiles; i += NT)
+        most = fmaxf(most, p.magnitude[(long long)row * p.tiles + i]);
+      most = warp_max(most);
+      if (lane == 0) s_red[warp] = most;
+      __syncthreads();
+      most = warp_max(lane < NWARP ? s_red[lane] : 0.f);
+      // histogram of the keys over [kmin, kmax], each bin 2^shift keys wide
+      kmin = s_ends[0];
+      kmax = s_ends[1];
+      const int shift = max(0, 32 - __clz(kmax - kmin) - 11);
+#pragma unroll 2
+      for (int at = tid; at < last; at += NT) {
+        const unsigned k = at >= first ? K[at] : 0u;
+        if (k) atomicAdd(&s_bins[(k - kmin) >> shift], 1);
       }
       __syncthreads();
-      big = warp_max(lane < NWARP ? s_red[0][lane] : 0.f);
-      l1 = warp_max(lane < NWARP ? s_red[1][lane] : 0.f);
-      const unsigned T32 =
-          bisect<NT, unsigned>(s_cnt, turn, s_ends[0], s_ends[1], r, [&](unsigned t) {
-            int c = 0;
-            each([&](int, unsigned k) { c += k >= t; });
-            return c;
-          });
-      const float E = big * l1 * 0x1p-14f + 0x1p-118f;
-      const float tf = score_of(T32);
-      unsigned near_lo = 1u, near_hi = 0xfffffffeu;
-      if (fabsf(E) < 0x1p126f && fabsf(tf) < 0x1p126f) {
-        near_lo = max(1u, key_of(tf - 2.001f * E));
-        near_hi = key_of(tf + 2.001f * E);
+      // the bin of the r-th largest: a thread's bins, from the top, then the scan
+      constexpr int BPT = kBins / NT;
+      int in_bins = 0;
+#pragma unroll 1
+      for (int i = 0; i < BPT; ++i) in_bins += s_bins[kBins - 1 - (tid * BPT + i)];
+      int upto = in_bins;  // keys in this warp's bins down to this thread's
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
       }
-      int above = 0, near = 0;
-      each([&](int, unsigned k) {
+      if (lane == 31) s_count[warp] = upto;
+      __syncthreads();
+      // keys in the bins of the warps before, and before this thread's
+      int over = __reduce_add_sync(0xffffffffu, lane < warp ? s_count[lane] : 0) + upto - in_bins;
+      if (over < r && over + in_bins >= r) {
+#pragma unroll 1
+        for (int i = 0; over < r; ++i) {
+          s_bin = kBins - 1 - (tid * BPT + i);
+          over += s_bins[s_bin];
+        }
+      }
+      __syncthreads();
+      const unsigned start = kmin + ((unsigned)s_bin << shift);
+      const unsigned end = min(kmax, start + ((1u << shift) - 1u));
+      const float E = most * 0x1p-14f + 0x1p-118f;
+      const float flo = score_of(start), fhi = score_of(end);
+      unsigned near_lo = 1u, near_hi = 0xfffffffeu;
+      if (fabsf(E) < 0x1p126f && fabsf(flo) < 0x1p126f && fabsf(fhi) < 0x1p126f) {
+        near_lo = max(1u, key_of(flo - 2.001f * E));
+        near_hi = key_of(fhi + 2.001f * E);
+      }
+      // pages above, and the list of the near ones: its first kNearCap entries
+      // in shared memory too
+      unsigned* far_page = p.near_page + (long long)row * p.max_blocks;
+      int above = 0;
+#pragma unroll 2
+      for (int at = tid; at < last; at += NT) {
+        const unsigned k = at >= first ? K[at] : 0u;
         above += k > near_hi;
-        near += k >= near_lo && k <= near_hi;
-      });
-      above = block_sum<NT>(s_cnt, above, turn);
-      near = block_sum<NT>(s_cnt, near, turn);
-      const int need = r - above;
+        if (k >= near_lo && k <= near_hi) {
+          const int to = atomicAdd(&s_near, 1);
+          far_page[to] = (unsigned)at;
+          if (to < kNearCap) s_near_page[to] = (unsigned)at;
+        }
+      }
+      const int need = r - block_sum<NT>(s_cnt, above, turn);
+      const int near = s_near;
       take = near_lo;
       if (near > need) {
         const bool few = near <= kNearCap;
-        unsigned* lp = few ? s_near_page : p.near_page + (long long)row * p.max_blocks;
+        const unsigned* lp = few ? s_near_page : far_page;
         unsigned long long* lk = few ? s_near_key : p.near_key + (long long)row * p.max_blocks;
-        each([&](int at, unsigned k) {
-          if (k >= near_lo && k <= near_hi) lp[atomicAdd(&s_near, 1)] = (unsigned)at;
-        });
-        __syncthreads();
+        const T* q =
+            static_cast<const T*>(p.q) + ((long long)b * p.Hq + (long long)h * p.GS) * p.D;
+#pragma unroll 1
         for (int i = warp; i < near; i += NWARP) {
-          const int e = table_entry(p, b, (int)lp[i]);
+          const int e = __ldg(p.block_tables + (long long)b * p.max_blocks + lp[i]);
+          const T* lo = static_cast<const T*>(p.bounds) + ((long long)e * p.Hkv + h) * 2 * p.D;
+          T l[8], u[8];  // D <= 256
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int d = lane + 32 * k;
+            l[k] = d < p.D ? lo[d] : from_float<T>(0.f);
+            u[k] = d < p.D ? lo[p.D + d] : from_float<T>(0.f);
+          }
           double best = -INFINITY;
-          const T* lo = static_cast<const T*>(p.bounds) +
-                        ((long long)(e < 0 ? 0 : e) * p.Hkv + h) * 2 * p.D;
-          for (int x = 0; x < p.GS && e >= 0; ++x) {
+#pragma unroll 2
+          for (int x = 0; x < p.GS; ++x) {
             double s = 0.0;
-            for (int d = lane; d < p.D; d += 32) {
-              const double qd =
-                  (double)(p.sign * tame(to_float<T>(q[(long long)x * p.D + d]), top));
-              s = fma(fmax(qd, 0.0), (double)to_float<T>(lo[p.D + d]), s);
-              s = fma(fmin(qd, 0.0), (double)to_float<T>(lo[d]), s);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int d = lane + 32 * k;
+              if (d >= p.D) break;
+              const float qd = p.sign * tame(to_float<T>(q[(long long)x * p.D + d]), top);
+              s = fma((double)qd, (double)to_float<T>(qd > 0.f ? u[k] : l[k]), s);
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -652,8 +734,9 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p) 
             const unsigned long long k = lk[i];
             const unsigned at = lp[i];
             int rank = 0;
+#pragma unroll 4
             for (int o = 0; o < near; ++o) rank += lk[o] > k || (lk[o] == k && lp[o] < at);
-            keys[at] = rank < need ? near_hi : 0u;
+            K[at] = rank < need ? near_hi : 0u;
           }
         } else {
           const unsigned long long T64 = bisect<NT, unsigned long long>(
@@ -672,97 +755,62 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p) 
                 for (int i = tid; i < near; i += NT) c += lk[i] == T64 && ~lp[i] >= t;
                 return c;
               });
-          for (int i = tid; i < near; i += NT) {
-            const bool in = lk[i] > T64 || (lk[i] == T64 && lp[i] <= cut);
-            keys[lp[i]] = in ? near_hi : 0u;
-          }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < KPT; ++i) {
-          const int at = tid + i * NT;
-          if (at >= first && at < last && kr[i] >= near_lo && kr[i] <= near_hi) kr[i] = keys[at];
+          for (int i = tid; i < near; i += NT)
+            K[lp[i]] = lk[i] > T64 || (lk[i] == T64 && lp[i] <= cut) ? near_hi : 0u;
         }
       }
     }
+    __syncthreads();  // every key is in its final place
   }
-  // ── the kept pages, in order: NT * KPT pages a round ────────────────────
+  // ── the kept pages, in order: a warp's run of pages, then the scan ──────
+  const int run = ((n + NT - 1) / NT) * 32, begin = min(n, warp * run), stop = min(n, begin + run);
+  auto kept = [&](int at) {
+    if (at >= stop) return false;
+    if (!scored) return table_entry(p, b, at) >= 0;
+    const unsigned k = K[at];
+    return at < first || at >= last ? k != 0u : k >= take;
+  };
+  int count = 0;
+#pragma unroll 2
+  for (int at = begin; at < stop; at += 32)
+    count += __popc(__ballot_sync(0xffffffffu, kept(at + lane)));
+  if (lane == 0) s_count[warp] = count;
+  __syncthreads();
+  int to = __reduce_add_sync(0xffffffffu, lane < warp ? s_count[lane] : 0);
+  const int done = __reduce_add_sync(0xffffffffu, lane < NWARP ? s_count[lane] : 0);
   int* tab = p.sel_tables + (long long)row * p.keep;
   int* pages = p.sel_pages ? p.sel_pages + (long long)row * p.keep : nullptr;
-  int done = 0;
   bool tail = false;  // the sequence's last page is kept
-  for (int base = 0; base < n; base += NT * KPT) {
-    unsigned in = 0;  // bit i: page base + tid + i * NT is kept
-    unsigned before[KPT];
-#pragma unroll
-    for (int i = 0; i < KPT; ++i) {
-      const int at = base + tid + i * NT;
-      unsigned k = kr[i];
-      if (base > 0) {
-        k = 0u;
-        if (at < n) k = scored ? keys[at] : table_entry(p, b, at) >= 0;
-      }
-      const bool kept = k && (!scored || at < first || at >= last || k >= take);
-      const unsigned m = __ballot_sync(0xffffffffu, kept);
-      if (kept) in |= 1u << i;
-      before[i] = __popc(m & ((1u << lane) - 1u));
-      if (lane == 0) s_count[i * NWARP + warp] = __popc(m);
+#pragma unroll 2
+  for (int base = begin; base < stop; base += 32) {
+    const int at = base + lane;
+    const bool in = kept(at);
+    const unsigned m = __ballot_sync(0xffffffffu, in);
+    if (in) {
+      const int o = to + __popc(m & ((1u << lane) - 1u));
+      const int e = __ldg(p.block_tables + (long long)b * p.max_blocks + at);
+      tab[o] = (int)((long long)e * p.head_pages + h);
+      if (pages) pages[o] = at;
+      tail |= at == n - 1;
     }
-    __syncthreads();
-    // exclusive sums of s_count, by the first warp
-    constexpr int PER = (KPT * NWARP + 31) / 32;
-    if (warp == 0) {
-      int c[PER], sum = 0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int x = lane * PER + i;
-        c[i] = x < KPT * NWARP ? s_count[x] : 0;
-        sum += c[i];
-      }
-      int pre = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, pre, o);
-        if (lane >= o) pre += y;
-      }
-      if (lane == 31) s_near = pre;
-      pre -= sum;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int x = lane * PER + i;
-        if (x < KPT * NWARP) s_count[x] = pre;
-        pre += c[i];
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < KPT; ++i)
-      if (in >> i & 1u) {
-        const int at = base + tid + i * NT;
-        const int to = done + s_count[i * NWARP + warp] + (int)before[i];
-        const int e = __ldg(p.block_tables + (long long)b * p.max_blocks + at);
-        tab[to] = (int)((long long)e * p.head_pages + h);
-        if (pages) pages[to] = at;
-        if (at == n - 1) tail = true;
-      }
-    done += s_near;
-    __syncthreads();
+    to += __popc(m);
   }
-  tail = __syncthreads_or(tail);
   for (int i = done + tid; i < p.keep; i += NT) {
     tab[i] = -1;
     if (pages) pages[i] = -1;
   }
+  tail = __syncthreads_or(tail);
   if (tid == 0)
     p.sel_lens[row] = done * p.block_size - (tail ? n * p.block_size - L : 0);
 }
 
 template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kern)(KArgs...), long long grid, unsigned block, cudaStream_t st,
-                       Args&&... args) {
+cudaError_t launch_pdl(void (*kern)(KArgs...), long long grid, unsigned block, size_t smem,
+                       cudaStream_t st, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -772,6 +820,26 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), long long grid, unsigned block, c
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
+template <int S, bool FULL>
+cudaError_t launch_score_mma(const SelectParams& p, cudaStream_t st) {
+  constexpr int NW = kScoreWarps;
+  const long long ctas = (long long)p.B * ((p.Hkv + NW - 1) / NW) * p.chunks;
+  auto kern = pa_score_mma_kernel<S, FULL>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)score_smem_bytes(8 * S));
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kern, ctas, NW * 32, score_smem_bytes(p.D), st, p);
+}
+
+template <typename T, int NT>
+cudaError_t launch_select_nt(const SelectParams& p, long long rows, int keys, cudaStream_t st) {
+  auto kern = pa_select_kernel<T, NT>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             kSmemKeys * (int)sizeof(unsigned));
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kern, rows, NT, keys * sizeof(unsigned), st, p, keys);
+}
+
 template <typename T>
 cudaError_t launch_select_t(const SelectParams& p, cudaStream_t st) {
   const long long rows = (long long)p.B * p.Hkv;
@@ -779,28 +847,32 @@ cudaError_t launch_select_t(const SelectParams& p, cudaStream_t st) {
   if (p.max_blocks > p.keep) {
     cudaError_t e;
     if (!p.vec)
-      e = launch_pdl(pa_score_kernel<T>, rows * p.chunks, 128, st, p);
-    else if (p.D <= 64)
-      e = launch_pdl(pa_score_mma_kernel<2>, rows * p.chunks, 128, st, p);
-    else if (p.D <= 128)
-      e = launch_pdl(pa_score_mma_kernel<4>, rows * p.chunks, 128, st, p);
+      e = launch_pdl(pa_score_kernel<T>, rows * p.chunks, 128, 0, st, p);
+    else if (p.D == 64)
+      e = launch_score_mma<8, true>(p, st);
+    else if (p.D == 128)
+      e = launch_score_mma<16, true>(p, st);
+    else if (p.D == 256)
+      e = launch_score_mma<32, true>(p, st);
+    else if (p.D < 128)
+      e = launch_score_mma<16, false>(p, st);
     else
-      e = launch_pdl(pa_score_mma_kernel<8>, rows * p.chunks, 128, st, p);
+      e = launch_score_mma<32, false>(p, st);
     if (e != cudaSuccess) return e;
   }
-  // enough threads that each holds few keys, few enough that a barrier is short
-  if (p.max_blocks <= 1024)
-    return launch_pdl(pa_select_kernel<T, 128, 8>, rows, 128, st, p);
-  return launch_pdl(pa_select_kernel<T, 512, 16>, rows, 512, st, p);
+  const int keys = p.max_blocks > p.keep ? std::min(p.max_blocks, kSmemKeys) : 0;
+  // few threads for short rows, whose barriers are then shorter
+  if (p.max_blocks <= 1024) return launch_select_nt<T, 128>(p, rows, keys, st);
+  return launch_select_nt<T, 512>(p, rows, keys, st);
 }
 
 }  // namespace
 
 cudaError_t launch_bounds(const BoundsParams& p, cudaStream_t st) {
   const long long grid = (long long)p.B * p.pages_per_seq;
-  if (p.kind == kBoundsQ4) return launch_pdl(pa_bounds_q4_kernel, grid, 128, st, p);
-  if (p.kind == kBoundsF32) return launch_pdl(pa_bounds_kernel<float>, grid, 128, st, p);
-  return launch_pdl(pa_bounds_kernel<__half>, grid, 128, st, p);
+  if (p.kind == kBoundsQ4) return launch_pdl(pa_bounds_q4_kernel, grid, 128, 0, st, p);
+  if (p.kind == kBoundsF32) return launch_pdl(pa_bounds_kernel<float>, grid, 128, 0, st, p);
+  return launch_pdl(pa_bounds_kernel<__half>, grid, 128, 0, st, p);
 }
 
 cudaError_t launch_select(const SelectParams& p, int dtype_size, cudaStream_t st) {

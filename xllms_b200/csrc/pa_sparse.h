@@ -42,26 +42,25 @@ struct SelectParams {
   int* sel_pages;   // [B * Hkv][keep] page index within the sequence, -1 past the last; or null
   // workspace
   unsigned* keys;         // [B * Hkv][max_blocks] ordered scores, 0: page not eligible
-  float* absmax;          // [B * Hkv][chunks] largest |bound| seen by the score kernel's CTAs
+  float* magnitude;       // [B * Hkv][tiles] per tile_pages pages, the largest sum of the
+                          // magnitudes of a score's terms
   unsigned* near_page;    // [B * Hkv][max_blocks] pages too near the border for fp32
   unsigned long long* near_key;  // [B * Hkv][max_blocks] their scores in 64 bits
   long long num_blocks;
   long long head_pages;  // kv_block_stride / kv_head_stride
   int B, Hq, Hkv, D, GS, max_blocks, block_size;
   int keep, sink, recent;
-  int chunks, chunk_pages;  // score CTAs per row, pages of each
+  int chunks, chunk_pages;  // score CTAs per row (or 8 rows), pages of each
+  int tiles, tile_pages;    // entries of a row's magnitude, pages of each
   float sign;  // of the score scale: -1, 0 or 1
   int vec;     // fp16, D % 8 == 0, q and bounds on 16-byte boundaries
 };
 
-// Pages of one score CTA: 256 in the tensor-core kernel where that still fills
-// the GPU (four tiles of 16 pages a warp), else 64; 32 in the scalar one, whose
-// warps take a page at a time.
-inline int score_chunk_pages(long long rows, int max_blocks, bool vec, int sms) {
-  if (!vec) return 32;
-  return rows * ((max_blocks + 255) / 256) >= 4LL * sms ? 256 : 64;
-}
-constexpr int kMinScoreChunk = 32;
+// Pages of one score CTA and of one magnitude entry: the tensor-core kernel takes
+// tiles of 16, 128 pages a CTA (8 sequences of 32-128K tokens: 64 pages 80 us
+// with the selection, 128 74, 32 91); the scalar one, whose warps take a page at
+// a time, 32.
+constexpr int kScoreTile = 16, kScoreChunk = 128, kScoreChunkScalar = 32;
 
 cudaError_t launch_select(const SelectParams& p, int dtype_size, cudaStream_t st);
 

@@ -94,13 +94,13 @@ struct SparseCall {
 // further. A row holds few pages here, so the partials of a finer split cost
 // more than an idle SM.
 #ifndef XPA_SPARSE_ITEMS_PER_SM
-#define XPA_SPARSE_ITEMS_PER_SM 8
+#define XPA_SPARSE_ITEMS_PER_SM 3
 #endif
 
 // Workspace: scores and near pages of the selection, the kept pages' tables,
 // the attention's partials, each from a 256-byte boundary.
 struct Layout {
-  size_t keys, absmax, near_page, near_key, tables, lens, part, total;
+  size_t keys, magnitude, near_page, near_key, tables, lens, part, total;
   size_t part_bytes;
 };
 
@@ -115,7 +115,7 @@ Layout layout_of(long long rows, int GS, int D, int max_blocks, int bs, int ds, 
   };
   const size_t scored = max_blocks > keep ? (size_t)rows * max_blocks : 0;
   l.keys = take(scored * sizeof(unsigned));
-  l.absmax = take(scored ? (size_t)rows * ceil_div(max_blocks, xpa::kMinScoreChunk) * sizeof(float) : 0);
+  l.magnitude = take(scored ? (size_t)rows * ceil_div(max_blocks, xpa::kScoreTile) * sizeof(float) : 0);
   l.near_page = take(scored * sizeof(unsigned));
   l.near_key = take(scored * sizeof(unsigned long long));
   if (attention) {
@@ -155,7 +155,7 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
   if (ws && !workspace_aligned(ws)) return NXT_PA_EINVAL;
   const long long rows = (long long)c.B * c.Hkv;
   const int GS = c.Hq / c.Hkv;
-  if (rows * ceil_div(c.max_blocks, xpa::kMinScoreChunk) > INT_MAX || rows * GS > INT_MAX ||
+  if (rows * ceil_div(c.max_blocks, xpa::kScoreChunkScalar) > INT_MAX || rows * GS > INT_MAX ||
       rows * c.keep > INT_MAX)
     return NXT_PA_EINVAL;
   const long long head_pages = c.Hkv > 1 ? c.kbs / c.khs : 1;
@@ -189,7 +189,7 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
   p.sel_lens = attention ? reinterpret_cast<int*>(base + l.lens) : sel_lens;
   p.sel_pages = c.sel_pages;
   p.keys = reinterpret_cast<unsigned*>(base + l.keys);
-  p.absmax = reinterpret_cast<float*>(base + l.absmax);
+  p.magnitude = reinterpret_cast<float*>(base + l.magnitude);
   p.near_page = reinterpret_cast<unsigned*>(base + l.near_page);
   p.near_key = reinterpret_cast<unsigned long long*>(base + l.near_key);
   p.num_blocks = c.num_blocks;
@@ -206,8 +206,10 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
   p.recent = c.recent;
   p.sign = c.scale > 0.f ? 1.f : c.scale < 0.f ? -1.f : 0.f;
   p.vec = c.ds == 2 && c.D % 8 == 0 && aligned(c.q, 16) && aligned(c.bounds, 16);
-  p.chunk_pages = xpa::score_chunk_pages(rows, c.max_blocks, p.vec, sm_count_of(dev));
+  p.chunk_pages = p.vec ? xpa::kScoreChunk : xpa::kScoreChunkScalar;
+  p.tile_pages = p.vec ? xpa::kScoreTile : xpa::kScoreChunkScalar;
   p.chunks = ceil_div(c.max_blocks, p.chunk_pages);
+  p.tiles = ceil_div(c.max_blocks, p.tile_pages);
   const cudaError_t e = xpa::launch_select(p, c.ds, st);
   if (e != cudaSuccess) return map_cuda(e);
   if (!attention) return NXT_PA_OK;
