@@ -318,6 +318,7 @@ template <int S, bool FULL>
 __global__ void __launch_bounds__(kScoreWarps * 32) pa_score_mma_kernel(const SelectParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_wait_primary();
+  pdl_launch_dependents();  // the selection may be scheduled; it waits for this grid
   const int D = FULL ? 8 * S : p.D;
   constexpr int NW = kScoreWarps;
   const int groups = (p.Hkv + NW - 1) / NW;
@@ -475,6 +476,7 @@ __global__ void __launch_bounds__(128) pa_score_kernel(const SelectParams p) {
   __shared__ float s_max[4];
   constexpr float top = sizeof(T) == 2 ? 65504.f : FLT_MAX;
   pdl_wait_primary();
+  pdl_launch_dependents();
   const int row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
   const int b = row / p.Hkv, h = row - b * p.Hkv;
   const int L = clamped_len(p.seq_lens, b, p.max_blocks, p.block_size, nullptr, false);
@@ -492,6 +494,7 @@ __global__ void __launch_bounds__(128) pa_score_kernel(const SelectParams p) {
       float best = -INFINITY;
       for (int x = 0; x < p.GS; ++x) {
         float s = 0.f, m = 0.f;
+#pragma unroll 4
         for (int d = lane; d < p.D; d += 32) {
           const float qd = p.sign * tame(to_float<T>(q[(long long)x * p.D + d]), top);
           const float l = to_float<T>(lo[d]), u = to_float<T>(lo[p.D + d]);
@@ -582,6 +585,8 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p, 
   __shared__ int s_bins[kBins];
   constexpr float top = sizeof(T) == 2 ? 65504.f : FLT_MAX;
   pdl_wait_primary();
+  // No early trigger here: the merge behind the attention reads sel_lens
+  // before it waits for anything, so nothing may start until they are written.
   const int row = blockIdx.x;
   const int b = row / p.Hkv, h = row - b * p.Hkv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -711,19 +716,28 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p, 
             u[k] = d < p.D ? lo[p.D + d] : from_float<T>(0.f);
           }
           double best = -INFINITY;
-#pragma unroll 2
-          for (int x = 0; x < p.GS; ++x) {
-            double s = 0.0;
+#pragma unroll 1
+          for (int x0 = 0; x0 < p.GS; x0 += 4) {  // four heads' sums side by side
+            double s[4] = {};
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const int d = lane + 32 * k;
-              if (d >= p.D) break;
-              const float qd = p.sign * tame(to_float<T>(q[(long long)x * p.D + d]), top);
-              s = fma((double)qd, (double)to_float<T>(qd > 0.f ? u[k] : l[k]), s);
+              T qx[4];  // all four loads before their use
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                qx[x] = d < p.D ? q[(long long)min(x0 + x, p.GS - 1) * p.D + d]
+                                : from_float<T>(0.f);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float qd = p.sign * tame(to_float<T>(qx[x]), top);
+                s[x] = fma((double)qd, (double)to_float<T>(qd > 0.f ? u[k] : l[k]), s[x]);
+              }
             }
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            best = fmax(best, s);
+            for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) s[x] += __shfl_xor_sync(0xffffffffu, s[x], o);
+            best = fmax(best, fmax(fmax(s[0], s[1]), fmax(s[2], s[3])));
           }
           if (lane == 0) lk[i] = key_of(best);
         }
@@ -780,20 +794,22 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p, 
   const int done = __reduce_add_sync(0xffffffffu, lane < NWARP ? s_count[lane] : 0);
   int* tab = p.sel_tables + (long long)row * p.keep;
   int* pages = p.sel_pages ? p.sel_pages + (long long)row * p.keep : nullptr;
-  bool tail = false;  // the sequence's last page is kept
 #pragma unroll 2
   for (int base = begin; base < stop; base += 32) {
-    const int at = base + lane;
-    const bool in = kept(at);
+    const bool in = kept(base + lane);
     const unsigned m = __ballot_sync(0xffffffffu, in);
-    if (in) {
-      const int o = to + __popc(m & ((1u << lane) - 1u));
-      const int e = __ldg(p.block_tables + (long long)b * p.max_blocks + at);
-      tab[o] = (int)((long long)e * p.head_pages + h);
-      if (pages) pages[o] = at;
-      tail |= at == n - 1;
-    }
+    if (in) tab[to + __popc(m & ((1u << lane) - 1u))] = base + lane;
     to += __popc(m);
+  }
+  __syncthreads();
+  // page indices -> per-head page ids, all table reads at once
+  bool tail = false;  // the sequence's last page is kept
+  for (int i = tid; i < done; i += NT) {
+    const int at = tab[i];
+    const int e = __ldg(p.block_tables + (long long)b * p.max_blocks + at);
+    if (pages) pages[i] = at;
+    tail |= at == n - 1;
+    tab[i] = (int)((long long)e * p.head_pages + h);
   }
   for (int i = done + tid; i < p.keep; i += NT) {
     tab[i] = -1;
