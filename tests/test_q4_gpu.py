@@ -82,7 +82,8 @@ def test_write_stores_the_formats_bytes_and_read_returns_its_values(cuda, T, hkv
     torch.cuda.synchronize()
 
 
-@pytest.mark.parametrize("ps", [1.0, 0.37, 2.0 ** -9])
+@pytest.mark.parametrize("ps", [1.0, 0.37, 2.0 ** -9, 0.0119, 7.7, float.fromhex("0x1.fffffep-7"),
+                                1e-30, 1e25])
 def test_every_fp16_value_is_encoded_as_the_format_says(cuda, ps):
     """All finite fp16 bit patterns, infinities and a NaN, in groups whose largest element varies."""
     bits = np.arange(65536).astype(np.uint16)

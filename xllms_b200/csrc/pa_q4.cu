@@ -13,86 +13,130 @@ namespace xpa {
 namespace {
 
 // ════════════════════════════════════════════════════════════════════════
-// Rows <-> tiles. One warp per (token, KV head); a lane holds 8 channels of
-// the K row (lanes below D / 8) or of the V row (the lanes after), so at
-// D = 128 a warp is full and a group's maximum is one shuffle away.
+// Rows <-> tiles. A token's K and V rows are pieces of 8 channels, head by head,
+// K before V; a lane takes a piece, neighbouring lanes a 16-channel group, and
+// a warp P times 32 pieces, whose reads are all in flight together: four where
+// that still leaves the GPU warps enough, one for the few tokens of a decode
+// step, whose time is the chain of one piece.
 // ════════════════════════════════════════════════════════════════════════
+
 struct RowAt {
-  int t, h;           // token, KV head
-  long long tile;     // byte offset of the 16-token tile in its pool
-  int tok;            // token's row in the tile
+  long long tile;  // byte offset of the 16-token tile in its pool, head 0
+  int tok;         // token's row in the tile
 };
 
-__device__ __forceinline__ bool q4_row_at(const Q4RowsParams& a, long long w, RowAt& r) {
-  r.t = (int)(w / a.Hkv);
-  r.h = (int)(w - (long long)r.t * a.Hkv);
-  const long long slot = a.slots[r.t];
+__device__ __forceinline__ bool q4_row_at(const Q4RowsParams& a, int t, RowAt& r) {
+  const long long slot = __ldg(a.slots + t);
   if (slot < 0 || slot >= a.num_slots) return false;
   const long long page = slot / a.block_size;
   const int s = (int)(slot - page * a.block_size);
-  r.tile = page * a.kv_block_stride + (long long)r.h * a.kv_head_stride +
-           (long long)(s >> 4) * (9 * a.D);
+  r.tile = page * a.kv_block_stride + (long long)(s >> 4) * (9 * a.D);
   r.tok = s & 15;
   return true;
 }
 
+// Piece j of a token: its head, its K or V row, its 8 channels.
+struct Piece {
+  int h, v;
+  bool is_v;
+};
+__device__ __forceinline__ Piece q4_piece(const Q4RowsParams& a, int j) {
+  const int per_head = a.D / 4;  // pieces of K and V
+  Piece c;
+  c.h = a.D == 128 ? j >> 5 : j / per_head;
+  const int i = j - c.h * per_head;
+  c.is_v = i >= per_head / 2;
+  c.v = c.is_v ? i - per_head / 2 : i;
+  return c;
+}
+
+// x / y rounded to nearest, from r = 1 / y rounded to nearest: the quotient
+// estimate's residual is exact in one fused step and corrects it (Markstein,
+// IBM J. Res. Dev. 34, 1990; y > 0, its significand not all ones, nothing near
+// the range's ends). The sign is x's, a zero's too.
+__device__ __forceinline__ float div_by(float x, float y, float r) {
+  const float q = x * r;
+  return copysignf(fmaf(fmaf(-q, y, x), r, q), x);
+}
+
+template <int P>
 __global__ void __launch_bounds__(128) pa_q4_write_kernel(const Q4RowsParams a) {
-  const long long w = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int w = (int)(((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5);
   const int lane = threadIdx.x & 31;
-  if (w >= (long long)a.num_tokens * a.Hkv) return;
+  const int t = w / a.warps_per_token, first = (w - t * a.warps_per_token) * 32 * P;
+  if (t >= a.num_tokens) return;
+  const int pieces = a.Hkv * (a.D / 4);
   RowAt r;
-  if (!q4_row_at(a, w, r)) return;
-  const int NV = a.D / 8;  // 8-channel pieces of a row, an even number
-  const long long src = (long long)r.t * a.token_stride + (long long)r.h * a.D;
-  for (int i0 = 0; i0 < 2 * NV; i0 += 32) {
-    const int i = i0 + lane;
-    const bool act = i < 2 * NV, is_v = i >= NV;
-    const int v = is_v ? i - NV : i;
-    const __half* row = static_cast<const __half*>(is_v ? a.value : a.key) + src + v * 8;
-    const float ps = is_v ? a.v_scale : a.k_scale;
-    float x[8];
-    float amax = 0.f;
-    if (act) {
-      if (a.vec16) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(row));
-        const uint32_t q[4] = {u.x, u.y, u.z, u.w};
+  const bool live = q4_row_at(a, t, r);
+  uint4 x4[P];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 f = unpack_half2(q[k]);
-          x[2 * k] = f.x;
-          x[2 * k + 1] = f.y;
-        }
-      } else {
+  for (int k = 0; k < P; ++k) {
+    const int j = first + 32 * k + lane;
+    x4[k] = make_uint4(0u, 0u, 0u, 0u);
+    if (j >= pieces) continue;
+    const Piece c = q4_piece(a, j);
+    const __half* row = static_cast<const __half*>(c.is_v ? a.value : a.key) +
+                        (long long)t * a.token_stride + (long long)c.h * a.D + c.v * 8;
+    if (a.vec16) {
+      x4[k] = __ldg(reinterpret_cast<const uint4*>(row));
+    } else {
+      const unsigned short* u = reinterpret_cast<const unsigned short*>(row);
+      x4[k] = make_uint4(u[0] | ((uint32_t)u[1] << 16), u[2] | ((uint32_t)u[3] << 16),
+                         u[4] | ((uint32_t)u[5] << 16), u[6] | ((uint32_t)u[7] << 16));
+    }
+  }
+  if (!live) return;  // warp-uniform
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = __half2float(row[k]);
-      }
+  for (int k = 0; k < P; ++k) {
+    const int j = first + 32 * k + lane;
+    if (first + 32 * k >= pieces) break;  // warp-uniform
+    const Piece c = q4_piece(a, j);
+    const float ps = c.is_v ? a.v_scale : a.k_scale, inv = c.is_v ? a.v_inverse : a.k_inverse;
+    const uint32_t u[4] = {x4[k].x, x4[k].y, x4[k].z, x4[k].w};
+    float x[8], amax = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        x[k] = isnan(x[k]) ? 0.f : __fdiv_rn(x[k], ps);
-        amax = fmaxf(amax, fabsf(x[k]));
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack_half2(u[i]);
+      x[2 * i] = a.divide ? __fdiv_rn(f.x, ps) : div_by(f.x, ps, inv);
+      x[2 * i + 1] = a.divide ? __fdiv_rn(f.y, ps) : div_by(f.y, ps, inv);
+    }
+    // A quotient that is an infinity or a NaN (an infinity's residual is one)
+    // stands for an infinity, here any value whose scale saturates, or a NaN: 0.
+    constexpr float kHuge = 1e30f;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) odd |= !(fabsf(x[i]) < kHuge);
+    if (odd) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 f = unpack_half2(u[i >> 1]);
+        const float y = i & 1 ? f.y : f.x;
+        if (!(fabsf(x[i]) < kHuge)) x[i] = isnan(y) ? 0.f : copysignf(kHuge, y);
       }
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
     // a 16-channel group is two neighbouring lanes (pieces 2 g, 2 g + 1)
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    if (!act) continue;
+    if (j >= pieces) continue;
     const uint32_t sb = q4_scale(amax);
     const float s = fp8_to_float<kKvE4M3>((uint8_t)sb);
+    const float si = s > 0.f ? __frcp_rn(s) : 0.f;  // no scale: all codes 0
     uint32_t code = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float p = s > 0.f ? __fdiv_rn(x[2 * k], s) : 0.f;
-      const float q = s > 0.f ? __fdiv_rn(x[2 * k + 1], s) : 0.f;
-      code |= q4_pair(p, q) << (8 * k);
-    }
-    uint8_t* tile = static_cast<uint8_t*>(is_v ? a.value_cache : a.key_cache) + r.tile;
-    if (is_v) {
-      *reinterpret_cast<uint32_t*>(tile + q4_v_off(a.D, r.tok, v)) = code;
-      if ((v & 1) == 0) tile[q4_v_scale_off(a.D, r.tok, v >> 1)] = (uint8_t)sb;
+    for (int i = 0; i < 4; ++i)
+      code |= q4_pair(div_by(x[2 * i], s, si), div_by(x[2 * i + 1], s, si)) << (8 * i);
+    uint8_t* tile = static_cast<uint8_t*>(c.is_v ? a.value_cache : a.key_cache) + r.tile +
+                    (long long)c.h * a.kv_head_stride;
+    if (!(s > 0.f)) code = 0;
+    if (c.is_v) {
+      *reinterpret_cast<uint32_t*>(tile + q4_v_off(a.D, r.tok, c.v)) = code;
+      if ((c.v & 1) == 0) tile[q4_v_scale_off(a.D, r.tok, c.v >> 1)] = (uint8_t)sb;
     } else {
-      uint8_t* dst = tile + q4_k_off(a.D, r.tok, v);
+      uint8_t* dst = tile + q4_k_off(a.D, r.tok, c.v);
       *reinterpret_cast<uint16_t*>(dst) = (uint16_t)code;
       *reinterpret_cast<uint16_t*>(dst + a.D / 8) = (uint16_t)(code >> 16);
-      if ((v & 1) == 0) tile[q4_k_scale_off(a.D, r.tok, v >> 1)] = (uint8_t)sb;
+      if ((c.v & 1) == 0) tile[q4_k_scale_off(a.D, r.tok, c.v >> 1)] = (uint8_t)sb;
     }
   }
 }
@@ -103,49 +147,56 @@ __device__ __forceinline__ float q4_value(float cs, float ps) {
   return fminf(fmaxf(cs * ps, -65504.f), 65504.f);
 }
 
+template <int P>
 __global__ void __launch_bounds__(128) pa_q4_read_kernel(const Q4RowsParams a) {
-  const long long w = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int w = (int)(((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5);
   const int lane = threadIdx.x & 31;
-  if (w >= (long long)a.num_tokens * a.Hkv) return;
+  const int t = w / a.warps_per_token, first = (w - t * a.warps_per_token) * 32 * P;
+  if (t >= a.num_tokens) return;
+  const int pieces = a.Hkv * (a.D / 4);
   RowAt r;
-  const bool live = q4_row_at(a, w, r);
-  const int NV = a.D / 8;
-  const long long dst0 = (long long)r.t * a.token_stride + (long long)r.h * a.D;
-  for (int i = lane; i < 2 * NV; i += 32) {
-    const bool is_v = i >= NV;
-    const int v = is_v ? i - NV : i;
-    uint4 u = make_uint4(0u, 0u, 0u, 0u);
-    if (live) {
-      const uint8_t* tile = static_cast<const uint8_t*>(is_v ? a.value_cache : a.key_cache) + r.tile;
-      uint32_t code, sb;
-      if (is_v) {
-        code = *reinterpret_cast<const uint32_t*>(tile + q4_v_off(a.D, r.tok, v));
-        sb = tile[q4_v_scale_off(a.D, r.tok, v >> 1)];
-      } else {
-        const uint8_t* at = tile + q4_k_off(a.D, r.tok, v);
-        code = *reinterpret_cast<const uint16_t*>(at) |
-               ((uint32_t) * reinterpret_cast<const uint16_t*>(at + a.D / 8) << 16);
-        sb = tile[q4_k_scale_off(a.D, r.tok, v >> 1)];
-      }
-      const float s = fp8_to_float<kKvE4M3>((uint8_t)sb);
-      const float ps = is_v ? a.v_scale : a.k_scale;
-      uint32_t h[4], o[4];
-      q4x8_to_h2(code, h);
+  const bool live = q4_row_at(a, t, r);
+  uint32_t code[P], sb[P];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 f = unpack_half2(h[k]);
-        o[k] = pack_half2(q4_value(f.x * s, ps), q4_value(f.y * s, ps));
-      }
-      u = make_uint4(o[0], o[1], o[2], o[3]);
-    }
-    __half* dst = static_cast<__half*>(is_v ? a.value : a.key) + dst0 + v * 8;
-    if (a.vec16) {
-      *reinterpret_cast<uint4*>(dst) = u;
+  for (int k = 0; k < P; ++k) {
+    const int j = first + 32 * k + lane;
+    code[k] = sb[k] = 0u;  // a row of zeros
+    if (!live || j >= pieces) continue;
+    const Piece c = q4_piece(a, j);
+    const uint8_t* tile = static_cast<const uint8_t*>(c.is_v ? a.value_cache : a.key_cache) +
+                          r.tile + (long long)c.h * a.kv_head_stride;
+    if (c.is_v) {
+      code[k] = __ldg(reinterpret_cast<const uint32_t*>(tile + q4_v_off(a.D, r.tok, c.v)));
+      sb[k] = __ldg(tile + q4_v_scale_off(a.D, r.tok, c.v >> 1));
     } else {
-      const uint32_t o[4] = {u.x, u.y, u.z, u.w};
+      const uint8_t* at = tile + q4_k_off(a.D, r.tok, c.v);
+      code[k] = __ldg(reinterpret_cast<const uint16_t*>(at)) |
+                ((uint32_t)__ldg(reinterpret_cast<const uint16_t*>(at + a.D / 8)) << 16);
+      sb[k] = __ldg(tile + q4_k_scale_off(a.D, r.tok, c.v >> 1));
+    }
+  }
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        dst[k] = __ushort_as_half((unsigned short)(o[k >> 1] >> (16 * (k & 1))));
+  for (int k = 0; k < P; ++k) {
+    const int j = first + 32 * k + lane;
+    if (j >= pieces) break;
+    const Piece c = q4_piece(a, j);
+    const float s = fp8_to_float<kKvE4M3>((uint8_t)sb[k]);
+    const float ps = c.is_v ? a.v_scale : a.k_scale;
+    uint32_t h[4], o[4];
+    q4x8_to_h2(code[k], h);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack_half2(h[i]);
+      o[i] = live ? pack_half2(q4_value(f.x * s, ps), q4_value(f.y * s, ps)) : 0u;
+    }
+    __half* dst = static_cast<__half*>(c.is_v ? a.value : a.key) +
+                  (long long)t * a.token_stride + (long long)c.h * a.D + c.v * 8;
+    if (a.vec16) {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        dst[i] = __ushort_as_half((unsigned short)(o[i >> 1] >> (16 * (i & 1))));
     }
   }
 }
@@ -882,16 +933,31 @@ cudaError_t launch_q4_attention(const Params& p, cudaStream_t st) {
   return launch_q4_t<4, 1, false>(p, st);
 }
 
-cudaError_t launch_q4_write(const Q4RowsParams& a, cudaStream_t st) {
-  const long long warps = (long long)a.num_tokens * a.Hkv;
-  pa_q4_write_kernel<<<(unsigned)((warps + 3) / 4), 128, 0, st>>>(a);
+namespace {
+
+// Launches one of a rows kernel's two forms: four pieces a lane from 8 warps of
+// them per SM on (8192 tokens x 8 heads x 128, write and read: one 51 us, four
+// XX us; 64 tokens: 4.7 against 8.2 us).
+cudaError_t launch_rows(void (*one)(Q4RowsParams), void (*four)(Q4RowsParams),
+                        const Q4RowsParams& a, cudaStream_t st) {
+  Q4RowsParams p = a;
+  const int pieces = a.Hkv * (a.D / 4);
+  const long long steps = (long long)a.num_tokens * ((pieces + 31) / 32);
+  const int P = steps >= 4LL * 8 * a.sms ? 4 : 1;
+  p.warps_per_token = (pieces + 32 * P - 1) / (32 * P);
+  const unsigned grid = (unsigned)(((long long)a.num_tokens * p.warps_per_token + 3) / 4);
+  (P == 4 ? four : one)<<<grid, 128, 0, st>>>(p);
   return cudaGetLastError();
 }
 
+}  // namespace
+
+cudaError_t launch_q4_write(const Q4RowsParams& a, cudaStream_t st) {
+  return launch_rows(pa_q4_write_kernel<1>, pa_q4_write_kernel<4>, a, st);
+}
+
 cudaError_t launch_q4_read(const Q4RowsParams& a, cudaStream_t st) {
-  const long long warps = (long long)a.num_tokens * a.Hkv;
-  pa_q4_read_kernel<<<(unsigned)((warps + 3) / 4), 128, 0, st>>>(a);
-  return cudaGetLastError();
+  return launch_rows(pa_q4_read_kernel<1>, pa_q4_read_kernel<4>, a, st);
 }
 
 }  // namespace xpa

@@ -20,6 +20,10 @@ struct Q4RowsParams {
   int num_tokens, Hkv, D, block_size;
   int vec16;  // every row starts on a 16-byte boundary
   float k_scale, v_scale;
+  float k_inverse, v_inverse;  // 1 / scale rounded to nearest
+  int divide;                  // 1: divide by the scales instead
+  int sms;
+  int warps_per_token;  // set by the launchers
 };
 
 cudaError_t launch_q4_write(const Q4RowsParams& a, cudaStream_t st);

@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstring>
 #include <numeric>
 
 #include "operator_api.h"
@@ -19,6 +20,15 @@ int map_cuda(cudaError_t e) { return e == cudaSuccess ? NXT_PA_OK : NXT_PA_ECUDA
 bool scale_ok(float s) { return s > 0.f && std::isfinite(s); }
 
 bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// 1 / s for the kernel's corrected quotient, which needs a significand that is
+// not all ones and room at both ends of the range; 0: divide.
+float inverse_of(float s) {
+  uint32_t u;
+  std::memcpy(&u, &s, sizeof u);
+  const bool ones = (u & 0x7fffffu) == 0x7fffffu;
+  return ones || s < 0x1p-60f || s > 0x1p60f ? 0.f : 1.f / s;
+}
 
 // What every call on 4-bit pools needs of them.
 int check_pools(const void* k, const void* v, int Hkv, int D, int bs, float ks, float vs,
@@ -39,7 +49,7 @@ int rows_call(bool write, void* key, void* value, void* kc, void* vc, const int6
   if (rc != NXT_PA_OK) return rc;
   if (!key || !value || !slots || token_stride < (int64_t)Hkv * D) return NXT_PA_EINVAL;
   if (!aligned(key, 2) || !aligned(value, 2)) return NXT_PA_EINVAL;
-  if ((long long)T * Hkv > INT_MAX) return NXT_PA_EINVAL;  // warps of one grid
+  if ((long long)T * Hkv > INT_MAX / 2) return NXT_PA_EINVAL;  // warps of one grid
   xpa::Q4RowsParams a{};
   a.key = key;
   a.value = value;
@@ -57,6 +67,12 @@ int rows_call(bool write, void* key, void* value, void* kc, void* vc, const int6
   a.num_slots = num_blocks > 0 ? num_blocks * bs : LLONG_MAX;
   a.k_scale = ks;
   a.v_scale = vs;
+  a.k_inverse = inverse_of(ks);
+  a.v_inverse = inverse_of(vs);
+  a.divide = a.k_inverse == 0.f || a.v_inverse == 0.f;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return NXT_PA_ECUDA;
+  a.sms = sm_count_of(dev);
   return map_cuda(write ? xpa::launch_q4_write(a, st) : xpa::launch_q4_read(a, st));
 }
 
