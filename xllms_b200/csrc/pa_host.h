@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <stddef.h>
 
+#include <atomic>
 #include <mutex>
 
 namespace xpa {
@@ -70,6 +71,24 @@ bool fast_layout_ok(const void* k, const void* v, int D, int Hkv, long long kbs,
 int check_args(const void* out, const void* q, const void* k, const void* v, const int* bt,
                const int* sl, int B, int Hq, int D, int Hkv, int max_blocks, int bs, int ds,
                long long kbs, long long khs);
+
+// Raises a kernel's dynamic shared memory limit once per device (`done` is the
+// kernel's own set of devices), with all of the L1 / shared storage as shared
+// memory when `carve`.
+template <typename Kernel>
+cudaError_t smem_limit(Kernel kern, size_t bytes, bool carve, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess && carve)
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout,
+                             (int)cudaSharedmemCarveoutMaxShared);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 // The library status word of device `dev` (the current device).
 int status_word(int dev, int** out);

@@ -5,6 +5,7 @@
 #include <type_traits>
 #include <utility>
 
+#include "pa_host.h"
 #include "pa_q4.cuh"
 #include "pa_q4.h"
 
@@ -890,11 +891,8 @@ cudaError_t launch_q4_t(const Params& p, cudaStream_t st) {
   constexpr int MINB = (EXACT && W <= 2 && NT == 1) ? XPA_Q4_MIN_CTAS : 1;
   using C = Q4Cfg<W, NT, EXACT, NW, STAGES, U>;
   auto kern = pa_q4_kernel<W, NT, EXACT, NW, STAGES, U, MINB>;
-  cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
-  if (e != cudaSuccess) return e;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout,
-                           (int)cudaSharedmemCarveoutMaxShared);
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t e = host::smem_limit(kern, C::kSmem, true, done);
   if (e != cudaSuccess) return e;
   // addresses in the largest unit that divides a page's and a tile's bytes
   Q4Units q;

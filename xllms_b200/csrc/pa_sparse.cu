@@ -12,6 +12,7 @@
 #include <climits>
 #include <utility>
 
+#include "pa_host.h"
 #include "pa_q4.cuh"
 #include "pa_sparse.h"
 
@@ -841,8 +842,8 @@ cudaError_t launch_score_mma(const SelectParams& p, cudaStream_t st) {
   constexpr int NW = kScoreWarps;
   const long long ctas = (long long)p.B * ((p.Hkv + NW - 1) / NW) * p.chunks;
   auto kern = pa_score_mma_kernel<S, FULL>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)score_smem_bytes(8 * S));
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t e = host::smem_limit(kern, score_smem_bytes(8 * S), false, done);
   if (e != cudaSuccess) return e;
   return launch_pdl(kern, ctas, NW * 32, score_smem_bytes(p.D), st, p);
 }
@@ -850,8 +851,8 @@ cudaError_t launch_score_mma(const SelectParams& p, cudaStream_t st) {
 template <typename T, int NT>
 cudaError_t launch_select_nt(const SelectParams& p, long long rows, int keys, cudaStream_t st) {
   auto kern = pa_select_kernel<T, NT>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             kSmemKeys * (int)sizeof(unsigned));
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t e = host::smem_limit(kern, kSmemKeys * sizeof(unsigned), false, done);
   if (e != cudaSuccess) return e;
   return launch_pdl(kern, rows, NT, keys * sizeof(unsigned), st, p, keys);
 }

@@ -552,135 +552,164 @@ def paged_attention_fp8_append(query, key_cache, value_cache, block_tables, seq_
 
 
 # ── 4-bit KV cache ─────────────────────────────────────────────────────────
-@contextlib.contextmanager
-def _launching(like, stream):
-    """Makes `like`'s device current and yields the stream pointer to launch
-    on; tensors made inside belong to that stream, so that the allocator gives
-    their memory to no one else while the kernels run."""
+# The calls below take microseconds on the device for a decode step, so what the
+# host does per call counts: native functions are looked up once, and devices
+# are compared by index (-1: not CUDA).
+_functions = {}
+
+
+def _native_call(name, *args):
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(_native.xpa(), name)
+    rc = fn(*args)
+    if rc != _native.NXT_PA_OK:
+        raise PagedAttentionError(rc, name)
+
+
+def _launch_on(device, stream):
+    """(stream pointer, what to close after the call or None): `device` is
+    current until then, and tensors made until then belong to the stream, so
+    that the allocator gives their memory to no one else while kernels run."""
     import torch
-    with torch.cuda.device(like.device):
-        if stream is None:
-            yield torch.cuda.current_stream().cuda_stream
-            return
-        st = torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream
-        with torch.cuda.stream(st):
-            yield st.cuda_stream
+    if stream is None and torch._C._cuda_getDevice() == device:
+        return torch._C._cuda_getCurrentRawStream(device), None
+    leave = contextlib.ExitStack()
+    leave.enter_context(torch.cuda.device(device))
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(device), leave
+    if isinstance(stream, int):
+        # a raw 0 is the legacy default stream, which torch calls its default
+        stream = (torch.cuda.ExternalStream(stream, device=device) if stream
+                  else torch.cuda.default_stream(device))
+    leave.enter_context(torch.cuda.stream(stream))
+    return stream.cuda_stream, leave
+
+
+def _refuse(where, msg):
+    raise PagedAttentionError(_native.NXT_PA_EINVAL, f"{where}: {msg}")
+
+
+def _opt_ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def q4_pool_shape(num_blocks, num_kv_heads, block_size, head_size):
     """Shape of a 4-bit K or V pool (uint8): [num_blocks, Hkv, block_size / 16,
     9 * head_size], one row of bytes per 16 tokens (include/operator_api.h)."""
     if block_size <= 0 or block_size % 16 or head_size <= 0 or head_size % 16 or head_size > 256:
-        raise PagedAttentionError(_native.NXT_PA_EINVAL, "q4_pool_shape: block_size and head_size "
-                                  "must be multiples of 16, head_size at most 256")
+        _refuse("q4_pool_shape", "block_size and head_size must be multiples of 16, head_size at "
+                "most 256")
     return (num_blocks, num_kv_heads, block_size // 16, 9 * head_size)
 
 
-def _check_q4_pools(where, key_cache, value_cache, like):
-    """(num_blocks, Hkv, block_size, head_size) of two 4-bit pools."""
+def _q4_dims(where, key_cache, value_cache, device):
+    """(num_blocks, Hkv, block size, head size, page and head strides) of 4-bit pools."""
     import torch
-    for c in (key_cache, value_cache):
-        if (c.dim() != 4 or c.dtype != torch.uint8 or c.shape[3] % 144 or not c.shape[3]
-                or c.shape[3] > 9 * 256 or tuple(c.shape) != tuple(key_cache.shape)
-                or not c.is_contiguous() or not c.is_cuda or c.device != like.device):
-            raise PagedAttentionError(
-                _native.NXT_PA_EINVAL, f"{where}: 4-bit pools must be contiguous uint8 [num_blocks, "
-                "Hkv, block_size / 16, 9 * head_size] on the rows' device")
-    nb, hkv, spp, tile = key_cache.shape
-    return nb, hkv, 16 * spp, tile // 9
+    shape = key_cache.shape
+    if (len(shape) != 4 or value_cache.shape != shape or key_cache.dtype != torch.uint8
+            or value_cache.dtype != torch.uint8 or shape[3] % 144 or not 0 < shape[3] <= 2304
+            or not key_cache.is_contiguous() or not value_cache.is_contiguous() or device < 0
+            or key_cache.get_device() != device or value_cache.get_device() != device):
+        _refuse(where, "4-bit pools must be contiguous uint8 [num_blocks, Hkv, block_size / 16, "
+                "9 * head_size] on one CUDA device")
+    nb, hkv, spp, tile = shape
+    return nb, hkv, 16 * spp, tile // 9, hkv * spp * tile, spp * tile
 
 
-def _q4_strides(hkv, bs, d):
-    return hkv * bs * d * 9 // 16, bs * d * 9 // 16
-
-
-def _check_rows(where, key, value, slots, heads, dim):
+def _row_stride(where, key, value, slots, heads, dim, device):
     import torch
-    if (key.dim() != 3 or tuple(key.shape[1:]) != (heads, dim) or key.shape != value.shape
-            or key.dtype != torch.float16 or value.dtype != torch.float16
-            or (key.shape[0] and (key.stride(2) != 1 or (heads > 1 and key.stride(1) != dim)
-                                  or (key.shape[0] > 1 and key.stride(0) < heads * dim)
-                                  or key.stride() != value.stride()))
-            or not key.is_cuda or value.device != key.device
-            or not _index_ok(slots, key.shape[0], key)):
-        raise PagedAttentionError(_native.NXT_PA_EINVAL, f"{where}: rows must be fp16 [T, Hkv, D] "
-                                  "with dense heads and slot_mapping int64 [T], on one device")
-    return key.stride(0) if key.shape[0] > 1 else heads * dim
+    T = key.shape[0] if key.dim() == 3 else -1
+    ks = key.stride()
+    if (key.shape != (T, heads, dim) or value.shape != key.shape or key.dtype != torch.float16
+            or value.dtype != torch.float16 or value.stride() != ks
+            or (T and (ks[2] != 1 or (heads > 1 and ks[1] != dim)
+                       or (T > 1 and ks[0] < heads * dim)))
+            or slots.dtype != torch.int64 or slots.numel() < T or not slots.is_contiguous()
+            or device < 0 or key.get_device() != device or value.get_device() != device
+            or slots.get_device() != device):
+        _refuse(where, "rows must be fp16 [T, Hkv, D] with dense heads and slot_mapping int64 [T], "
+                "on the pools' CUDA device")
+    return ks[0] if T > 1 else heads * dim
 
 
 def reshape_and_cache_q4(key, value, key_cache, value_cache, slot_mapping, k_scale, v_scale,
                          stream=None) -> None:
     """Quantise fp16 key/value [T, Hkv, D] into 4-bit pools (q4_pool_shape) at
     slot_mapping[t] (int64; negative or past the pools: skipped; distinct)."""
-    nb, hkv, bs, d = _check_q4_pools("reshape_and_cache_q4", key_cache, value_cache, key)
-    ts = _check_rows("reshape_and_cache_q4", key, value, slot_mapping, hkv, d)
-    with _launching(key, stream) as st:
-        rc = _native.xpa().nxt_reshape_and_cache_q4(
-            _ptr(key), _ptr(value), _ptr(key_cache), _ptr(value_cache), _ptr(slot_mapping),
-            key.shape[0], hkv, d, bs, float(k_scale), float(v_scale), *_q4_strides(hkv, bs, d),
-            ts, nb, st)
-    if rc != _native.NXT_PA_OK:
-        raise PagedAttentionError(rc, "nxt_reshape_and_cache_q4")
+    where = "reshape_and_cache_q4"
+    device = key_cache.get_device()
+    nb, hkv, bs, d, page, head = _q4_dims(where, key_cache, value_cache, device)
+    ts = _row_stride(where, key, value, slot_mapping, hkv, d, device)
+    st, leave = _launch_on(device, stream)
+    try:
+        _native_call("nxt_reshape_and_cache_q4", key.data_ptr(), value.data_ptr(),
+                     key_cache.data_ptr(), value_cache.data_ptr(), slot_mapping.data_ptr(),
+                     key.shape[0], hkv, d, bs, k_scale, v_scale, page, head, ts, nb, st)
+    finally:
+        if leave is not None:
+            leave.close()
 
 
 def read_cache_q4(key_cache, value_cache, slot_mapping, k_scale, v_scale, *, key=None, value=None,
                   stream=None):
     """The rows that 4-bit pools hold at slot_mapping[t], as fp16 key and value
-    [T, Hkv, D]; rows of negative slots, or slots past the pools, are zero."""
+    [T, Hkv, D] (in `key` and `value`, of equal strides, when given); rows of
+    negative slots, or slots past the pools, are zero."""
     import torch
-    nb, hkv, bs, d = _check_q4_pools("read_cache_q4", key_cache, value_cache, key_cache)
-    with _launching(key_cache, stream) as st:
-        shape = (slot_mapping.numel(), hkv, d)
+    where = "read_cache_q4"
+    device = key_cache.get_device()
+    nb, hkv, bs, d, page, head = _q4_dims(where, key_cache, value_cache, device)
+    T = slot_mapping.numel()
+    st, leave = _launch_on(device, stream)
+    try:
         if key is None:
-            key = torch.empty(shape, dtype=torch.float16, device=key_cache.device)
+            key = torch.empty((T, hkv, d), dtype=torch.float16, device=key_cache.device)
         if value is None:
-            value = (torch.empty(shape, dtype=torch.float16, device=key_cache.device)
-                     if key.is_contiguous() else torch.empty_strided(
-                         shape, key.stride(), dtype=torch.float16, device=key_cache.device))
-        if key.dim() != 3 or key.shape[0] != slot_mapping.numel():
-            raise PagedAttentionError(_native.NXT_PA_EINVAL, "read_cache_q4: rows")
-        ts = _check_rows("read_cache_q4", key, value, slot_mapping, hkv, d)
-        if key.device != key_cache.device:
-            raise PagedAttentionError(_native.NXT_PA_EINVAL, "read_cache_q4: devices")
-        rc = _native.xpa().nxt_read_cache_q4(
-            _ptr(key), _ptr(value), _ptr(key_cache), _ptr(value_cache), _ptr(slot_mapping),
-            key.shape[0], hkv, d, bs, float(k_scale), float(v_scale), *_q4_strides(hkv, bs, d),
-            ts, nb, st)
-    if rc != _native.NXT_PA_OK:
-        raise PagedAttentionError(rc, "nxt_read_cache_q4")
+            value = torch.empty_strided(key.shape, key.stride(), dtype=torch.float16,
+                                        device=key_cache.device)
+        ts = _row_stride(where, key, value, slot_mapping, hkv, d, device)
+        if key.shape[0] != T:
+            _refuse(where, "one row per slot")
+        _native_call("nxt_read_cache_q4", key.data_ptr(), value.data_ptr(), key_cache.data_ptr(),
+                     value_cache.data_ptr(), slot_mapping.data_ptr(), T, hkv, d, bs, k_scale,
+                     v_scale, page, head, ts, nb, st)
+    finally:
+        if leave is not None:
+            leave.close()
     return key, value
 
 
-def _check_q4_attention(where, query, key_cache, value_cache, block_tables, seq_lens, out):
+def _check_step(where, query, block_tables, seq_lens, out, device):
+    """What every attention call needs besides its pools; (B, Hq, D)."""
     import torch
+    shape = query.shape
+    if len(shape) != 3 or not query.is_contiguous() or device < 0:
+        _refuse(where, "query must be a contiguous CUDA tensor [B, Hq, D]")
+    B = shape[0]
+    if (block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] < B
+            or not block_tables.is_contiguous() or block_tables.get_device() != device):
+        _refuse(where, "block_tables must be contiguous int32 [B, max_blocks] on the query's device")
+    if (seq_lens.dtype != torch.int32 or seq_lens.numel() < B or not seq_lens.is_contiguous()
+            or seq_lens.get_device() != device):
+        _refuse(where, "seq_lens must be contiguous int32 [B] on the query's device")
+    if out is not None and (out.shape != shape or out.dtype != query.dtype
+                            or not out.is_contiguous() or out.get_device() != device):
+        _refuse(where, "out must be a contiguous tensor like query")
+    return shape
 
-    def bad(msg):
-        raise PagedAttentionError(_native.NXT_PA_EINVAL, f"{where}: {msg}")
-    if query.dim() != 3 or query.dtype != torch.float16 or not query.is_contiguous():
-        bad("query must be contiguous fp16 [B, Hq, D]")
-    if not query.is_cuda:
-        bad("every tensor must be on the query's CUDA device")
-    nb, hkv, bs, d = _check_q4_pools(where, key_cache, value_cache, query)
-    if query.shape[2] != d:
-        bad("head size of query and pools")
-    _check_tables(bad, query, block_tables, seq_lens, out)
-    return nb, hkv, bs, d
 
-
-def _check_tables(bad, query, block_tables, seq_lens, out):
+def _check_q4_step(where, query, key_cache, value_cache, block_tables, seq_lens, out, device):
     import torch
-    B = query.shape[0]
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] < B:
-        bad("block_tables must be int32 [B, max_blocks]")
-    if seq_lens.dtype != torch.int32 or seq_lens.numel() < B:
-        bad("seq_lens must be int32 [B]")
-    if out is not None and (tuple(out.shape) != tuple(query.shape) or out.dtype != query.dtype):
-        bad("out must have the query's shape and dtype")
-    for t in (block_tables, seq_lens) + (() if out is None else (out,)):
-        if not t.is_contiguous():
-            bad("non-contiguous input")
-        if t.device != query.device:
-            bad("every tensor must be on the query's CUDA device")
+    B, Hq, D = _check_step(where, query, block_tables, seq_lens, out, device)
+    dims = _q4_dims(where, key_cache, value_cache, device)
+    if query.dtype != torch.float16 or D != dims[3]:
+        _refuse(where, "query must be fp16 with the pools' head size")
+    return B, Hq, dims
+
+
+def _workspace(t):
+    return (None, 0) if t is None else (t.data_ptr(), t.numel() * t.element_size())
 
 
 def paged_attention_q4(query, key_cache, value_cache, block_tables, seq_lens, k_scale, v_scale, *,
@@ -689,21 +718,22 @@ def paged_attention_q4(query, key_cache, value_cache, block_tables, seq_lens, k_
     """Decode attention over 4-bit pools (q4_pool_shape); query and output fp16
     [B, Hq, D], any number of query heads per KV head."""
     import torch
-    nb, hkv, bs, d = _check_q4_attention("paged_attention_q4", query, key_cache, value_cache,
-                                         block_tables, seq_lens, out)
-    B, Hq, _ = query.shape
-    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    with _launching(query, stream) as st:
+    device = query.get_device()
+    B, Hq, (nb, hkv, bs, d, page, head) = _check_q4_step(
+        "paged_attention_q4", query, key_cache, value_cache, block_tables, seq_lens, out, device)
+    st, leave = _launch_on(device, stream)
+    try:
         if out is None:
             out = torch.empty_like(query)
-        rc = _native.xpa().nxt_paged_attention_q4_ex(
-            _ptr(out), _ptr(query), _ptr(key_cache), _ptr(value_cache), _ptr(block_tables),
-            _ptr(seq_lens), B, Hq, d, hkv, 1.0 / math.sqrt(d) if scale is None else float(scale),
-            block_tables.shape[1], bs, float(k_scale), float(v_scale), *_q4_strides(hkv, bs, d),
-            nb if num_blocks is None else int(num_blocks), _ptr(workspace), ws_bytes,
-            _ptr(device_status), st)
-    if rc != _native.NXT_PA_OK:
-        raise PagedAttentionError(rc, "nxt_paged_attention_q4_ex")
+        _native_call("nxt_paged_attention_q4_ex", out.data_ptr(), query.data_ptr(),
+                     key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
+                     seq_lens.data_ptr(), B, Hq, d, hkv, d ** -0.5 if scale is None else scale,
+                     block_tables.shape[1], bs, k_scale, v_scale, page, head,
+                     nb if num_blocks is None else num_blocks, *_workspace(workspace),
+                     _opt_ptr(device_status), st)
+    finally:
+        if leave is not None:
+            leave.close()
     return out
 
 
@@ -722,33 +752,45 @@ def paged_attention_q4_append(query, key_cache, value_cache, block_tables, seq_l
     them)."""
     import torch
     where = "paged_attention_q4_append"
-    nb, hkv, bs, d = _check_q4_attention(where, query, key_cache, value_cache, block_tables,
-                                         seq_lens, out)
-    B, Hq, _ = query.shape
-    _check_rows(where, new_key, new_value, slot_mapping, hkv, d)
-    if (new_key.shape[0] != B or not new_key.is_contiguous() or not new_value.is_contiguous()
-            or new_key.device != query.device):
-        raise PagedAttentionError(_native.NXT_PA_EINVAL, f"{where}: new rows must be contiguous "
-                                  "[B, Hkv, D] on the query's device")
-    with _launching(query, stream) as st:
+    device = query.get_device()
+    B, Hq, (nb, hkv, bs, d, page, head) = _check_q4_step(
+        where, query, key_cache, value_cache, block_tables, seq_lens, out, device)
+    _row_stride(where, new_key, new_value, slot_mapping, hkv, d, device)
+    if new_key.shape[0] != B or not new_key.is_contiguous() or not new_value.is_contiguous():
+        _refuse(where, "new rows must be contiguous [B, Hkv, D]")
+    st, leave = _launch_on(device, stream)
+    try:
         if out is None:
             out = torch.empty_like(query)
-        rc = _native.xpa().nxt_paged_attention_q4_append_ex(
-            _ptr(out), _ptr(query), _ptr(key_cache), _ptr(value_cache), _ptr(block_tables),
-            _ptr(seq_lens), _ptr(new_key), _ptr(new_value), _ptr(slot_mapping), B, Hq, d, hkv,
-            1.0 / math.sqrt(d) if scale is None else float(scale), block_tables.shape[1], bs,
-            float(k_scale), float(v_scale), *_q4_strides(hkv, bs, d),
-            nb if num_blocks is None else int(num_blocks), _ptr(device_status), st)
-    if rc != _native.NXT_PA_OK:
-        raise PagedAttentionError(rc, "nxt_paged_attention_q4_append_ex")
+        _native_call("nxt_paged_attention_q4_append_ex", out.data_ptr(), query.data_ptr(),
+                     key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
+                     seq_lens.data_ptr(), new_key.data_ptr(), new_value.data_ptr(),
+                     slot_mapping.data_ptr(), B, Hq, d, hkv, d ** -0.5 if scale is None else scale,
+                     block_tables.shape[1], bs, k_scale, v_scale, page, head,
+                     nb if num_blocks is None else num_blocks, _opt_ptr(device_status), st)
+    finally:
+        if leave is not None:
+            leave.close()
     return out
 
 
 # ── page bounds and sparse attention ───────────────────────────────────────
-def _check_bounds(bad, bounds, num_blocks, hkv, d, dtype, like):
-    if (tuple(bounds.shape) != (num_blocks, hkv, 2, d) or bounds.dtype != dtype
-            or not bounds.is_contiguous() or bounds.device != like.device):
-        bad("bounds must be contiguous [num_blocks, Hkv, 2, D] beside the pools")
+def _check_bounds(where, bounds, nb, hkv, d, dtype, device):
+    if (bounds.shape != (nb, hkv, 2, d) or bounds.dtype != dtype or not bounds.is_contiguous()
+            or bounds.get_device() != device):
+        _refuse(where, "bounds must be contiguous [num_blocks, Hkv, 2, D] beside the pools")
+
+
+def _plain_dims(where, key_cache, value_cache, device):
+    """(num_blocks, Hkv, block size, head size, page and head strides) of fp16 or fp32 pools."""
+    shape = key_cache.shape
+    if (len(shape) != 4 or value_cache.shape != shape or value_cache.dtype != key_cache.dtype
+            or not key_cache.is_contiguous() or not value_cache.is_contiguous() or device < 0
+            or key_cache.get_device() != device or value_cache.get_device() != device):
+        _refuse(where, "pools must be contiguous [num_blocks, Hkv, block_size, D] on one CUDA "
+                "device")
+    nb, hkv, bs, d = shape
+    return nb, hkv, bs, d, hkv * bs * d, bs * d
 
 
 def page_bounds(key_cache, block_tables, seq_lens, bounds, *, num_new_tokens=0, k_scale=None,
@@ -759,61 +801,50 @@ def page_bounds(key_cache, block_tables, seq_lens, bounds, *, num_new_tokens=0, 
     fp16 or fp32 pool [num_blocks, Hkv, P, D] (bounds of its type) or, with
     k_scale, a 4-bit pool (q4_pool_shape; bounds fp16). Returns `bounds`."""
     import torch
-
-    def bad(msg):
-        raise PagedAttentionError(_native.NXT_PA_EINVAL, f"page_bounds: {msg}")
-    if not key_cache.is_cuda or key_cache.dim() != 4 or not key_cache.is_contiguous():
-        bad("the pool must be a contiguous 4-D CUDA tensor")
-    if seq_lens.dim() != 1:
-        bad("seq_lens must be int32 [B]")
+    where = "page_bounds"
+    device = key_cache.get_device()
     if k_scale is None:
-        ds = _dtype_size(key_cache)
-        nb, hkv, bs, d = key_cache.shape
-        strides, dtype, kind = (hkv * bs * d, bs * d), key_cache.dtype, ds
+        kind = _dtype_size(key_cache)
+        nb, hkv, bs, d, page, head = _plain_dims(where, key_cache, key_cache, device)
+        dtype, name = key_cache.dtype, "nxt_page_bounds"
     else:
-        nb, hkv, bs, d = _check_q4_pools("page_bounds", key_cache, key_cache, key_cache)
-        strides, dtype, kind = _q4_strides(hkv, bs, d), torch.float16, float(k_scale)
-    _check_bounds(bad, bounds, nb, hkv, d, dtype, key_cache)
+        kind = k_scale
+        nb, hkv, bs, d, page, head = _q4_dims(where, key_cache, key_cache, device)
+        dtype, name = torch.float16, "nxt_page_bounds_q4"
+    _check_bounds(where, bounds, nb, hkv, d, dtype, device)
     B = seq_lens.numel()
     if (block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] < B
-            or seq_lens.dtype != torch.int32 or not block_tables.is_contiguous()
-            or not seq_lens.is_contiguous() or block_tables.device != key_cache.device
-            or seq_lens.device != key_cache.device):
-        bad("block_tables must be int32 [B, max_blocks] and seq_lens int32 [B], beside the pool")
-    name = "nxt_page_bounds" if k_scale is None else "nxt_page_bounds_q4"
-    with _launching(key_cache, stream) as st:
-        rc = getattr(_native.xpa(), name)(
-            _ptr(bounds), _ptr(key_cache), _ptr(block_tables), _ptr(seq_lens), B, hkv, d,
-            block_tables.shape[1], bs, kind, *strides,
-            nb if num_blocks is None else int(num_blocks), int(num_new_tokens),
-            _ptr(device_status), st)
-    if rc != _native.NXT_PA_OK:
-        raise PagedAttentionError(rc, name)
+            or seq_lens.dtype != torch.int32 or seq_lens.dim() != 1
+            or not block_tables.is_contiguous() or not seq_lens.is_contiguous()
+            or block_tables.get_device() != device or seq_lens.get_device() != device):
+        _refuse(where, "block_tables must be int32 [B, max_blocks] and seq_lens int32 [B], beside "
+                "the pool")
+    st, leave = _launch_on(device, stream)
+    try:
+        _native_call(name, bounds.data_ptr(), key_cache.data_ptr(), block_tables.data_ptr(),
+                     seq_lens.data_ptr(), B, hkv, d, block_tables.shape[1], bs, kind, page, head,
+                     nb if num_blocks is None else num_blocks, num_new_tokens,
+                     _opt_ptr(device_status), st)
+    finally:
+        if leave is not None:
+            leave.close()
     return bounds
 
 
 def _check_sparse(where, query, key_cache, value_cache, bounds, block_tables, seq_lens, out,
-                  selected, max_pages, q4):
-    """(num_blocks, Hkv, page size, strides) of a sparse call's pools."""
+                  device, q4):
     import torch
-
-    def bad(msg):
-        raise PagedAttentionError(_native.NXT_PA_EINVAL, f"{where}: {msg}")
     if q4:
-        nb, hkv, bs, d = _check_q4_attention(where, query, key_cache, value_cache, block_tables,
-                                             seq_lens, out)
-        strides = _q4_strides(hkv, bs, d)
+        B, Hq, dims = _check_q4_step(where, query, key_cache, value_cache, block_tables, seq_lens,
+                                     out, device)
     else:
-        _check_attention_inputs(where, query, key_cache, value_cache, block_tables, seq_lens, out)
-        nb, hkv, bs, d = key_cache.shape
-        strides = (hkv * bs * d, bs * d)
-    _check_bounds(bad, bounds, nb, hkv, d, query.dtype, query)
-    if selected is not None and (
-            selected.dtype != torch.int32 or not selected.is_contiguous()
-            or tuple(selected.shape) != (query.shape[0], hkv, max_pages)
-            or selected.device != query.device):
-        bad("selected must be contiguous int32 [B, Hkv, max_pages] on the query's device")
-    return nb, hkv, bs, strides
+        B, Hq, D = _check_step(where, query, block_tables, seq_lens, out, device)
+        dims = _plain_dims(where, key_cache, value_cache, device)
+        if (query.dtype not in (torch.float16, torch.float32) or key_cache.dtype != query.dtype
+                or D != dims[3]):
+            _refuse(where, "query and pools must be fp16 or fp32, of one type and head size")
+    _check_bounds(where, bounds, dims[0], dims[1], dims[3], query.dtype, device)
+    return B, Hq, dims
 
 
 def select_pages(query, key_cache, bounds, block_tables, seq_lens, max_pages, *, sink_pages=0,
@@ -823,21 +854,23 @@ def select_pages(query, key_cache, bounds, block_tables, seq_lens, max_pages, *,
     key_cache.view(NB * Hkv, 1, P, D), query.view(B * Hkv, G, D), tables and
     lens are the inputs of any attention call over the pool."""
     import torch
-    nb, hkv, bs, strides = _check_sparse("select_pages", query, key_cache, key_cache, bounds,
-                                         block_tables, seq_lens, None, None, max_pages, False)
-    B, Hq, d = query.shape
-    with _launching(query, stream) as st:
+    device = query.get_device()
+    B, Hq, (nb, hkv, bs, d, page, head) = _check_sparse(
+        "select_pages", query, key_cache, key_cache, bounds, block_tables, seq_lens, None, device,
+        False)
+    st, leave = _launch_on(device, stream)
+    try:
         new = lambda *s: torch.empty(s, dtype=torch.int32, device=query.device)
-        tables, lens = new(B * hkv, int(max_pages)), new(B * hkv)
-        pages = new(B, hkv, int(max_pages))
-        rc = _native.xpa().nxt_select_pages(
-            _ptr(tables), _ptr(lens), _ptr(pages), _ptr(query), _ptr(bounds), _ptr(block_tables),
-            _ptr(seq_lens), B, Hq, d, hkv, 1.0 / math.sqrt(d) if scale is None else float(scale),
-            block_tables.shape[1], bs, _dtype_size(query), *strides,
-            nb if num_blocks is None else int(num_blocks), int(max_pages), int(sink_pages),
-            int(recent_pages), None, 0, _ptr(device_status), st)
-    if rc != _native.NXT_PA_OK:
-        raise PagedAttentionError(rc, "nxt_select_pages")
+        tables, lens, pages = new(B * hkv, max_pages), new(B * hkv), new(B, hkv, max_pages)
+        _native_call("nxt_select_pages", tables.data_ptr(), lens.data_ptr(), pages.data_ptr(),
+                     query.data_ptr(), bounds.data_ptr(), block_tables.data_ptr(),
+                     seq_lens.data_ptr(), B, Hq, d, hkv, d ** -0.5 if scale is None else scale,
+                     block_tables.shape[1], bs, query.element_size(), page, head,
+                     nb if num_blocks is None else num_blocks, max_pages, sink_pages, recent_pages,
+                     None, 0, _opt_ptr(device_status), st)
+    finally:
+        if leave is not None:
+            leave.close()
     return tables, lens, pages
 
 
@@ -851,29 +884,34 @@ def paged_attention_sparse(query, key_cache, value_cache, bounds, block_tables, 
     with k_scale and v_scale. ``selected`` (int32 [B, Hkv, max_pages]) receives
     the kept pages' indices within each sequence, -1 past the last."""
     import torch
+    where = "paged_attention_sparse"
+    device = query.get_device()
     q4 = k_scale is not None
     if q4 != (v_scale is not None):
-        raise PagedAttentionError(_native.NXT_PA_EINVAL,
-                                  "paged_attention_sparse: k_scale and v_scale go together")
-    nb, hkv, bs, strides = _check_sparse(
-        "paged_attention_sparse", query, key_cache, value_cache, bounds, block_tables, seq_lens,
-        out, selected, max_pages, q4)
-    B, Hq, d = query.shape
-    name = "nxt_paged_attention_q4_sparse_ex" if q4 else "nxt_paged_attention_sparse_ex"
-    kind = (float(k_scale), float(v_scale)) if q4 else (_dtype_size(query),)
-    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    with _launching(query, stream) as st:
+        _refuse(where, "k_scale and v_scale go together")
+    B, Hq, (nb, hkv, bs, d, page, head) = _check_sparse(
+        where, query, key_cache, value_cache, bounds, block_tables, seq_lens, out, device, q4)
+    if selected is not None and (
+            selected.dtype != torch.int32 or not selected.is_contiguous()
+            or selected.shape != (B, hkv, max_pages) or selected.get_device() != device):
+        _refuse(where, "selected must be contiguous int32 [B, Hkv, max_pages] on the query's device")
+    if q4:
+        name, kind = "nxt_paged_attention_q4_sparse_ex", (k_scale, v_scale)
+    else:
+        name, kind = "nxt_paged_attention_sparse_ex", (query.element_size(),)
+    st, leave = _launch_on(device, stream)
+    try:
         if out is None:
             out = torch.empty_like(query)
-        rc = getattr(_native.xpa(), name)(
-            _ptr(out), _ptr(query), _ptr(key_cache), _ptr(value_cache), _ptr(bounds),
-            _ptr(block_tables), _ptr(seq_lens), _ptr(selected), B, Hq, d, hkv,
-            1.0 / math.sqrt(d) if scale is None else float(scale), block_tables.shape[1], bs,
-            *kind, *strides, nb if num_blocks is None else int(num_blocks), int(max_pages),
-            int(sink_pages), int(recent_pages), _ptr(workspace), ws_bytes, _ptr(device_status),
-            st)
-    if rc != _native.NXT_PA_OK:
-        raise PagedAttentionError(rc, name)
+        _native_call(name, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(),
+                     value_cache.data_ptr(), bounds.data_ptr(), block_tables.data_ptr(),
+                     seq_lens.data_ptr(), _opt_ptr(selected), B, Hq, d, hkv,
+                     d ** -0.5 if scale is None else scale, block_tables.shape[1], bs, *kind, page,
+                     head, nb if num_blocks is None else num_blocks, max_pages, sink_pages,
+                     recent_pages, *_workspace(workspace), _opt_ptr(device_status), st)
+    finally:
+        if leave is not None:
+            leave.close()
     return out
 
 
