@@ -179,6 +179,8 @@ SHAPES = [
     (40, 1, 128, 16), (12, 12, 64, 16), (16, 1, 64, 48), (10, 2, 256, 16), (20, 2, 256, 32),
     (6, 2, 16, 16), (6, 3, 32, 16), (5, 1, 48, 16), (20, 4, 96, 32), (9, 1, 80, 16),
     (4, 2, 144, 16), (34, 2, 192, 64), (3, 3, 208, 16), (7, 1, 240, 16),
+    (12, 1, 112, 16), (2, 1, 160, 16), (11, 1, 176, 32), (24, 2, 224, 16), (18, 2, 48, 16),
+    (9, 1, 16, 16), (16, 1, 96, 16), (30, 2, 80, 16), (10, 1, 32, 16),
 ]
 LENS = [[1], [0, 1, 15, 16, 17, 33], [127, 700, 5, 2049, 0, 64]]
 

@@ -108,6 +108,7 @@ SHAPES = [
     (8, 2, 128, 16, np.float16), (32, 4, 64, 16, np.float16), (12, 12, 64, 16, np.float32),
     (20, 2, 256, 16, np.float16), (5, 1, 80, 32, np.float16), (3, 1, 36, 8, np.float16),
     (34, 1, 40, 16, np.float16), (6, 2, 33, 16, np.float32), (16, 1, 24, 4, np.float16),
+    (32, 2, 256, 16, np.float16), (20, 1, 64, 16, np.float16), (33, 1, 128, 16, np.float16),
 ]
 
 

@@ -229,11 +229,11 @@ __global__ void __launch_bounds__(128) pa_q4_read_kernel(const Q4RowsParams a) {
 constexpr float kRaise = 8.f;  // log2 units a score may exceed m by
 constexpr float kShift = 7.f;  // p = 2^(x - m + kShift) <= 2^15
 
-template <int W, int NT, bool EXACT, int NW, int STAGES, int U>
+template <int D, int NT, int NW, int STAGES, int U>
 struct Q4Cfg {
-  static constexpr int kDMax = 64 * W;
+  static constexpr int kDMax = (D + 63) / 64 * 64;  // whole words of V per lane
   static constexpr int kHeads = 8 * NT;
-  static constexpr int kTileBytes = 18 * kDMax;   // one K and one V tile
+  static constexpr int kTileBytes = 18 * D;         // one K and one V tile
   static constexpr int kStageBytes = U * kTileBytes;
   static constexpr int kRow = kDMax + 4;          // merge rows, floats
   static constexpr size_t kMergeBytes =
@@ -282,23 +282,25 @@ __device__ __forceinline__ void cp_async16_at(uint32_t dst, const uint8_t* src) 
 // EXACT (D = 64 W, W = 1, 2, 4): rows are placed and chunks swizzled so that
 // every read below is conflict-free; K row r's place is its S^T row, V row
 // 4 t + k's place is 4 k + t. Otherwise a tile is copied as it is.
-template <int W, bool EXACT>
+template <int D>
 struct Q4Stage {
-  int D, lane, g, t;
+  static constexpr int W = (D + 63) / 64;
+  static constexpr bool EXACT = D == 64 || D == 128 || D == 256;
+  int lane, g, t;
   // sources in page 0; EXACT: this lane's first chunk of each piece
   const uint8_t *ksrc, *vsrc, *ssrc;
   uint32_t ring;               // the warp's ring
   uint32_t kd, sd, vd[W];      // EXACT: copy destinations in stage 0
   uint32_t ka[2], ksa, va, vsa;  // read addresses in stage 0
 
-  __device__ __forceinline__ Q4Stage(int D_, int lane_, const uint8_t* k, const uint8_t* v,
+  __device__ __forceinline__ Q4Stage(int lane_, const uint8_t* k, const uint8_t* v,
                                      uint32_t ring_)
-      : D(D_), lane(lane_), ksrc(k), vsrc(v), ssrc(k), ring(ring_) {
+      : lane(lane_), ksrc(k), vsrc(v), ssrc(k), ring(ring_) {
     g = lane >> 2;
     t = lane & 3;
     const int tok = 4 * (g >> 1) + (g & 1);  // sigma(g); sigma(g + 8) is + 2
     if constexpr (EXACT) {
-      constexpr int DD = 64 * W;
+      constexpr int DD = D;
       constexpr int CPR = 2 * W;  // 16-byte chunks per row
       ksrc = k + lane * 16;
       vsrc = v + lane * 16;
@@ -364,10 +366,14 @@ struct Q4Stage {
       if (W == 4 || (lane & 15) < 4 * W) cp_async16_at<S0, 0>(sd, s);
     } else {
       const unsigned long long off = (unsigned long long)at * unit;
-      const int n = 9 * D / 16;
-      for (int x = lane; x < n; x += 32) {
-        cp_async16_at<S0, 0>(ring + x * 16, ksrc + off + x * 16);
-        cp_async16_at<S0, 0>(ring + 9 * D + x * 16, vsrc + off + x * 16);
+      constexpr int n = 9 * D / 16;
+#pragma unroll
+      for (int i = 0; i < (n + 31) / 32; ++i) {
+        const int x = lane + 32 * i;
+        if (x < n) {
+          cp_async16_at<S0, 0>(ring + x * 16, ksrc + off + x * 16);
+          cp_async16_at<S0, 0>(ring + 9 * D + x * 16, vsrc + off + x * 16);
+        }
       }
     }
   }
@@ -390,25 +396,34 @@ struct Q4Stage {
       lds_words<W, S0>(ksa, ks[0]);
       lds_words<W, S0 + 8 * W>(ksa, ks[1]);
     } else {
-      const int NG = D / 16;
+      constexpr int NG = D / 16;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const uint32_t row = ka[0] + 2 * r * (D / 2);
         const uint32_t sc = ksa + 2 * r * NG;
 #pragma unroll
         for (int i = 0; i < 2 * W; ++i) {
-          uint32_t lo = 0, hi = 0;
-          if (2 * i < NG) lo = lds16<S0>(row + 4 * i);
-          if (2 * i + 1 < NG) hi = lds16<S0>(row + 4 * i + 2);
-          kw[r][i] = lo | (hi << 16);
+          kw[r][i] = 0u;
+          if constexpr (NG % 2 == 0) {  // whole words
+            if (2 * i < NG) lds_words<1, S0>(row + 4 * i, &kw[r][i]);
+          } else {
+            if (2 * i < NG) kw[r][i] = lds16<S0>(row + 4 * i);
+            if (2 * i + 1 < NG) kw[r][i] |= lds16<S0>(row + 4 * i + 2) << 16;
+          }
         }
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-          uint32_t s = 0;
+          ks[r][i] = 0u;
+          if constexpr (NG % 4 == 0) {
+            if (4 * i < NG) lds_words<1, S0>(sc + 4 * i, &ks[r][i]);
+          } else if constexpr (NG % 2 == 0) {
+            if (4 * i < NG) ks[r][i] = lds16<S0>(sc + 4 * i);
+            if (4 * i + 2 < NG) ks[r][i] |= lds16<S0>(sc + 4 * i + 2) << 16;
+          } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (4 * i + j < NG) s |= lds8<S0>(sc + 4 * i + j) << (8 * j);
-          ks[r][i] = s;
+            for (int j = 0; j < 4; ++j)
+              if (4 * i + j < NG) ks[r][i] |= lds8<S0>(sc + 4 * i + j) << (8 * j);
+          }
         }
       }
     }
@@ -489,16 +504,15 @@ __device__ __forceinline__ ItemKind q4_item(const Params& p, int row, Item& it) 
   return kItemWork;
 }
 
-template <int W, int NT, bool EXACT, int NW, int STAGES, int U, int MINB>
+template <int D, int NT, int NW, int STAGES, int U, int MINB>
 __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, const Q4Units q) {
-  using C = Q4Cfg<W, NT, EXACT, NW, STAGES, U>;
+  using C = Q4Cfg<D, NT, NW, STAGES, U>;
+  constexpr int W = Q4Stage<D>::W, NG = D / 16;  // V words per lane, channel groups
   extern __shared__ __align__(128) uint8_t smem[];
   // Every CTA waits for the kernel before this one (which may be this call's
   // append); the merge may be scheduled from here on and waits for this grid.
   pdl_wait_primary();
   pdl_launch_dependents();
-  const int D = EXACT ? C::kDMax : p.D;
-  const int NG = D / 16;
   Item it;
   // grid: x = partition, y and z = (sequence, KV head, head chunk)
   const int col = blockIdx.y + blockIdx.z * kGridY;
@@ -524,7 +538,10 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, co
   const float slack = fminf(kRaise / sl, 1e30f);  // kRaise in units of q . k
 
   // ── Q fragments: head g of tile nt, channels 16 j + 4 t .. + 3 ──────────
-  uint32_t qf[4 * W][NT][2];
+  // Groups go in pairs, a missing one as 0: with the second half of a word's
+  // conversions unused, the compiler's conversions of the first came out wrong.
+  constexpr int NGP = NG + NG % 2;
+  uint32_t qf[NGP][NT][2];
   {
     const __half* query = static_cast<const __half*>(p.q);
     const bool al = (reinterpret_cast<uintptr_t>(query) & 7u) == 0;
@@ -533,7 +550,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, co
       const bool head = nt * 8 + g < nh;
       const __half* src = query + (row0 + nt * 8 + g) * D + 4 * t;
 #pragma unroll
-      for (int j = 0; j < 4 * W; ++j) {
+      for (int j = 0; j < NGP; ++j) {
         uint2 u = make_uint2(0u, 0u);
         if (head && j < NG) {
           if (al) {
@@ -562,9 +579,9 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, co
   const int steps = (tiles + U - 1) / U;
   const int n = steps > warp ? (steps - warp + NW - 1) / NW : 0;
   const long long head_off = (long long)it.kvh * p.kv_head_stride;
-  const Q4Stage<W, EXACT> sg(D, lane, static_cast<const uint8_t*>(p.k) + head_off,
-                             static_cast<const uint8_t*>(p.v) + head_off,
-                             smem_u32(smem) + warp * (STAGES * C::kStageBytes));
+  const Q4Stage<D> sg(lane, static_cast<const uint8_t*>(p.k) + head_off,
+                      static_cast<const uint8_t*>(p.v) + head_off,
+                      smem_u32(smem) + warp * (STAGES * C::kStageBytes));
   const int* table = p.block_tables + (long long)it.b * p.max_blocks + it.page_begin;
   auto entry_ok = [&](int e) { return e >= 0 && e < q.page_limit; };
 
@@ -646,7 +663,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, co
       });
 #pragma unroll
       for (int i2 = 0; i2 < 2 * W; ++i2) {
-        if (!EXACT && 2 * i2 >= NG) break;
+        if (2 * i2 >= NGP) break;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           uint32_t a[2][4];
@@ -751,7 +768,6 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, co
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        if (!EXACT && w * 8 >= D) break;
         const uint32_t sw = vs[u][w] & keep[u];
         const uint32_t s01 = fp8x2_to_h2<kKvE4M3>(sw), s23 = fp8x2_to_h2<kKvE4M3>(sw >> 16);
         uint32_t a[4][4];  // [even 01, odd 01, even 23, odd 23][channel pair]
@@ -878,6 +894,12 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t
 #ifndef XPA_Q4_TILES
 #define XPA_Q4_TILES 2
 #endif
+#ifndef XPA_Q4_TILES_ODD
+#define XPA_Q4_TILES_ODD 1
+#endif
+#ifndef XPA_Q4_MIN_CTAS_ODD
+#define XPA_Q4_MIN_CTAS_ODD 3
+#endif
 #ifndef XPA_Q4_STAGES
 #define XPA_Q4_STAGES 2
 #endif
@@ -885,12 +907,16 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t
 #define XPA_Q4_MIN_CTAS 4
 #endif
 
-template <int W, int NT, bool EXACT>
+template <int D, int NT>
 cudaError_t launch_q4_t(const Params& p, cudaStream_t st) {
-  constexpr int NW = XPA_Q4_WARPS, STAGES = XPA_Q4_STAGES, U = XPA_Q4_TILES;
-  constexpr int MINB = (EXACT && W <= 2 && NT == 1) ? XPA_Q4_MIN_CTAS : 1;
-  using C = Q4Cfg<W, NT, EXACT, NW, STAGES, U>;
-  auto kern = pa_q4_kernel<W, NT, EXACT, NW, STAGES, U, MINB>;
+  constexpr bool EXACT = Q4Stage<D>::EXACT;
+  constexpr int NW = XPA_Q4_WARPS;
+  // the other head sizes take more registers per tile: one at a time, a longer ring
+  constexpr int U = EXACT ? XPA_Q4_TILES : XPA_Q4_TILES_ODD;
+  constexpr int STAGES = U == 1 ? 4 : XPA_Q4_STAGES;
+  constexpr int MINB = D <= 128 && NT == 1 ? (EXACT ? XPA_Q4_MIN_CTAS : XPA_Q4_MIN_CTAS_ODD) : 1;
+  using C = Q4Cfg<D, NT, NW, STAGES, U>;
+  auto kern = pa_q4_kernel<D, NT, NW, STAGES, U, MINB>;
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = host::smem_limit(kern, C::kSmem, true, done);
   if (e != cudaSuccess) return e;
@@ -920,15 +946,32 @@ cudaError_t launch_q4_attention(const Params& p, cudaStream_t st) {
   // 16 heads per CTA where the group has more than 8 and the accumulators fit
   const bool two = p.GS > 8;
   switch (p.D) {
-    case 64: return two ? launch_q4_t<1, 2, true>(p, st) : launch_q4_t<1, 1, true>(p, st);
-    case 128: return two ? launch_q4_t<2, 2, true>(p, st) : launch_q4_t<2, 1, true>(p, st);
-    case 256: return launch_q4_t<4, 1, true>(p, st);
-    default: break;
+#define XPA_Q4_SMALL(D) \
+  case D:               \
+    return two ? launch_q4_t<D, 2>(p, st) : launch_q4_t<D, 1>(p, st)
+#define XPA_Q4_LARGE(D) \
+  case D:               \
+    return launch_q4_t<D, 1>(p, st)
+    XPA_Q4_SMALL(16);
+    XPA_Q4_SMALL(32);
+    XPA_Q4_SMALL(48);
+    XPA_Q4_SMALL(64);
+    XPA_Q4_SMALL(80);
+    XPA_Q4_SMALL(96);
+    XPA_Q4_SMALL(112);
+    XPA_Q4_SMALL(128);
+    XPA_Q4_LARGE(144);
+    XPA_Q4_LARGE(160);
+    XPA_Q4_LARGE(176);
+    XPA_Q4_LARGE(192);
+    XPA_Q4_LARGE(208);
+    XPA_Q4_LARGE(224);
+    XPA_Q4_LARGE(240);
+    XPA_Q4_LARGE(256);
+#undef XPA_Q4_SMALL
+#undef XPA_Q4_LARGE
+    default: return cudaErrorInvalidValue;
   }
-  if (p.D < 64) return launch_q4_t<1, 1, false>(p, st);
-  if (p.D < 128) return launch_q4_t<2, 1, false>(p, st);
-  if (p.D <= 192) return launch_q4_t<3, 1, false>(p, st);
-  return launch_q4_t<4, 1, false>(p, st);
 }
 
 namespace {

@@ -78,7 +78,10 @@ int rows_call(bool write, void* key, void* value, void* kc, void* vc, const int6
 
 // Partitions of a 4-bit call, in 16-token tiles rounded to whole pages: at
 // most XPA_Q4_PART_TILES, halved while the grid would hold fewer than
-// XPA_Q4_ITEMS_PER_SM items per SM, but not below XPA_Q4_MIN_TILES.
+// XPA_Q4_ITEMS_PER_SM items per SM, but not below 8, nor below sqrt(tiles / 2):
+// with few rows, a shorter partition saves its own time and costs as much in
+// the merge of the longer list of partials (2 rows of 3254 tiles, D = 256: 8
+// tiles 47 us, 19 + 31 in the merge; 64 tiles 21).
 #ifndef XPA_Q4_PART_TILES
 #define XPA_Q4_PART_TILES 128
 #endif
@@ -93,7 +96,7 @@ Plan q4_plan(int B, int Hq, int D, int Hkv, int max_blocks, int bs, int nsm) {
   const long long tiles = std::max(1LL, (long long)max_blocks * spp);
   const long long rows = (long long)B * Hkv, want = (long long)XPA_Q4_ITEMS_PER_SM * nsm;
   long long pt = XPA_Q4_PART_TILES;
-  while (pt > XPA_Q4_MIN_TILES && rows * ceil_div(tiles, pt) < want) pt >>= 1;
+  while (pt > XPA_Q4_MIN_TILES && pt * pt > tiles && rows * ceil_div(tiles, pt) < want) pt >>= 1;
   while (ceil_div(tiles, pt) > 8192) pt <<= 1;
   Plan pl;
   pl.part_pages = (int)std::max(1LL, pt / spp);

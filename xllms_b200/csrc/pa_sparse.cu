@@ -310,7 +310,7 @@ __device__ __forceinline__ int table_entry(const SelectParams& p, int b, int at)
 // of memory), each with its own KV head, and with a second set of tiles where
 // there are few heads.
 // S: steps of 16 values, 2 D <= 16 S; FULL: 2 D = 16 S.
-constexpr int kScoreWarps = 4;  // W: three CTAs per SM at D = 128, whose starts overlap
+// W = kScoreWarps: three CTAs per SM at D = 128, whose starts overlap.
 inline size_t score_smem_bytes(int D) {
   return (size_t)kScoreWarps * 2 * kScoreTile * (4 * D + 16);
 }
@@ -368,12 +368,15 @@ __global__ void __launch_bounds__(kScoreWarps * 32) pa_score_mma_kernel(const Se
           cp_async16(dst + r * row_bytes + c * 512, from + c * 512);
       }
     } else {
-#pragma unroll 1
-      for (int r = 0; r < kScoreTile; ++r) {
+      const int cpr = D / 4;  // 16-byte chunks per row, fewer than 64
+      int r = lane >= cpr ? lane / cpr : 0, c = lane - r * cpr;
+#pragma unroll 4
+      for (int i = 0; i < kScoreTile * cpr; i += 32) {
         const int er = max(__shfl_sync(0xffffffffu, e, r), 0);
-        const uint8_t* from = bounds + (unsigned long long)(unsigned)er * page_bytes;
-        for (int c = lane; c < D / 4; c += 32)
-          cp_async16(st + r * row_bytes + c * 16, from + c * 16);
+        if (r < kScoreTile)
+          cp_async16(st + r * row_bytes + c * 16,
+                     bounds + (unsigned long long)(unsigned)er * page_bytes + c * 16);
+        for (c += 32; c >= cpr; c -= cpr) ++r;
       }
     }
   };
@@ -393,26 +396,20 @@ __global__ void __launch_bounds__(kScoreWarps * 32) pa_score_mma_kernel(const Se
                         ((long long)b * p.Hq + (long long)h * p.GS + h0 + g) * D + 2 * t;
       const __half2 zero = __float2half2_rn(0.f), top = __float2half2_rn(65504.f);
       const __half2 sg = __float2half2_rn(p.sign);
+      const bool head = h0 + g < p.GS;
 #pragma unroll
       for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int at = 16 * s + 8 * k;
           const bool upper = at >= D;
-          qf[s][k] = 0u;
-          if (h0 + g < p.GS && (FULL || at < 2 * D)) {
-            // max and min drop a NaN operand, so a NaN becomes 0 in both halves
-            const __half2 x = __ldg(reinterpret_cast<const __half2*>(q + at - (upper ? D : 0)));
-            __half2 pos = __hmin2(__hmax2(x, zero), top);
-            __half2 neg = __hmax2(__hmin2(x, zero), __hneg2(top));
-            if (p.sign <= 0.f) {
-              const __half2 a = __hmul2(neg, sg), z = __hmul2(pos, sg);
-              pos = a;
-              neg = z;
-            }
-            const __half2 y = upper ? pos : neg;
-            qf[s][k] = *reinterpret_cast<const uint32_t*>(&y);
-          }
+          __half2 x = zero;
+          if (head && (FULL || at < 2 * D))
+            x = __ldg(reinterpret_cast<const __half2*>(q + at - (upper ? D : 0)));
+          x = __hmul2(x, sg);
+          // max and min drop a NaN operand, so a NaN becomes 0 in both halves
+          x = upper ? __hmin2(__hmax2(x, zero), top) : __hmax2(__hmin2(x, zero), __hneg2(top));
+          qf[s][k] = *reinterpret_cast<const uint32_t*>(&x);
         }
     }
     uint32_t st = 0;
@@ -793,7 +790,7 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p, 
   __syncthreads();
   int to = __reduce_add_sync(0xffffffffu, lane < warp ? s_count[lane] : 0);
   const int done = __reduce_add_sync(0xffffffffu, lane < NWARP ? s_count[lane] : 0);
-  int* tab = p.sel_tables + (long long)row * p.keep;
+  int* tab = p.sel_tables + (long long)row * p.copies * p.keep;
   int* pages = p.sel_pages ? p.sel_pages + (long long)row * p.keep : nullptr;
 #pragma unroll 2
   for (int base = begin; base < stop; base += 32) {
@@ -810,15 +807,17 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p, 
     const int e = __ldg(p.block_tables + (long long)b * p.max_blocks + at);
     if (pages) pages[i] = at;
     tail |= at == n - 1;
-    tab[i] = (int)((long long)e * p.head_pages + h);
+    const int id = (int)((long long)e * p.head_pages + h);
+    for (int c = 0; c < p.copies; ++c) tab[(long long)c * p.keep + i] = id;
   }
   for (int i = done + tid; i < p.keep; i += NT) {
-    tab[i] = -1;
+    for (int c = 0; c < p.copies; ++c) tab[(long long)c * p.keep + i] = -1;
     if (pages) pages[i] = -1;
   }
   tail = __syncthreads_or(tail);
-  if (tid == 0)
-    p.sel_lens[row] = done * p.block_size - (tail ? n * p.block_size - L : 0);
+  if (tid < p.copies)
+    p.sel_lens[(long long)row * p.copies + tid] =
+        done * p.block_size - (tail ? n * p.block_size - L : 0);
 }
 
 template <typename... KArgs, typename... Args>

@@ -37,8 +37,8 @@ struct SelectParams {
   const int* block_tables;
   const int* seq_lens;
   int* status;
-  int* sel_tables;  // [B * Hkv][keep] page * head_pages + kv head
-  int* sel_lens;    // [B * Hkv] tokens kept
+  int* sel_tables;  // [B * Hkv][copies][keep] page * head_pages + kv head
+  int* sel_lens;    // [B * Hkv][copies] tokens kept
   int* sel_pages;   // [B * Hkv][keep] page index within the sequence, -1 past the last; or null
   // workspace
   unsigned* keys;         // [B * Hkv][max_blocks] ordered scores, 0: page not eligible
@@ -50,17 +50,24 @@ struct SelectParams {
   long long head_pages;  // kv_block_stride / kv_head_stride
   int B, Hq, Hkv, D, GS, max_blocks, block_size;
   int keep, sink, recent;
+  int copies;  // of every row's tables, for attention that takes its heads in parts
   int chunks, chunk_pages;  // score CTAs per row (or 8 rows), pages of each
   int tiles, tile_pages;    // entries of a row's magnitude, pages of each
   float sign;  // of the score scale: -1, 0 or 1
   int vec;     // fp16, D % 8 == 0, q and bounds on 16-byte boundaries
 };
 
-// Pages of one score CTA and of one magnitude entry: the tensor-core kernel takes
-// tiles of 16, 128 pages a CTA (8 sequences of 32-128K tokens: 64 pages 80 us
-// with the selection, 128 74, 32 91); the scalar one, whose warps take a page at
-// a time, 32.
-constexpr int kScoreTile = 16, kScoreChunk = 128, kScoreChunkScalar = 32;
+// Pages of one magnitude entry and of one score CTA. The tensor-core kernel
+// takes tiles of 16, 128 pages a CTA (8 sequences of 32-128K tokens: 64 pages
+// 80 us with the selection, 128 74, 32 91), fewer while that leaves the GPU
+// without three CTAs per SM; the scalar one, whose warps take a page at a time, 32.
+constexpr int kScoreTile = 16, kScoreChunkScalar = 32, kScoreWarps = 4;
+inline int score_chunk(int B, int Hkv, int max_blocks, int sms) {
+  const long long cols = (long long)B * ((Hkv + kScoreWarps - 1) / kScoreWarps);
+  int chunk = 128;
+  while (chunk > kScoreTile && cols * ((max_blocks + chunk - 1) / chunk) < 3LL * sms) chunk >>= 1;
+  return chunk;
+}
 
 cudaError_t launch_select(const SelectParams& p, int dtype_size, cudaStream_t st);
 

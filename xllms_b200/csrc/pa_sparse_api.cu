@@ -97,16 +97,31 @@ struct SparseCall {
 #define XPA_SPARSE_ITEMS_PER_SM 3
 #endif
 
+// Parts that a KV head's group of query heads is taken in: the tensor-core
+// decode kernel of fp16 pools reads a page for up to 16 heads (8 at head size
+// 256), and re-reading it from L2 for the next part costs less than the
+// CUDA-core kernel (48 heads over 3 KV heads, D = 256, 18 pages: 83 -> 12 us).
+int head_parts(int GS, int D, int bs, int ds, bool q4) {
+  if (q4 || ds != 2 || bs != 16 || (D != 64 && D != 128 && D != 256)) return 1;
+  const int most = D == 256 ? 8 : 16;
+  if (GS <= most) return 1;
+  for (int s = 2; s <= 8; ++s)
+    if (GS % s == 0 && GS / s <= most) return s;
+  return 1;
+}
+
 // Workspace: scores and near pages of the selection, the kept pages' tables,
 // the attention's partials, each from a 256-byte boundary.
 struct Layout {
   size_t keys, magnitude, near_page, near_key, tables, lens, part, total;
   size_t part_bytes;
+  int parts;  // of a group's heads, see head_parts
 };
 
 Layout layout_of(long long rows, int GS, int D, int max_blocks, int bs, int ds, int keep, bool q4,
                  bool attention, int sms) {
   Layout l{};
+  l.parts = 1;
   size_t at = 0;
   auto take = [&at](size_t bytes) {
     const size_t here = at;
@@ -119,10 +134,14 @@ Layout layout_of(long long rows, int GS, int D, int max_blocks, int bs, int ds, 
   l.near_page = take(scored * sizeof(unsigned));
   l.near_key = take(scored * sizeof(unsigned long long));
   if (attention) {
-    l.tables = take((size_t)rows * keep * sizeof(int));
-    l.lens = take((size_t)rows * sizeof(int));
-    l.part_bytes = q4 ? nxt_paged_attention_q4_workspace_size((int)rows, GS, D, 1, keep, bs)
-                      : make_plan((int)rows, GS, D, 1, keep, sms, ds, XPA_SPARSE_ITEMS_PER_SM).ws_bytes;
+    l.parts = head_parts(GS, D, bs, ds, q4);
+    const long long n = rows * l.parts;
+    l.tables = take((size_t)n * keep * sizeof(int));
+    l.lens = take((size_t)n * sizeof(int));
+    l.part_bytes = q4 ? nxt_paged_attention_q4_workspace_size((int)n, GS, D, 1, keep, bs)
+                      : make_plan((int)n, GS / l.parts, D, 1, keep, sms, ds,
+                                  XPA_SPARSE_ITEMS_PER_SM)
+                            .ws_bytes;
     l.part = take(l.part_bytes);
   }
   l.total = at;
@@ -155,8 +174,8 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
   if (ws && !workspace_aligned(ws)) return NXT_PA_EINVAL;
   const long long rows = (long long)c.B * c.Hkv;
   const int GS = c.Hq / c.Hkv;
-  if (rows * ceil_div(c.max_blocks, xpa::kScoreChunkScalar) > INT_MAX || rows * GS > INT_MAX ||
-      rows * c.keep > INT_MAX)
+  if (rows * ceil_div(c.max_blocks, xpa::kScoreTile) > INT_MAX || rows * GS > INT_MAX ||
+      rows * c.keep > INT_MAX / 8)
     return NXT_PA_EINVAL;
   const long long head_pages = c.Hkv > 1 ? c.kbs / c.khs : 1;
   const int64_t page_stride = c.Hkv > 1 ? c.khs : c.kbs;
@@ -204,9 +223,11 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
   p.keep = c.keep;
   p.sink = c.sink;
   p.recent = c.recent;
+  p.copies = l.parts;
   p.sign = c.scale > 0.f ? 1.f : c.scale < 0.f ? -1.f : 0.f;
   p.vec = c.ds == 2 && c.D % 8 == 0 && aligned(c.q, 16) && aligned(c.bounds, 16);
-  p.chunk_pages = p.vec ? xpa::kScoreChunk : xpa::kScoreChunkScalar;
+  p.chunk_pages = p.vec ? xpa::score_chunk(c.B, c.Hkv, c.max_blocks, sm_count_of(dev))
+                        : xpa::kScoreChunkScalar;
   p.tile_pages = p.vec ? xpa::kScoreTile : xpa::kScoreChunkScalar;
   p.chunks = ceil_div(c.max_blocks, p.chunk_pages);
   p.tiles = ceil_div(c.max_blocks, p.tile_pages);
@@ -222,9 +243,9 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
                                      GS, c.D, 1, c.scale, c.keep, c.bs, c.k_scale,
                                      c.v_scale, page_stride, c.khs, nb, part, l.part_bytes, status,
                                      st);
-  return attention_planned(c.out, c.q, c.k, c.v, p.sel_tables, p.sel_lens, (int)rows, GS, c.D, 1,
-                           c.scale, c.keep, c.bs, c.ds, page_stride, c.khs, nb, part, l.part_bytes,
-                           status, st, XPA_SPARSE_ITEMS_PER_SM);
+  return attention_planned(c.out, c.q, c.k, c.v, p.sel_tables, p.sel_lens, (int)rows * l.parts,
+                           GS / l.parts, c.D, 1, c.scale, c.keep, c.bs, c.ds, page_stride, c.khs, nb,
+                           part, l.part_bytes, status, st, XPA_SPARSE_ITEMS_PER_SM);
 }
 
 }  // namespace
@@ -313,7 +334,7 @@ size_t nxt_paged_attention_sparse_workspace_size(int num_seqs, int num_heads, in
       max_pages <= 0 || max_num_blocks_per_seq < 0)
     return 0;
   const long long rows = (long long)num_seqs * num_kv_heads;
-  if (rows > INT_MAX) return 0;
+  if (rows > INT_MAX / 8) return 0;
   const int GS = num_heads / num_kv_heads;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) dev = -1;
