@@ -36,48 +36,47 @@ __device__ __forceinline__ bool q4_row_at(const Q4RowsParams& a, int t, RowAt& r
   return true;
 }
 
-// Piece j of a token: its head, its K or V row, its 8 channels.
+// Piece j of a token: its head, its K or V row, its 8 channels, and where they
+// are in the tile. K and V lanes go the same way: 16 codes each at two places.
 struct Piece {
   int h, v;
   bool is_v;
+  int code, code2, scale;  // byte offsets of the codes' halves and the scale
 };
-__device__ __forceinline__ Piece q4_piece(const Q4RowsParams& a, int j) {
-  const int per_head = a.D / 4;  // pieces of K and V
+__device__ __forceinline__ Piece q4_piece(int D, int tok, int j) {
+  const int per_head = D / 4;  // pieces of K and V
   Piece c;
-  c.h = a.D == 128 ? j >> 5 : j / per_head;
+  c.h = j / per_head;
   const int i = j - c.h * per_head;
   c.is_v = i >= per_head / 2;
   c.v = c.is_v ? i - per_head / 2 : i;
+  c.code = c.is_v ? q4_v_off(D, tok, c.v) : q4_k_off(D, tok, c.v);
+  c.code2 = c.code + (c.is_v ? 2 : D / 8);
+  c.scale = c.is_v ? q4_v_scale_off(D, tok, c.v >> 1) : q4_k_scale_off(D, tok, c.v >> 1);
   return c;
 }
 
-// x / y rounded to nearest, from r = 1 / y rounded to nearest: the quotient
-// estimate's residual is exact in one fused step and corrects it (Markstein,
-// IBM J. Res. Dev. 34, 1990; y > 0, its significand not all ones, nothing near
-// the range's ends). The sign is x's, a zero's too.
-__device__ __forceinline__ float div_by(float x, float y, float r) {
-  const float q = x * r;
-  return copysignf(fmaf(fmaf(-q, y, x), r, q), x);
-}
-
-template <int P>
+template <int P, int DC>
 __global__ void __launch_bounds__(128) pa_q4_write_kernel(const Q4RowsParams a) {
+  const int D = DC ? DC : a.D;
   const int w = (int)(((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5);
   const int lane = threadIdx.x & 31;
   const int t = w / a.warps_per_token, first = (w - t * a.warps_per_token) * 32 * P;
   if (t >= a.num_tokens) return;
-  const int pieces = a.Hkv * (a.D / 4);
+  const int pieces = a.Hkv * (D / 4);
   RowAt r;
   const bool live = q4_row_at(a, t, r);
+  const long long src = (long long)t * a.token_stride;
+  const int tok = live ? r.tok : 0;
   uint4 x4[P];
 #pragma unroll
   for (int k = 0; k < P; ++k) {
     const int j = first + 32 * k + lane;
     x4[k] = make_uint4(0u, 0u, 0u, 0u);
     if (j >= pieces) continue;
-    const Piece c = q4_piece(a, j);
-    const __half* row = static_cast<const __half*>(c.is_v ? a.value : a.key) +
-                        (long long)t * a.token_stride + (long long)c.h * a.D + c.v * 8;
+    const Piece c = q4_piece(D, tok, j);
+    const __half* row =
+        static_cast<const __half*>(c.is_v ? a.value : a.key) + src + c.h * D + c.v * 8;
     if (a.vec16) {
       x4[k] = __ldg(reinterpret_cast<const uint4*>(row));
     } else {
@@ -91,15 +90,26 @@ __global__ void __launch_bounds__(128) pa_q4_write_kernel(const Q4RowsParams a) 
   for (int k = 0; k < P; ++k) {
     const int j = first + 32 * k + lane;
     if (first + 32 * k >= pieces) break;  // warp-uniform
-    const Piece c = q4_piece(a, j);
+    const Piece c = q4_piece(D, tok, j);
     const float ps = c.is_v ? a.v_scale : a.k_scale, inv = c.is_v ? a.v_inverse : a.k_inverse;
     const uint32_t u[4] = {x4[k].x, x4[k].y, x4[k].z, x4[k].w};
     float x[8], amax = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 f = unpack_half2(u[i]);
-      x[2 * i] = a.divide ? __fdiv_rn(f.x, ps) : div_by(f.x, ps, inv);
-      x[2 * i + 1] = a.divide ? __fdiv_rn(f.y, ps) : div_by(f.y, ps, inv);
+      x[2 * i] = div_by(f.x, ps, inv);
+      x[2 * i + 1] = div_by(f.y, ps, inv);
+    }
+    if (a.divide) {  // a scale that div_by does not take
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        const float y = __half2float(__ushort_as_half(
+            (unsigned short)((i < 2 ? x4[k].x : i < 4 ? x4[k].y : i < 6 ? x4[k].z : x4[k].w) >>
+                             (16 * (i & 1)))));
+        const float q = __fdiv_rn(y, ps);
+#pragma unroll
+        for (int m = 0; m < 8; ++m) x[m] = m == i ? q : x[m];
+      }
     }
     // A quotient that is an infinity or a NaN (an infinity's residual is one)
     // stands for an infinity, here any value whose scale saturates, or a NaN: 0.
@@ -122,39 +132,32 @@ __global__ void __launch_bounds__(128) pa_q4_write_kernel(const Q4RowsParams a) 
     if (j >= pieces) continue;
     const uint32_t sb = q4_scale(amax);
     const float s = fp8_to_float<kKvE4M3>((uint8_t)sb);
-    const float si = s > 0.f ? __frcp_rn(s) : 0.f;  // no scale: all codes 0
+    const float si = s > 0.f ? __frcp_rn(s) : 0.f;
     uint32_t code = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      code |= q4_pair(div_by(x[2 * i], s, si), div_by(x[2 * i + 1], s, si)) << (8 * i);
-    uint8_t* tile = static_cast<uint8_t*>(c.is_v ? a.value_cache : a.key_cache) + r.tile +
-                    (long long)c.h * a.kv_head_stride;
-    if (!(s > 0.f)) code = 0;
-    if (c.is_v) {
-      *reinterpret_cast<uint32_t*>(tile + q4_v_off(a.D, r.tok, c.v)) = code;
-      if ((c.v & 1) == 0) tile[q4_v_scale_off(a.D, r.tok, c.v >> 1)] = (uint8_t)sb;
-    } else {
-      uint8_t* dst = tile + q4_k_off(a.D, r.tok, c.v);
-      *reinterpret_cast<uint16_t*>(dst) = (uint16_t)code;
-      *reinterpret_cast<uint16_t*>(dst + a.D / 8) = (uint16_t)(code >> 16);
-      if ((c.v & 1) == 0) tile[q4_k_scale_off(a.D, r.tok, c.v >> 1)] = (uint8_t)sb;
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack_half2(u[i]);  // the signs, zeros' too
+      code |= q4_pair(copysignf(div_by(x[2 * i], s, si), f.x),
+                      copysignf(div_by(x[2 * i + 1], s, si), f.y))
+              << (8 * i);
     }
+    if (!(s > 0.f)) code = 0;  // no scale
+    uint8_t* tile = static_cast<uint8_t*>(c.is_v ? a.value_cache : a.key_cache) + r.tile +
+                    c.h * a.kv_head_stride;
+    *reinterpret_cast<uint16_t*>(tile + c.code) = (uint16_t)code;
+    *reinterpret_cast<uint16_t*>(tile + c.code2) = (uint16_t)(code >> 16);
+    if ((c.v & 1) == 0) tile[c.scale] = (uint8_t)sb;
   }
 }
 
-// c * s * ps, rounded to fp16 once and kept finite: a group's largest element
-// may have been rounded up past the fp16 range.
-__device__ __forceinline__ float q4_value(float cs, float ps) {
-  return fminf(fmaxf(cs * ps, -65504.f), 65504.f);
-}
-
-template <int P>
+template <int P, int DC>
 __global__ void __launch_bounds__(128) pa_q4_read_kernel(const Q4RowsParams a) {
+  const int D = DC ? DC : a.D;
   const int w = (int)(((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5);
   const int lane = threadIdx.x & 31;
   const int t = w / a.warps_per_token, first = (w - t * a.warps_per_token) * 32 * P;
   if (t >= a.num_tokens) return;
-  const int pieces = a.Hkv * (a.D / 4);
+  const int pieces = a.Hkv * (D / 4);
   RowAt r;
   const bool live = q4_row_at(a, t, r);
   uint32_t code[P], sb[P];
@@ -163,35 +166,36 @@ __global__ void __launch_bounds__(128) pa_q4_read_kernel(const Q4RowsParams a) {
     const int j = first + 32 * k + lane;
     code[k] = sb[k] = 0u;  // a row of zeros
     if (!live || j >= pieces) continue;
-    const Piece c = q4_piece(a, j);
+    const Piece c = q4_piece(D, r.tok, j);
     const uint8_t* tile = static_cast<const uint8_t*>(c.is_v ? a.value_cache : a.key_cache) +
-                          r.tile + (long long)c.h * a.kv_head_stride;
-    if (c.is_v) {
-      code[k] = __ldg(reinterpret_cast<const uint32_t*>(tile + q4_v_off(a.D, r.tok, c.v)));
-      sb[k] = __ldg(tile + q4_v_scale_off(a.D, r.tok, c.v >> 1));
-    } else {
-      const uint8_t* at = tile + q4_k_off(a.D, r.tok, c.v);
-      code[k] = __ldg(reinterpret_cast<const uint16_t*>(at)) |
-                ((uint32_t)__ldg(reinterpret_cast<const uint16_t*>(at + a.D / 8)) << 16);
-      sb[k] = __ldg(tile + q4_k_scale_off(a.D, r.tok, c.v >> 1));
-    }
+                          r.tile + c.h * a.kv_head_stride;
+    code[k] = __ldg(reinterpret_cast<const uint16_t*>(tile + c.code)) |
+              ((uint32_t)__ldg(reinterpret_cast<const uint16_t*>(tile + c.code2)) << 16);
+    sb[k] = __ldg(tile + c.scale);
   }
 #pragma unroll
   for (int k = 0; k < P; ++k) {
     const int j = first + 32 * k + lane;
     if (j >= pieces) break;
-    const Piece c = q4_piece(a, j);
-    const float s = fp8_to_float<kKvE4M3>((uint8_t)sb[k]);
+    const Piece c = q4_piece(D, 0, j);
+    const uint32_t s2 = fp8x2_to_h2<kKvE4M3>(sb[k]);
     const float ps = c.is_v ? a.v_scale : a.k_scale;
     uint32_t h[4], o[4];
     q4x8_to_h2(code[k], h);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack_half2(h[i]);
-      o[i] = live ? pack_half2(q4_value(f.x * s, ps), q4_value(f.y * s, ps)) : 0u;
+      // c * s is exact in fp16, times ps in fp32, rounded to fp16 and, where a
+      // group's largest element may have been rounded up past the range, kept finite
+      const float2 f = unpack_half2(h2_mul_low(h[i], s2));
+      float x = f.x * ps, y = f.y * ps;
+      if (a.clamp) {
+        x = fminf(fmaxf(x, -65504.f), 65504.f);
+        y = fminf(fmaxf(y, -65504.f), 65504.f);
+      }
+      o[i] = pack_half2(x, y);
     }
     __half* dst = static_cast<__half*>(c.is_v ? a.value : a.key) +
-                  (long long)t * a.token_stride + (long long)c.h * a.D + c.v * 8;
+                  (long long)t * a.token_stride + c.h * D + c.v * 8;
     if (a.vec16) {
       *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
     } else {
@@ -994,11 +998,16 @@ cudaError_t launch_rows(void (*one)(Q4RowsParams), void (*four)(Q4RowsParams),
 }  // namespace
 
 cudaError_t launch_q4_write(const Q4RowsParams& a, cudaStream_t st) {
-  return launch_rows(pa_q4_write_kernel<1>, pa_q4_write_kernel<4>, a, st);
+  // head size 128, where most rows come from, with its address arithmetic folded
+  if (a.D == 128)
+    return launch_rows(pa_q4_write_kernel<1, 128>, pa_q4_write_kernel<4, 128>, a, st);
+  return launch_rows(pa_q4_write_kernel<1, 0>, pa_q4_write_kernel<4, 0>, a, st);
 }
 
 cudaError_t launch_q4_read(const Q4RowsParams& a, cudaStream_t st) {
-  return launch_rows(pa_q4_read_kernel<1>, pa_q4_read_kernel<4>, a, st);
+  if (a.D == 128)
+    return launch_rows(pa_q4_read_kernel<1, 128>, pa_q4_read_kernel<4, 128>, a, st);
+  return launch_rows(pa_q4_read_kernel<1, 0>, pa_q4_read_kernel<4, 0>, a, st);
 }
 
 }  // namespace xpa

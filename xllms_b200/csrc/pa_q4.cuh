@@ -68,9 +68,18 @@ __device__ __forceinline__ uint32_t h2_mul_high(uint32_t a, uint32_t s) {
 }
 
 // ── encoding ────────────────────────────────────────────────────────────
+// x / y rounded to nearest, from r = 1 / y rounded to nearest: the quotient
+// estimate's residual is exact in one fused step and corrects it (Markstein,
+// IBM J. Res. Dev. 34, 1990; y > 0, its significand not all ones, nothing near
+// the range's ends). The sign of a zero is lost.
+__device__ __forceinline__ float div_by(float x, float y, float r) {
+  const float q = x * r;
+  return fmaf(fmaf(-q, y, x), r, q);
+}
+
 // The E4M3 scale of a group whose largest |t| is amax.
 __device__ __forceinline__ uint32_t q4_scale(float amax) {
-  return float2_to_fp8x2<kKvE4M3>(__fdiv_rn(amax, 6.f), 0.f) & 0xffu;
+  return float2_to_fp8x2<kKvE4M3>(div_by(amax, 6.f, 1.f / 6.f), 0.f) & 0xffu;
 }
 // t / s as two E2M1 codes, a in the low nibble.
 __device__ __forceinline__ uint32_t q4_pair(float a, float b) {

@@ -22,6 +22,7 @@ struct Q4RowsParams {
   float k_scale, v_scale;
   float k_inverse, v_inverse;  // 1 / scale rounded to nearest
   int divide;                  // 1: divide by the scales instead
+  int clamp;                   // 1: a value read back may pass the fp16 range
   int sms;
   int warps_per_token;  // set by the launchers
 };

@@ -70,6 +70,7 @@ int rows_call(bool write, void* key, void* value, void* kc, void* vc, const int6
   a.k_inverse = inverse_of(ks);
   a.v_inverse = inverse_of(vs);
   a.divide = a.k_inverse == 0.f || a.v_inverse == 0.f;
+  a.clamp = !(6.f * 448.f * std::max(ks, vs) <= 65504.f);
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return NXT_PA_ECUDA;
   a.sms = sm_count_of(dev);
