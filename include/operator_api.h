@@ -323,8 +323,8 @@ int nxt_paged_attention_fp8_append_ex(
  * head_size is a multiple of 16 up to 256, block_size a multiple of 16.
  * Pools are bytes: page p of KV head h starts at p * kv_block_stride +
  * h * kv_head_stride (strides in bytes, multiples of 16, kv_block_stride
- * below 2^31; pools start on 16-byte boundaries) and holds block_size / 16 tiles of 9 * head_size bytes,
- * one per 16 tokens:
+ * below 2^31; pools start on 16-byte boundaries) and holds block_size / 16
+ * tiles of 9 * head_size bytes, one per 16 tokens:
  *   K: 16 rows of head_size / 2 code bytes, then scales [16][head_size / 16];
  *      a row is, for t = 0..3, for j = 0..head_size / 16 - 1, the codes of
  *      channels 16 j + 4 t .. 16 j + 4 t + 3 (two per byte, low nibble first);
@@ -349,7 +349,8 @@ int nxt_reshape_and_cache_q4(
 
 /* Reads rows back: row t of key/value (fp16, token_stride elements) receives
  * the values at slot slot_mapping[t], rounded to fp16 and at most its largest
- * finite value; a slot that the write would skip gives a row of zeros. Slots may repeat. */
+ * finite value; a slot that the write would skip gives a row of zeros. Slots
+ * may repeat. */
 int nxt_read_cache_q4(
     void *key, void *value,
     const void *key_cache, const void *value_cache,
@@ -364,8 +365,11 @@ int nxt_read_cache_q4(
  * nxt_paged_attention_ex over the dequantised cache, for any number of query
  * heads per KV head. Masking, clamping, status bits and workspace as there; a
  * caller-owned workspace needs nxt_paged_attention_q4_workspace_size bytes.
- * The library's own workspace is one per (device, stream): graphs captured on
- * one stream and replayed at the same time need workspaces of their own. */
+ * The library's own workspace is one per (device, stream), and for captured
+ * calls one per capture, which lives as long as the graph. With num_blocks
+ * unknown (<= 0), a page that reaches 2^32 times the largest common divisor of
+ * kv_block_stride and 9 * head_size bytes into the pool is masked like one
+ * outside it; with num_blocks known, such pools are refused. */
 int nxt_paged_attention_q4_ex(
     void *out, const void *query,
     const void *key_cache, const void *value_cache,
@@ -426,7 +430,8 @@ int nxt_paged_attention_q4_append_ex(
 /* Writes the bounds of the pages that hold the last num_new_tokens tokens of
  * each sequence (0: of all its pages), over their valid tokens. To call after
  * the tokens are stored: with the number of tokens added since the last call,
- * or more. dtype_size 2 or 4. */
+ * or more. Sequences that share a page have equally many valid tokens in it.
+ * dtype_size 2 or 4. */
 int nxt_page_bounds(
     void *bounds, const void *key_cache,
     const int *block_tables, const int *seq_lens,

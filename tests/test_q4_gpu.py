@@ -396,3 +396,74 @@ def test_a_run_as_it_is_used(cuda):
                                _expected(prompt[0].cpu().numpy(), KS)[1].astype(np.float64),
                                rtol=2.0 ** -10)
     assert v.shape == (n0 + 5, hkv, D)
+
+
+def test_graphs_replayed_at_the_same_time_have_scratch_of_their_own(cuda):
+    """Two graphs captured on one stream and an eager call, each with partials
+    to merge, run side by side again and again."""
+    import torch
+    side, streams = torch.cuda.Stream(), [torch.cuda.Stream() for _ in range(2)]
+    runs = []
+    for seed in (71, 72, 73):
+        q, pools, table, lens = _case(seed, [6000, 5000, 4000, 7000], 32, 8, 128, 16)
+        args = [_t(x, cuda) for x in (q, pools[0], pools[1], table, lens)]
+        want = PA.paged_attention_q4(*args, KS, VS)
+        runs.append((args, want, torch.empty_like(want)))
+    assert PA.q4_workspace_size(4, 32, 128, 8, table.shape[1]) > 0
+    torch.cuda.synchronize()
+    graphs = []
+    for args, _, out in runs[:2]:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            for _ in range(4):
+                PA.paged_attention_q4(*args, KS, VS, out=out)
+    for _ in range(20):
+        for _, _, out in runs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+        for _ in range(4):
+            PA.paged_attention_q4(*runs[2][0], KS, VS, out=runs[2][2], stream=side)
+        torch.cuda.synchronize()
+        for _, want, out in runs:
+            assert torch.equal(out, want)
+    assert _native.xpa().nxt_paged_attention_release_workspaces() == _native.NXT_PA_OK
+    runs[0][2].zero_()  # a graph keeps its scratch
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(runs[0][2], runs[0][1])
+
+
+def test_graphs_that_are_gone_give_their_scratch_back(cuda):
+    import torch
+    q, pools, table, lens = _case(74, [6000] * 24, 32, 8, 128, 16)
+    args = [_t(x, cuda) for x in (q, pools[0], pools[1], table, lens)]
+    out = PA.paged_attention_q4(*args, KS, VS)
+    need = PA.q4_workspace_size(24, 32, 128, 8, table.shape[1])
+    assert need > 2 ** 20
+    side = torch.cuda.Stream()
+    free = []
+    for _ in range(40):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            PA.paged_attention_q4(*args, KS, VS, out=out)
+        graph.replay()
+        torch.cuda.synchronize()
+        del graph
+        torch.cuda.synchronize()
+        free.append(torch.cuda.mem_get_info()[0])
+    # the driver's thread may lag some captures behind
+    assert free[0] - free[-1] < 20 * need
+
+
+def test_more_blocks_than_the_pools_have_are_refused(cuda):
+    q, pools, table, lens = _case(75, [100], 8, 2, 128, 16)
+    args = [_t(x, cuda) for x in (q, pools[0], pools[1], table, lens)]
+    nb = pools[0].shape[0]
+    want = PA.paged_attention_q4(*args, KS, VS)
+    for few in (nb, -1):
+        assert (PA.paged_attention_q4(*args, KS, VS, num_blocks=few) == want).all()
+    with pytest.raises(PA.PagedAttentionError):
+        PA.paged_attention_q4(*args, KS, VS, num_blocks=nb + 1)

@@ -8,9 +8,11 @@
 #include <cstdio>
 #include <cstring>
 #include <map>
+#include <memory>
 #include <algorithm>
 #include <cmath>
 #include <mutex>
+#include <new>
 #include <thread>
 #include <functional>
 #include <utility>
@@ -63,9 +65,74 @@ struct Workspace {
 std::map<std::pair<int, uintptr_t>, Workspace> g_ws;
 
 // Scratch of the 4-bit and sparse entry points (acquire_scratch).
+struct Scratch {
+  Workspace eager;     // of calls that run at once
+  Workspace captured;  // of the calls in one stream capture
+  unsigned long long capture = 0;  // which
+};
 std::mutex g_scratch_mu;
-std::map<std::pair<int, uintptr_t>, Workspace> g_scratch;
+std::map<std::pair<int, uintptr_t>, Scratch> g_scratch;
 std::vector<std::pair<int, void*>> g_scratch_old;  // outgrown buffers, by device
+
+// A captured call's buffer belongs to its graph and comes back here when the
+// graph and what was instantiated from it are gone. That happens on a thread
+// of the driver's, possibly while the process ends: neither is ever destroyed.
+struct GraphBuffer {
+  int dev;
+  void* ptr;
+  size_t bytes;
+};
+std::mutex& g_back_mu = *new std::mutex;
+std::vector<GraphBuffer>& g_back = *new std::vector<GraphBuffer>;
+
+void CUDART_CB give_back(void* p) {
+  std::unique_ptr<GraphBuffer> b(static_cast<GraphBuffer*>(p));
+  std::lock_guard<std::mutex> lk(g_back_mu);
+  try {
+    g_back.push_back(*b);
+  } catch (...) {  // the buffer is lost, nothing else
+  }
+}
+
+// A buffer for the graph that is being captured: one that came back and is not
+// more than four times too large, or a new one.
+int buffer_of_graph(int dev, cudaGraph_t graph, size_t bytes, Workspace* out) {
+  std::unique_ptr<GraphBuffer> b(new GraphBuffer{dev, nullptr, bytes});
+  {
+    std::lock_guard<std::mutex> lk(g_back_mu);
+    for (size_t i = 0; i < g_back.size(); ++i)
+      if (g_back[i].dev == dev && g_back[i].bytes >= bytes && g_back[i].bytes / 4 <= bytes) {
+        *b = g_back[i];
+        g_back[i] = g_back.back();
+        g_back.pop_back();
+        break;
+      }
+  }
+  if (!b->ptr) {
+    // an allocation is no part of the capture
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return NXT_PA_ECUDA;
+    const cudaError_t e = cudaMalloc(&b->ptr, bytes);
+    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess || e != cudaSuccess) {
+      cudaGetLastError();
+      return NXT_PA_ENOMEM;
+    }
+  }
+  const Workspace w{b->ptr, b->bytes};
+  cudaUserObject_t obj;
+  if (cudaUserObjectCreate(&obj, b.get(), give_back, 1, cudaUserObjectNoDestructorSync) !=
+      cudaSuccess) {
+    give_back(b.release());
+    return NXT_PA_ECUDA;
+  }
+  b.release();  // the object's
+  if (cudaGraphRetainUserObject(graph, obj, 1, cudaGraphUserObjectMove) != cudaSuccess) {
+    cudaUserObjectRelease(obj, 1);
+    return NXT_PA_ECUDA;
+  }
+  *out = w;
+  return NXT_PA_OK;
+}
 
 int map_cuda(cudaError_t e) { return e == cudaSuccess ? NXT_PA_OK : NXT_PA_ECUDA; }
 
@@ -135,24 +202,45 @@ int status_word(int dev, int** out) {
 }
 
 int acquire_scratch(int dev, cudaStream_t st, size_t bytes, void** out,
-                    std::unique_lock<std::mutex>& lk) {
+                    std::unique_lock<std::mutex>& lk) try {
   if (dev < 0 || dev >= kMaxDevices) return NXT_PA_EINVAL;
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  cudaGraph_t graph = nullptr;
+  if (cudaStreamGetCaptureInfo(st, &capturing, &id, &graph) != cudaSuccess) {
+    cudaGetLastError();
+    return NXT_PA_ECUDA;
+  }
   lk = std::unique_lock<std::mutex>(g_scratch_mu);
-  Workspace& w = g_scratch[{dev, stream_key(st)}];
+  Scratch& s = g_scratch[{dev, stream_key(st)}];
+  if (capturing == cudaStreamCaptureStatusActive) {
+    if (s.capture != id || s.captured.bytes < bytes) {
+      const int rc = buffer_of_graph(dev, graph, bytes, &s.captured);
+      if (rc != NXT_PA_OK) return rc;
+      s.capture = id;
+    }
+    *out = s.captured.ptr;
+    return NXT_PA_OK;
+  }
+  Workspace& w = s.eager;
   if (w.bytes < bytes) {
     // at least doubled, so that what is kept of old buffers stays below the newest
     const size_t want = std::max(bytes, 2 * w.bytes);
+    if (w.ptr) g_scratch_old.reserve(g_scratch_old.size() + 1);
     void* p = nullptr;
     if (cudaMalloc(&p, want) != cudaSuccess) {
       cudaGetLastError();
       return NXT_PA_ENOMEM;
     }
+    // its last calls may still run
     if (w.ptr) g_scratch_old.emplace_back(dev, w.ptr);
     w.ptr = p;
     w.bytes = want;
   }
   *out = w.ptr;
   return NXT_PA_OK;
+} catch (const std::bad_alloc&) {
+  return NXT_PA_ENOMEM;
 }
 
 int release_scratch() {
@@ -163,8 +251,14 @@ int release_scratch() {
   auto drop = [&rc](int dev, void* p) {
     if (p && (cudaSetDevice(dev) != cudaSuccess || cudaFree(p) != cudaSuccess)) rc = NXT_PA_ECUDA;
   };
-  for (auto& kv : g_scratch) drop(kv.first.first, kv.second.ptr);
+  for (auto& kv : g_scratch) drop(kv.first.first, kv.second.eager.ptr);
   for (auto& o : g_scratch_old) drop(o.first, o.second);
+  std::vector<GraphBuffer> back;
+  {
+    std::lock_guard<std::mutex> lb(g_back_mu);
+    back.swap(g_back);
+  }
+  for (auto& o : back) drop(o.dev, o.ptr);  // those of living graphs stay theirs
   g_scratch.clear();
   g_scratch_old.clear();
   if (have_prev) cudaSetDevice(prev);

@@ -93,12 +93,14 @@ cudaError_t smem_limit(Kernel kern, size_t bytes, bool carve, std::atomic<unsign
 // The library status word of device `dev` (the current device).
 int status_word(int dev, int** out);
 
-// Library-owned scratch of the 4-bit and sparse entry points, one buffer per
-// (device, stream). `lk` holds the pool's lock on return: keep it until the
-// call's kernels are enqueued, so that no other thread on the same stream can
-// hand out the buffer in between. A buffer that has to grow is replaced, and
-// the old one kept until release_scratch(), since a captured graph may still
-// name it. EINVAL / ENOMEM / OK.
+// Library-owned scratch of the 4-bit and sparse entry points: one buffer per
+// (device, stream) for calls that run at once, and one per stream capture for
+// captured calls, which the graph owns, so that graphs may be replayed at the
+// same time as each other and as eager calls. `lk` holds the pool's lock on
+// return: keep it until the call's kernels are enqueued, so that no other
+// thread on the same stream can hand out the buffer in between. A buffer that
+// has to grow is replaced, and the old one kept until release_scratch().
+// EINVAL / ECUDA / ENOMEM / OK.
 int acquire_scratch(int dev, cudaStream_t st, size_t bytes, void** out,
                     std::unique_lock<std::mutex>& lk);
 int release_scratch();

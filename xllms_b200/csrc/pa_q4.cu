@@ -18,7 +18,12 @@ namespace {
 // K before V; a lane takes a piece, neighbouring lanes a 16-channel group, and
 // a warp P times 32 pieces, whose reads are all in flight together: four where
 // that still leaves the GPU warps enough, one for the few tokens of a decode
-// step, whose time is the chain of one piece.
+// step, whose time is the chain of one piece. HBM is not the bound: storing 8192
+// tokens x 8 heads x 128 and reading them back (43 MB each) takes 32 us, where the
+// bytes alone take 13, with 80 % of the issue slots used: the corrected
+// quotients, conversions and addresses are 30 instructions a channel to write
+// and 18 to read. A quotient by the reciprocal alone would be off by an ulp,
+// and a code by a step wherever that crosses a midpoint.
 // ════════════════════════════════════════════════════════════════════════
 
 struct RowAt {
@@ -229,6 +234,20 @@ __global__ void __launch_bounds__(128) pa_q4_read_kernel(const Q4RowsParams a) {
 // (2^-11 relative at most, next to codes of 1 mantissa bit) down to 2^-21 of
 // the largest and 2^-32 of it absolutely below. A second fp16 term for the
 // rest of p would cost a ninth of the kernel's time.
+//
+// Bound and measured: 64 sequences of 1-8K tokens, 32 heads over 8 of 128 (336
+// MB), take 78 us, 0.65 of the copy rate: 62 us if nothing is computed, 81 if
+// nothing is copied (two fp16 terms then). At the copy rate an SM has 3.1 issue
+// slots for 32 elements and the kernel uses 2.9 (0.5 each of them conversions
+// and scalings), with the issue slots 61 % and the conversions' half-rate pipe
+// 50 % busy, the tensor pipe 25 %. So the shape that counts is the one with the
+// fewest instructions per element: K and V go through mma.sync straight from
+// registers, where tcgen05 would want the unpacked fp16 operands written to
+// shared memory first (3.6 times the bytes that were read) and the few rows of
+// heads would fill a sixteenth of its tiles; and two tiles a step give a warp
+// two independent chains. A loop over the ring's stages instead of their
+// unrolling, a third stage, a fifth CTA per SM and Q kept in shared memory were
+// each slower.
 // ════════════════════════════════════════════════════════════════════════
 constexpr float kRaise = 8.f;  // log2 units a score may exceed m by
 constexpr float kShift = 7.f;  // p = 2^(x - m + kShift) <= 2^15
@@ -898,26 +917,24 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t
 #ifndef XPA_Q4_TILES
 #define XPA_Q4_TILES 2
 #endif
-#ifndef XPA_Q4_TILES_ODD
-#define XPA_Q4_TILES_ODD 1
-#endif
-#ifndef XPA_Q4_MIN_CTAS_ODD
-#define XPA_Q4_MIN_CTAS_ODD 3
-#endif
 #ifndef XPA_Q4_STAGES
 #define XPA_Q4_STAGES 2
 #endif
 #ifndef XPA_Q4_MIN_CTAS
 #define XPA_Q4_MIN_CTAS 4
 #endif
+#ifndef XPA_Q4_MIN_CTAS_ODD
+#define XPA_Q4_MIN_CTAS_ODD 2
+#endif
 
 template <int D, int NT>
 cudaError_t launch_q4_t(const Params& p, cudaStream_t st) {
   constexpr bool EXACT = Q4Stage<D>::EXACT;
   constexpr int NW = XPA_Q4_WARPS;
-  // the other head sizes take more registers per tile: one at a time, a longer ring
-  constexpr int U = EXACT ? XPA_Q4_TILES : XPA_Q4_TILES_ODD;
-  constexpr int STAGES = U == 1 ? 4 : XPA_Q4_STAGES;
+  // two tiles a step against one and a ring of four, 64 sequences of 1-8K tokens:
+  // D = 96 74 against 77 us, 160 109 / 115, 240 206 / 226
+  constexpr int U = XPA_Q4_TILES, STAGES = XPA_Q4_STAGES;
+  // the head sizes without a swizzle of their own take more registers
   constexpr int MINB = D <= 128 && NT == 1 ? (EXACT ? XPA_Q4_MIN_CTAS : XPA_Q4_MIN_CTAS_ODD) : 1;
   using C = Q4Cfg<D, NT, NW, STAGES, U>;
   auto kern = pa_q4_kernel<D, NT, NW, STAGES, U, MINB>;
@@ -981,8 +998,8 @@ cudaError_t launch_q4_attention(const Params& p, cudaStream_t st) {
 namespace {
 
 // Launches one of a rows kernel's two forms: four pieces a lane from 8 warps of
-// them per SM on (8192 tokens x 8 heads x 128, write and read: one 51 us, four
-// XX us; 64 tokens: 4.7 against 8.2 us).
+// them per SM on (8 heads x 128, write and read: 8192 tokens 32 us with four
+// pieces, 41 with one; 64 tokens 6.6 against 3.9 us).
 cudaError_t launch_rows(void (*one)(Q4RowsParams), void (*four)(Q4RowsParams),
                         const Q4RowsParams& a, cudaStream_t st) {
   Q4RowsParams p = a;

@@ -82,7 +82,7 @@ int rows_call(bool write, void* key, void* value, void* kc, void* vc, const int6
 // XPA_Q4_ITEMS_PER_SM items per SM, but not below 8, nor below sqrt(tiles / 2):
 // with few rows, a shorter partition saves its own time and costs as much in
 // the merge of the longer list of partials (2 rows of 3254 tiles, D = 256: 8
-// tiles 47 us, 19 + 31 in the merge; 64 tiles 21).
+// tiles 47 us, 64 tiles 23).
 #ifndef XPA_Q4_PART_TILES
 #define XPA_Q4_PART_TILES 128
 #endif

@@ -92,7 +92,7 @@ struct SparseCall {
 
 // Items per SM below which the attention over the kept pages splits its rows
 // further. A row holds few pages here, so the partials of a finer split cost
-// more than an idle SM.
+// more than an idle SM (64 rows of 256 pages, whole sparse call: 3 90 us, 8 95).
 #ifndef XPA_SPARSE_ITEMS_PER_SM
 #define XPA_SPARSE_ITEMS_PER_SM 3
 #endif
@@ -100,7 +100,8 @@ struct SparseCall {
 // Parts that a KV head's group of query heads is taken in: the tensor-core
 // decode kernel of fp16 pools reads a page for up to 16 heads (8 at head size
 // 256), and re-reading it from L2 for the next part costs less than the
-// CUDA-core kernel (48 heads over 3 KV heads, D = 256, 18 pages: 83 -> 12 us).
+// CUDA-core kernel (whole sparse call, 8 sequences: 192 heads over 8 KV heads,
+// D = 128, 64 pages: 302 -> 57 us; 48 over 3, D = 256, 18 pages: 116 -> 40).
 int head_parts(int GS, int D, int bs, int ds, bool q4) {
   if (q4 || ds != 2 || bs != 16 || (D != 64 && D != 128 && D != 256)) return 1;
   const int most = D == 256 ? 8 : 16;

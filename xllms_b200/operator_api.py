@@ -590,6 +590,15 @@ def _refuse(where, msg):
     raise PagedAttentionError(_native.NXT_PA_EINVAL, f"{where}: {msg}")
 
 
+def _known_blocks(where, given, nb):
+    """num_blocks of a call: the pools' own by default; <= 0: page ids are not checked."""
+    if given is None:
+        return nb
+    if given > nb:
+        _refuse(where, f"num_blocks {given} of pools with {nb}")
+    return given
+
+
 def _opt_ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -729,7 +738,7 @@ def paged_attention_q4(query, key_cache, value_cache, block_tables, seq_lens, k_
                      key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
                      seq_lens.data_ptr(), B, Hq, d, hkv, d ** -0.5 if scale is None else scale,
                      block_tables.shape[1], bs, k_scale, v_scale, page, head,
-                     nb if num_blocks is None else num_blocks, *_workspace(workspace),
+                     _known_blocks("paged_attention_q4", num_blocks, nb), *_workspace(workspace),
                      _opt_ptr(device_status), st)
     finally:
         if leave is not None:
@@ -767,7 +776,7 @@ def paged_attention_q4_append(query, key_cache, value_cache, block_tables, seq_l
                      seq_lens.data_ptr(), new_key.data_ptr(), new_value.data_ptr(),
                      slot_mapping.data_ptr(), B, Hq, d, hkv, d ** -0.5 if scale is None else scale,
                      block_tables.shape[1], bs, k_scale, v_scale, page, head,
-                     nb if num_blocks is None else num_blocks, _opt_ptr(device_status), st)
+                     _known_blocks(where, num_blocks, nb), _opt_ptr(device_status), st)
     finally:
         if leave is not None:
             leave.close()
@@ -823,7 +832,7 @@ def page_bounds(key_cache, block_tables, seq_lens, bounds, *, num_new_tokens=0, 
     try:
         _native_call(name, bounds.data_ptr(), key_cache.data_ptr(), block_tables.data_ptr(),
                      seq_lens.data_ptr(), B, hkv, d, block_tables.shape[1], bs, kind, page, head,
-                     nb if num_blocks is None else num_blocks, num_new_tokens,
+                     _known_blocks(where, num_blocks, nb), num_new_tokens,
                      _opt_ptr(device_status), st)
     finally:
         if leave is not None:
@@ -866,8 +875,8 @@ def select_pages(query, key_cache, bounds, block_tables, seq_lens, max_pages, *,
                      query.data_ptr(), bounds.data_ptr(), block_tables.data_ptr(),
                      seq_lens.data_ptr(), B, Hq, d, hkv, d ** -0.5 if scale is None else scale,
                      block_tables.shape[1], bs, query.element_size(), page, head,
-                     nb if num_blocks is None else num_blocks, max_pages, sink_pages, recent_pages,
-                     None, 0, _opt_ptr(device_status), st)
+                     _known_blocks("select_pages", num_blocks, nb), max_pages, sink_pages,
+                     recent_pages, None, 0, _opt_ptr(device_status), st)
     finally:
         if leave is not None:
             leave.close()
@@ -907,7 +916,7 @@ def paged_attention_sparse(query, key_cache, value_cache, bounds, block_tables, 
                      value_cache.data_ptr(), bounds.data_ptr(), block_tables.data_ptr(),
                      seq_lens.data_ptr(), _opt_ptr(selected), B, Hq, d, hkv,
                      d ** -0.5 if scale is None else scale, block_tables.shape[1], bs, *kind, page,
-                     head, nb if num_blocks is None else num_blocks, max_pages, sink_pages,
+                     head, _known_blocks(where, num_blocks, nb), max_pages, sink_pages,
                      recent_pages, *_workspace(workspace), _opt_ptr(device_status), st)
     finally:
         if leave is not None:
