@@ -235,13 +235,16 @@ __global__ void __launch_bounds__(128) pa_q4_read_kernel(const Q4RowsParams a) {
 // the largest and 2^-32 of it absolutely below. A second fp16 term for the
 // rest of p would cost a ninth of the kernel's time.
 //
-// Bound and measured: 64 sequences of 1-8K tokens, 32 heads over 8 of 128 (336
-// MB), take 78 us, 0.65 of the copy rate: 62 us if nothing is computed, 81 if
-// nothing is copied (two fp16 terms then). At the copy rate an SM has 3.1 issue
-// slots for 32 elements and the kernel uses 2.9 (0.5 each of them conversions
-// and scalings), with the issue slots 61 % and the conversions' half-rate pipe
-// 50 % busy, the tensor pipe 25 %. So the shape that counts is the one with the
-// fewest instructions per element: K and V go through mma.sync straight from
+// Bound and measured, 32 heads over 8 of 128: 12 sequences of 64K tokens (906
+// MB) take 174 us, 0.79 of the copy rate, 64 of 1-8K (336 MB) 78 us, 0.65, as
+// the items of a ragged batch end apart (shorter items, or the short ones last,
+// were no faster); 62 us if nothing is computed, 81 if nothing is copied (two
+// fp16 terms then). At the copy rate there are 3.1 issue slots for 32 elements
+// and the kernel uses 2.2, half an instruction each of them for conversions and
+// scalings; the long case has the issue slots 65 % busy, the conversions'
+// half-rate pipe 54 %, the tensor pipe 29 %, and a warp waits for its turn, a
+// fixed latency or a pipe. So the shape that counts is the one with the fewest
+// instructions per element: K and V go through mma.sync straight from
 // registers, where tcgen05 would want the unpacked fp16 operands written to
 // shared memory first (3.6 times the bytes that were read) and the few rows of
 // heads would fill a sixteenth of its tiles; and two tiles a step give a warp
