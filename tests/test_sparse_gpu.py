@@ -431,3 +431,62 @@ def test_decode_steps_with_bounds_kept_up_to_date(cuda):
         ref, _ = _sparse_reference(q, kn.astype(np.float64), vn.astype(np.float64), want, tab, lens,
                                    1 / math.sqrt(D))
         check_close(out, ref)
+
+
+@pytest.mark.parametrize("hq,hkv,D,bs,dtype", [
+    (32, 4, 128, 32, np.float16), (10, 5, 64, 64, np.float16), (16, 2, 256, 48, np.float16),
+    (20, 1, 128, 64, np.float16), (32, 2, 208, 64, np.float16), (48, 3, 144, 16, np.float32),
+    (13, 1, 256, 32, np.float16), (22, 1, 64, 32, np.float32)])
+def test_long_pages_and_wide_groups(cuda, hq, hkv, D, bs, dtype):
+    """Pages that attention takes in pieces, groups that it takes in parts; with
+    pages that are not there, and with the number of blocks unknown."""
+    keep, sink, recent = 6, 1, 1
+    lens = [0, 1, bs - 1, bs + 17, 4 * bs, 23 * bs + 5, 40 * bs]
+    q, k, v, table, lens = _case(hq + D + bs, lens, hq, hkv, D, bs, dtype)
+    bnd = _bounds_of(k, table, lens, dtype)
+    table[5, 2:20:3] = -1
+    table[6, 1:30:2] = len(k) + 5
+    want = S.select(q, bnd, table, lens, bs, keep, sink, recent, 1.0, len(k))
+    ref, _ = _sparse_reference(q, k.astype(np.float64), v.astype(np.float64), want, table, lens,
+                               1 / math.sqrt(D))
+    import torch
+    args = [_t(x, cuda) for x in (q, k, v, bnd, table, lens)]
+    kept = torch.empty(len(lens), hkv, keep, dtype=torch.int32, device=cuda)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    ws = torch.empty(PA.sparse_workspace_size(len(lens), hq, D, hkv, table.shape[1], keep, bs,
+                                              np.dtype(dtype).itemsize), dtype=torch.uint8,
+                     device=cuda)
+    out = PA.paged_attention_sparse(*args, keep, sink_pages=sink, recent_pages=recent,
+                                    selected=kept, workspace=ws, device_status=status)
+    np.testing.assert_array_equal(kept.cpu().numpy(), want)
+    assert int(status) == _native.NXT_PA_DEV_BAD_PAGE
+    check_close(out, ref)
+    args[4][args[4] > len(k)] = -1  # the number of blocks bounds no id now
+    out = PA.paged_attention_sparse(*args, keep, sink_pages=sink, recent_pages=recent,
+                                    selected=kept, num_blocks=-1)
+    np.testing.assert_array_equal(kept.cpu().numpy(), want)
+    check_close(out, ref)
+
+
+@pytest.mark.parametrize("hkv,pad", [(2, 2), (1, 16), (1, 8)])
+def test_long_pages_of_padded_pools(cuda, hkv, pad):
+    """Page strides that hold a whole number of 16-token pieces, and one that does not."""
+    import torch
+    hq, D, bs, keep = 4 * hkv, 64, 32, 5
+    q, k, v, table, lens = _case(80 + pad, [700, 77, 33], hq, hkv, D, bs)
+    bnd = _bounds_of(k, table, lens, np.float16)
+    want = S.select(q, bnd, table, lens, bs, keep, 0, 1, 1.0, len(k))
+    ref, _ = _sparse_reference(q, k.astype(np.float64), v.astype(np.float64), want, table, lens,
+                               0.125)
+    extra = pad * bs * D if hkv > 1 else pad * D
+    big = torch.zeros(2, len(k), hkv * bs * D + extra, dtype=torch.float16, device=cuda)
+    big[0, :, :hkv * bs * D] = _t(k.reshape(len(k), -1), cuda)
+    big[1, :, :hkv * bs * D] = _t(v.reshape(len(k), -1), cuda)
+    out = torch.empty(q.shape, dtype=torch.float16, device=cuda)
+    ins = [_t(q, cuda), big[0], big[1], _t(bnd, cuda), _t(table, cuda), _t(lens, cuda)]
+    rc = _native.xpa().nxt_paged_attention_sparse_ex(
+        out.data_ptr(), *(x.data_ptr() for x in ins), None, 3, hq, D, hkv, 0.125, table.shape[1],
+        bs, 2, hkv * bs * D + extra, bs * D, len(k), keep, 0, 1, None, 0, None,
+        torch.cuda.current_stream().cuda_stream)
+    assert rc == _native.NXT_PA_OK
+    check_close(out, ref)

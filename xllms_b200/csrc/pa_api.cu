@@ -302,13 +302,13 @@ int release_scratch() {
 #define XPA_FP8_MIN_ITEMS_PER_SM 24
 #endif
 Plan make_plan(int B, int Hq, int D, int Hkv, int max_blocks, int nsm, int kv_es,
-               int min_items_per_sm) {
+               int min_items_per_sm, int min_pages) {
   Plan pl;
   const long long mb = max_blocks > 0 ? max_blocks : 1;
   int pp = XPA_PART_PAGES;
   const long long min_items =
       (long long)(min_items_per_sm > 0 ? min_items_per_sm : kv_es == 1 ? XPA_FP8_MIN_ITEMS_PER_SM : XPA_MIN_ITEMS_PER_SM) * nsm;
-  while (pp > 4 && (long long)B * Hkv * ceil_div(mb, pp) < min_items) pp >>= 1;
+  while (pp > min_pages && (long long)B * Hkv * ceil_div(mb, pp) < min_items) pp >>= 1;
   while (ceil_div(mb, pp) > 8192) pp <<= 1;
   pl.part_pages = pp;
   pl.max_parts = ceil_div(mb, pp);
@@ -455,7 +455,7 @@ int run(void* out, const void* q, const void* k, const void* v, const int* bt, c
         long long kbs, long long khs, long long num_blocks, void* ws, size_t ws_bytes,
         int* dev_status, cudaStream_t st, const NxtPaShard* shard = nullptr,
         uint64_t step = 0, bool after_append = false, const PrefixArgs* pre = nullptr,
-        const KvQuant* kvq = nullptr, int min_items = 0) {
+        const KvQuant* kvq = nullptr, int min_items = 0, int min_pages = 4) {
   if (shard) {
     if (shard->world_size < 1 || shard->world_size > NXT_PA_MAX_PEERS || shard->rank < 0 ||
         shard->rank >= shard->world_size || step == 0 || shard->head_offset < 0 ||
@@ -483,7 +483,7 @@ int run(void* out, const void* q, const void* k, const void* v, const int* bt, c
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return NXT_PA_ECUDA;
   const int sms = sm_count_of(dev);
-  Plan pl = make_plan(B, Hq, D, Hkv, max_blocks, sms, kv_es, min_items);
+  Plan pl = make_plan(B, Hq, D, Hkv, max_blocks, sms, kv_es, min_items, min_pages);
   // A cascade call needs the TMA path's shapes; others run without the prefix
   // information, which gives the same result.
   CUtensorMap tk, tv;
@@ -667,9 +667,11 @@ namespace host {
 int attention_planned(void* out, const void* q, const void* k, const void* v, const int* bt,
                       const int* sl, int B, int Hq, int D, int Hkv, float scale, int max_blocks,
                       int bs, int ds, long long kbs, long long khs, long long num_blocks, void* ws,
-                      size_t ws_bytes, int* dev_status, cudaStream_t st, int min_items) {
+                      size_t ws_bytes, int* dev_status, cudaStream_t st, int min_items,
+                      int min_pages) {
   return run(out, q, k, v, bt, sl, B, Hq, D, Hkv, scale, max_blocks, bs, ds, kbs, khs, num_blocks,
-             ws, ws_bytes, dev_status, st, nullptr, 0, false, nullptr, nullptr, min_items);
+             ws, ws_bytes, dev_status, st, nullptr, 0, false, nullptr, nullptr, min_items,
+             min_pages);
 }
 
 }  // namespace host

@@ -47,16 +47,18 @@ struct Plan {
 };
 // kv_es: bytes per K / V element (1 for fp8 pools, whose partitions keep
 // shrinking until the grid holds 24 CTAs per SM instead of 12).
-// min_items: items per SM instead of the default floor (0).
+// min_items: items per SM instead of the default floor (0); min_pages: the
+// shortest partition, in pages.
 Plan make_plan(int B, int Hq, int D, int Hkv, int max_blocks, int nsm, int kv_es = 2,
-               int min_items = 0);
+               int min_items = 0, int min_pages = 4);
 
-// nxt_paged_attention_ex with that floor; `ws` holds at least
-// make_plan(...).ws_bytes of the same floor.
+// nxt_paged_attention_ex with these floors; `ws` holds at least
+// make_plan(...).ws_bytes of the same floors.
 int attention_planned(void* out, const void* q, const void* k, const void* v, const int* bt,
                       const int* sl, int B, int Hq, int D, int Hkv, float scale, int max_blocks,
                       int bs, int ds, long long kbs, long long khs, long long num_blocks, void* ws,
-                      size_t ws_bytes, int* dev_status, cudaStream_t st, int min_items);
+                      size_t ws_bytes, int* dev_status, cudaStream_t st, int min_items,
+                      int min_pages);
 
 // Tensor map of one pool for the TMA path; false when it cannot be encoded.
 // es: bytes per K / V element (2 = fp16, 1 = fp8).

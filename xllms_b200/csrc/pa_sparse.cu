@@ -791,28 +791,32 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p, 
   __syncthreads();
   int to = __reduce_add_sync(0xffffffffu, lane < warp ? s_count[lane] : 0);
   const int done = __reduce_add_sync(0xffffffffu, lane < NWARP ? s_count[lane] : 0);
-  int* tab = p.sel_tables + (long long)row * p.copies * p.keep;
+  int* tab = p.sel_tables + (long long)row * p.copies * p.keep * p.sub;
+  int* order = p.order ? p.order + (long long)row * p.keep : tab;
   int* pages = p.sel_pages ? p.sel_pages + (long long)row * p.keep : nullptr;
 #pragma unroll 2
   for (int base = begin; base < stop; base += 32) {
     const bool in = kept(base + lane);
     const unsigned m = __ballot_sync(0xffffffffu, in);
-    if (in) tab[to + __popc(m & ((1u << lane) - 1u))] = base + lane;
+    if (in) order[to + __popc(m & ((1u << lane) - 1u))] = base + lane;
     to += __popc(m);
   }
   __syncthreads();
   // page indices -> per-head page ids, all table reads at once
   bool tail = false;  // the sequence's last page is kept
   for (int i = tid; i < done; i += NT) {
-    const int at = tab[i];
+    const int at = order[i];
     const int e = __ldg(p.block_tables + (long long)b * p.max_blocks + at);
     if (pages) pages[i] = at;
     tail |= at == n - 1;
-    const int id = (int)((long long)e * p.head_pages + h);
-    for (int c = 0; c < p.copies; ++c) tab[(long long)c * p.keep + i] = id;
+    const int id = (int)(((long long)e * p.head_pages + h) * p.sub_ids);
+    for (int c = 0; c < p.copies; ++c)
+      for (int k = 0; k < p.sub; ++k)
+        tab[((long long)c * p.keep + i) * p.sub + k] = id + k;
   }
   for (int i = done + tid; i < p.keep; i += NT) {
-    for (int c = 0; c < p.copies; ++c) tab[(long long)c * p.keep + i] = -1;
+    for (int c = 0; c < p.copies; ++c)
+      for (int k = 0; k < p.sub; ++k) tab[((long long)c * p.keep + i) * p.sub + k] = -1;
     if (pages) pages[i] = -1;
   }
   tail = __syncthreads_or(tail);

@@ -2,6 +2,7 @@
 // (include/operator_api.h). Attention over the kept pages is the framework's
 // own decode attention on per-head pages: page p of KV head h is page
 // p * (kv_block_stride / kv_head_stride) + h of a pool with one KV head.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -97,30 +98,44 @@ struct SparseCall {
 #define XPA_SPARSE_ITEMS_PER_SM 3
 #endif
 
-// Parts that a KV head's group of query heads is taken in: the tensor-core
+bool tma_shape(int D, int bs, int ds) {
+  return ds == 2 && bs == 16 && (D == 64 || D == 128 || D == 256);
+}
+
+// Parts that a KV head's group of query heads is taken in. The tensor-core
 // decode kernel of fp16 pools reads a page for up to 16 heads (8 at head size
 // 256), and re-reading it from L2 for the next part costs less than the
 // CUDA-core kernel (whole sparse call, 8 sequences: 192 heads over 8 KV heads,
 // D = 128, 64 pages: 302 -> 57 us; 48 over 3, D = 256, 18 pages: 116 -> 40).
+// The CUDA-core kernel goes over a page once per `most` heads, so CTAs of that
+// many side by side read no more.
 int head_parts(int GS, int D, int bs, int ds, bool q4) {
-  if (q4 || ds != 2 || bs != 16 || (D != 64 && D != 128 && D != 256)) return 1;
-  const int most = D == 256 ? 8 : 16;
-  if (GS <= most) return 1;
-  for (int s = 2; s <= 8; ++s)
-    if (GS % s == 0 && GS / s <= most) return s;
-  return 1;
+  if (q4) return 1;
+  const int tma = !tma_shape(D, bs, ds) ? 0 : D == 256 ? 8 : 16;
+  const int most = D <= 64 ? 16 : D <= 128 ? 8 : 4;
+  int parts = 1;
+  for (int s = 1; s <= 8; ++s) {
+    if (GS % s) continue;
+    if (tma && GS / s <= tma) return s;
+    if (GS / parts > most) parts = s;
+  }
+  return parts;
 }
+
+// Shortest partition of the attention, in pages: 64 tokens.
+int min_pages(int bs) { return bs >= 64 ? 1 : 64 / bs; }
 
 // Workspace: scores and near pages of the selection, the kept pages' tables,
 // the attention's partials, each from a 256-byte boundary.
 struct Layout {
-  size_t keys, magnitude, near_page, near_key, tables, lens, part, total;
+  size_t keys, magnitude, near_page, near_key, order, tables, lens, part, total;
   size_t part_bytes;
   int parts;  // of a group's heads, see head_parts
 };
 
+// sub: the attention takes a page as this many of bs / sub tokens.
 Layout layout_of(long long rows, int GS, int D, int max_blocks, int bs, int ds, int keep, bool q4,
-                 bool attention, int sms) {
+                 bool attention, int sms, int sub) {
   Layout l{};
   l.parts = 1;
   size_t at = 0;
@@ -134,14 +149,15 @@ Layout layout_of(long long rows, int GS, int D, int max_blocks, int bs, int ds, 
   l.magnitude = take(scored ? (size_t)rows * ceil_div(max_blocks, xpa::kScoreTile) * sizeof(float) : 0);
   l.near_page = take(scored * sizeof(unsigned));
   l.near_key = take(scored * sizeof(unsigned long long));
+  l.order = take(sub > 1 ? (size_t)rows * keep * sizeof(int) : 0);
   if (attention) {
-    l.parts = head_parts(GS, D, bs, ds, q4);
+    l.parts = head_parts(GS, D, bs / sub, ds, q4);
     const long long n = rows * l.parts;
-    l.tables = take((size_t)n * keep * sizeof(int));
+    l.tables = take((size_t)n * keep * sub * sizeof(int));
     l.lens = take((size_t)n * sizeof(int));
     l.part_bytes = q4 ? nxt_paged_attention_q4_workspace_size((int)n, GS, D, 1, keep, bs)
-                      : make_plan((int)n, GS / l.parts, D, 1, keep, sms, ds,
-                                  XPA_SPARSE_ITEMS_PER_SM)
+                      : make_plan((int)n, GS / l.parts, D, 1, keep * sub, sms, ds,
+                                  XPA_SPARSE_ITEMS_PER_SM, min_pages(bs / sub))
                             .ws_bytes;
     l.part = take(l.part_bytes);
   }
@@ -176,10 +192,21 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
   const long long rows = (long long)c.B * c.Hkv;
   const int GS = c.Hq / c.Hkv;
   if (rows * ceil_div(c.max_blocks, xpa::kScoreTile) > INT_MAX || rows * GS > INT_MAX ||
-      rows * c.keep > INT_MAX / 8)
+      rows * c.keep * std::max(1, c.bs / 16) > INT_MAX / 8)
     return NXT_PA_EINVAL;
   const long long head_pages = c.Hkv > 1 ? c.kbs / c.khs : 1;
   const int64_t page_stride = c.Hkv > 1 ? c.khs : c.kbs;
+  // Longer pages go to the tensor-core kernel as pages of 16 tokens, where ids
+  // of those fit
+  int sub = 1;
+  long long sub_ids = 1;
+  const int64_t piece = 16LL * c.D;
+  if (attention && !c.q4 && c.bs > 16 && c.bs % 16 == 0 && tma_shape(c.D, 16, c.ds) &&
+      page_stride % piece == 0 && page_stride / piece >= c.bs / 16 && c.num_blocks > 0 &&
+      c.num_blocks <= INT_MAX / head_pages / (page_stride / piece)) {
+    sub = c.bs / 16;
+    sub_ids = page_stride / piece;
+  }
 
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return NXT_PA_ECUDA;
@@ -190,7 +217,7 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
   }
   const Layout l =
       layout_of(rows, GS, c.D, c.max_blocks, c.bs, c.ds, c.keep, c.q4, attention,
-                sm_count_of(dev));
+                sm_count_of(dev), sub);
   std::unique_lock<std::mutex> lk;
   if (ws) {
     if (ws_bytes < l.total) return NXT_PA_EWORKSPACE;
@@ -208,6 +235,9 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
   p.sel_tables = attention ? reinterpret_cast<int*>(base + l.tables) : sel_tables;
   p.sel_lens = attention ? reinterpret_cast<int*>(base + l.lens) : sel_lens;
   p.sel_pages = c.sel_pages;
+  p.order = sub > 1 ? reinterpret_cast<int*>(base + l.order) : nullptr;
+  p.sub = sub;
+  p.sub_ids = (int)sub_ids;
   p.keys = reinterpret_cast<unsigned*>(base + l.keys);
   p.magnitude = reinterpret_cast<float*>(base + l.magnitude);
   p.near_page = reinterpret_cast<unsigned*>(base + l.near_page);
@@ -244,9 +274,12 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
                                      GS, c.D, 1, c.scale, c.keep, c.bs, c.k_scale,
                                      c.v_scale, page_stride, c.khs, nb, part, l.part_bytes, status,
                                      st);
+  if (sub > 1) nb = c.num_blocks * head_pages * sub_ids;
   return attention_planned(c.out, c.q, c.k, c.v, p.sel_tables, p.sel_lens, (int)rows * l.parts,
-                           GS / l.parts, c.D, 1, c.scale, c.keep, c.bs, c.ds, page_stride, c.khs, nb,
-                           part, l.part_bytes, status, st, XPA_SPARSE_ITEMS_PER_SM);
+                           GS / l.parts, c.D, 1, c.scale, c.keep * sub, c.bs / sub, c.ds,
+                           sub > 1 ? piece : page_stride, sub > 1 ? piece : c.khs, nb, part,
+                           l.part_bytes, status, st, XPA_SPARSE_ITEMS_PER_SM,
+                           min_pages(c.bs / sub));
 }
 
 }  // namespace
@@ -335,18 +368,22 @@ size_t nxt_paged_attention_sparse_workspace_size(int num_seqs, int num_heads, in
       max_pages <= 0 || max_num_blocks_per_seq < 0)
     return 0;
   const long long rows = (long long)num_seqs * num_kv_heads;
-  if (rows > INT_MAX / 8) return 0;
+  if (rows > INT_MAX / 8 || max_pages > INT_MAX / block_size) return 0;
   const int GS = num_heads / num_kv_heads;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) dev = -1;
   const int sms = sm_count_of(dev);
-  const size_t plain = layout_of(rows, GS, head_size, max_num_blocks_per_seq, block_size,
-                                 dtype_size, max_pages, false, true, sms)
-                           .total;
-  const size_t q4 = layout_of(rows, GS, head_size, max_num_blocks_per_seq, block_size, dtype_size,
-                              max_pages, true, true, sms)
-                        .total;
-  return plain > q4 ? plain : q4;
+  // the largest of what a call may take: 4-bit pools, pages whole or in pieces
+  size_t most = 0;
+  auto add = [&](bool q4, int sub) {
+    most = std::max(most, layout_of(rows, GS, head_size, max_num_blocks_per_seq, block_size,
+                                    dtype_size, max_pages, q4, true, sms, sub)
+                              .total);
+  };
+  add(false, 1);
+  add(true, 1);
+  if (block_size % 16 == 0) add(false, block_size / 16);
+  return most;
 }
 
 }  // extern "C"
