@@ -791,8 +791,8 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p, 
   __syncthreads();
   int to = __reduce_add_sync(0xffffffffu, lane < warp ? s_count[lane] : 0);
   const int done = __reduce_add_sync(0xffffffffu, lane < NWARP ? s_count[lane] : 0);
-  int* tab = p.sel_tables + (long long)row * p.copies * p.keep * p.sub;
-  int* order = p.order ? p.order + (long long)row * p.keep : tab;
+  int* tab = p.sel_tables + (long long)row * p.copies * p.width * p.sub;
+  int* order = p.order ? p.order + (long long)row * p.width : tab;
   int* pages = p.sel_pages ? p.sel_pages + (long long)row * p.keep : nullptr;
 #pragma unroll 2
   for (int base = begin; base < stop; base += 32) {
@@ -812,13 +812,13 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p, 
     const int id = (int)(((long long)e * p.head_pages + h) * p.sub_ids);
     for (int c = 0; c < p.copies; ++c)
       for (int k = 0; k < p.sub; ++k)
-        tab[((long long)c * p.keep + i) * p.sub + k] = id + k;
+        tab[((long long)c * p.width + i) * p.sub + k] = id + k;
   }
-  for (int i = done + tid; i < p.keep; i += NT) {
+  for (int i = done + tid; i < p.width; i += NT)
     for (int c = 0; c < p.copies; ++c)
-      for (int k = 0; k < p.sub; ++k) tab[((long long)c * p.keep + i) * p.sub + k] = -1;
-    if (pages) pages[i] = -1;
-  }
+      for (int k = 0; k < p.sub; ++k) tab[((long long)c * p.width + i) * p.sub + k] = -1;
+  if (pages)
+    for (int i = done + tid; i < p.keep; i += NT) pages[i] = -1;
   tail = __syncthreads_or(tail);
   if (tid < p.copies)
     p.sel_lens[(long long)row * p.copies + tid] =

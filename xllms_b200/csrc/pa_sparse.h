@@ -37,11 +37,11 @@ struct SelectParams {
   const int* block_tables;
   const int* seq_lens;
   int* status;
-  int* sel_tables;  // [B * Hkv][copies][keep][sub] page * head_pages + kv head, see sub
+  int* sel_tables;  // [B * Hkv][copies][width][sub] page * head_pages + kv head, see sub
   int* sel_lens;    // [B * Hkv][copies] tokens kept
   int* sel_pages;   // [B * Hkv][keep] page index within the sequence, -1 past the last; or null
   // workspace
-  int* order;             // [B * Hkv][keep] kept pages' indices on the way; null: in sel_tables
+  int* order;             // [B * Hkv][width] kept pages' indices on the way; null: in sel_tables
   unsigned* keys;         // [B * Hkv][max_blocks] ordered scores, 0: page not eligible
   float* magnitude;       // [B * Hkv][tiles] per tile_pages pages, the largest sum of the
                           // magnitudes of a score's terms
@@ -51,6 +51,7 @@ struct SelectParams {
   long long head_pages;  // kv_block_stride / kv_head_stride
   int B, Hq, Hkv, D, GS, max_blocks, block_size;
   int keep, sink, recent;
+  int width;   // kept pages that a row's tables have room for
   int copies;  // of every row's tables, for attention that takes its heads in parts
   int sub;     // entries per kept page: page id * sub_ids + 0 .. sub - 1, for attention
   int sub_ids; // that takes a page in pieces of 16 tokens (sub > 1 needs order)

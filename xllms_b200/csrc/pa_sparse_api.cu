@@ -131,6 +131,7 @@ struct Layout {
   size_t keys, magnitude, near_page, near_key, order, tables, lens, part, total;
   size_t part_bytes;
   int parts;  // of a group's heads, see head_parts
+  int width;  // entries of a row's tables: no more than a sequence has pages
 };
 
 // sub: the attention takes a page as this many of bs / sub tokens.
@@ -138,6 +139,7 @@ Layout layout_of(long long rows, int GS, int D, int max_blocks, int bs, int ds, 
                  bool attention, int sms, int sub) {
   Layout l{};
   l.parts = 1;
+  l.width = attention ? std::max(1, std::min(keep, max_blocks)) : keep;
   size_t at = 0;
   auto take = [&at](size_t bytes) {
     const size_t here = at;
@@ -149,14 +151,14 @@ Layout layout_of(long long rows, int GS, int D, int max_blocks, int bs, int ds, 
   l.magnitude = take(scored ? (size_t)rows * ceil_div(max_blocks, xpa::kScoreTile) * sizeof(float) : 0);
   l.near_page = take(scored * sizeof(unsigned));
   l.near_key = take(scored * sizeof(unsigned long long));
-  l.order = take(sub > 1 ? (size_t)rows * keep * sizeof(int) : 0);
+  l.order = take(sub > 1 ? (size_t)rows * l.width * sizeof(int) : 0);
   if (attention) {
     l.parts = head_parts(GS, D, bs / sub, ds, q4);
     const long long n = rows * l.parts;
-    l.tables = take((size_t)n * keep * sub * sizeof(int));
+    l.tables = take((size_t)n * l.width * sub * sizeof(int));
     l.lens = take((size_t)n * sizeof(int));
-    l.part_bytes = q4 ? nxt_paged_attention_q4_workspace_size((int)n, GS, D, 1, keep, bs)
-                      : make_plan((int)n, GS / l.parts, D, 1, keep * sub, sms, ds,
+    l.part_bytes = q4 ? nxt_paged_attention_q4_workspace_size((int)n, GS, D, 1, l.width, bs)
+                      : make_plan((int)n, GS / l.parts, D, 1, l.width * sub, sms, ds,
                                   XPA_SPARSE_ITEMS_PER_SM, min_pages(bs / sub))
                             .ws_bytes;
     l.part = take(l.part_bytes);
@@ -236,6 +238,7 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
   p.sel_lens = attention ? reinterpret_cast<int*>(base + l.lens) : sel_lens;
   p.sel_pages = c.sel_pages;
   p.order = sub > 1 ? reinterpret_cast<int*>(base + l.order) : nullptr;
+  p.width = l.width;
   p.sub = sub;
   p.sub_ids = (int)sub_ids;
   p.keys = reinterpret_cast<unsigned*>(base + l.keys);
@@ -271,12 +274,12 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
   void* part = l.part_bytes ? base + l.part : nullptr;
   if (c.q4)
     return nxt_paged_attention_q4_ex(c.out, c.q, c.k, c.v, p.sel_tables, p.sel_lens, (int)rows,
-                                     GS, c.D, 1, c.scale, c.keep, c.bs, c.k_scale,
+                                     GS, c.D, 1, c.scale, l.width, c.bs, c.k_scale,
                                      c.v_scale, page_stride, c.khs, nb, part, l.part_bytes, status,
                                      st);
   if (sub > 1) nb = c.num_blocks * head_pages * sub_ids;
   return attention_planned(c.out, c.q, c.k, c.v, p.sel_tables, p.sel_lens, (int)rows * l.parts,
-                           GS / l.parts, c.D, 1, c.scale, c.keep * sub, c.bs / sub, c.ds,
+                           GS / l.parts, c.D, 1, c.scale, l.width * sub, c.bs / sub, c.ds,
                            sub > 1 ? piece : page_stride, sub > 1 ? piece : c.khs, nb, part,
                            l.part_bytes, status, st, XPA_SPARSE_ITEMS_PER_SM,
                            min_pages(c.bs / sub));
