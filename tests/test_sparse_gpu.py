@@ -490,3 +490,12 @@ def test_long_pages_of_padded_pools(cuda, hkv, pad):
         torch.cuda.current_stream().cuda_stream)
     assert rc == _native.NXT_PA_OK
     check_close(out, ref)
+
+
+def test_more_new_tokens_than_a_cache_can_hold(cuda):
+    _, k, _, table, lens = _case(90, [70, 5], 2, 2, 16, 1)
+    old = np.zeros((len(k), 2, 2, 16), np.float16)
+    got = PA.page_bounds(_t(k, cuda), _t(table, cuda), _t(lens, cuda), _t(old, cuda),
+                         num_new_tokens=2 ** 31 - 1)
+    np.testing.assert_array_equal(got.cpu().numpy(),
+                                  S.bounds(k, table, lens, 0, old, np.float16))

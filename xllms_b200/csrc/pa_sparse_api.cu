@@ -53,7 +53,8 @@ int bounds_call(void* bounds, const void* key_cache, const int* bt, const int* s
   p.num_new = num_new;
   // the last num_new tokens lie in at most this many pages
   p.pages_per_seq = max_blocks;
-  if (num_new > 0 && (num_new - 1) / bs + 2 < max_blocks) p.pages_per_seq = (num_new - 1) / bs + 2;
+  if (num_new > 0)
+    p.pages_per_seq = (int)std::min<long long>(max_blocks, (num_new - 1LL) / bs + 2);
   p.kind = kind;
   p.k_scale = k_scale;
   if (!q4) {
