@@ -566,23 +566,64 @@ __device__ __forceinline__ K bisect(BlockCount<NT>& s, int& turn, K lo, K hi, in
   return lo;
 }
 
+// The score of page e for KV head h of sequence b in 64 bits, over a warp (its
+// lanes all get it). K32: 32 K32 >= D; all loads of four heads before their use.
+template <typename T, int K32>
+__device__ __forceinline__ double score64(const SelectParams& p, int b, int h, int e, int lane) {
+  constexpr float top = sizeof(T) == 2 ? 65504.f : FLT_MAX;
+  const T* q = static_cast<const T*>(p.q) + ((long long)b * p.Hq + (long long)h * p.GS) * p.D;
+  const T* lo = static_cast<const T*>(p.bounds) + ((long long)e * p.Hkv + h) * 2 * p.D;
+  T l[K32], u[K32];
+#pragma unroll
+  for (int k = 0; k < K32; ++k) {
+    const int d = lane + 32 * k;
+    l[k] = d < p.D ? lo[d] : from_float<T>(0.f);
+    u[k] = d < p.D ? lo[p.D + d] : from_float<T>(0.f);
+  }
+  double best = -INFINITY;
+#pragma unroll 1
+  for (int x0 = 0; x0 < p.GS; x0 += 4) {  // four heads' sums side by side
+    T qx[K32][4];
+#pragma unroll
+    for (int k = 0; k < K32; ++k)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int d = lane + 32 * k;
+        qx[k][x] = d < p.D ? q[(long long)min(x0 + x, p.GS - 1) * p.D + d] : from_float<T>(0.f);
+      }
+    double s[4] = {};
+#pragma unroll
+    for (int k = 0; k < K32; ++k)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float qd = p.sign * tame(to_float<T>(qx[k][x]), top);
+        s[x] = fma((double)qd, (double)to_float<T>(qd > 0.f ? u[k] : l[k]), s[x]);
+      }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[x] += __shfl_xor_sync(0xffffffffu, s[x], o);
+    best = fmax(best, fmax(fmax(s[0], s[1]), fmax(s[2], s[3])));
+  }
+  return best;
+}
+
 // The row's keys stay in shared memory up to kSmemKeys pages (`smem_keys`),
 // longer rows are read again from the workspace.
 constexpr int kSmemKeys = 32768;
 
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p, int smem_keys) {
+__global__ void __launch_bounds__(NT, 512 / NT) pa_select_kernel(const SelectParams p, int smem_keys) {
   constexpr int NWARP = NT / 32;
   extern __shared__ unsigned s_keys[];
   __shared__ BlockCount<NT> s_cnt;
   __shared__ float s_red[NWARP];
-  __shared__ unsigned s_ends[2];
+  __shared__ unsigned s_low[NWARP], s_high[NWARP];
   __shared__ int s_near, s_bin;
   __shared__ unsigned s_near_page[kNearCap];
   __shared__ unsigned long long s_near_key[kNearCap];
-  __shared__ int s_count[NWARP];
-  __shared__ int s_bins[kBins];
-  constexpr float top = sizeof(T) == 2 ? 65504.f : FLT_MAX;
+  __shared__ int s_count[NWARP], s_total[NWARP];
+  __shared__ __align__(16) int s_bins[kBins];
   pdl_wait_primary();
   // No early trigger here: the merge behind the attention reads sel_lens
   // before it waits for anything, so nothing may start until they are written.
@@ -602,47 +643,51 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p, 
     int turn = 0;
     int mine = 0;
     unsigned kmin = 0xffffffffu, kmax = 0u;
-#pragma unroll 4
-    for (int at = tid; at < n; at += NT) {
-      const unsigned k = K[at];
-      if (n <= smem_keys) s_keys[at] = k;
-      if (k && at >= first && at < last) {
-        ++mine;
-        kmin = min(kmin, k);
-        kmax = max(kmax, k);
+    // the largest sum of magnitudes of the row
+    float most = 0.f;
+    const int tiles = (n + p.tile_pages - 1) / p.tile_pages;
+    for (int i = tid; i < tiles; i += NT)
+      most = fmaxf(most, p.magnitude[(long long)row * p.tiles + i]);
+#pragma unroll 1
+    for (int at0 = tid; at0 < n; at0 += 8 * NT) {
+      unsigned k[8];  // all eight on the way together, the row's end included
+#pragma unroll
+      for (int j = 0; j < 8; ++j) k[j] = at0 + j * NT < n ? K[at0 + j * NT] : 0u;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int at = at0 + j * NT;
+        if (at < n && n <= smem_keys) s_keys[at] = k[j];
+        if (k[j] && at >= first && at < last) {
+          ++mine;
+          kmin = min(kmin, k[j]);
+          kmax = max(kmax, k[j]);
+        }
       }
     }
     if (n <= smem_keys) K = s_keys;  // each thread goes on with the keys it copied
-    if (tid == 0) {
-      s_ends[0] = 0xffffffffu;
-      s_ends[1] = 0u;
-      s_near = 0;
-    }
+    if (tid == 0) s_near = 0;
     for (int i = tid; i < kBins; i += NT) s_bins[i] = 0;
-    const int eligible = block_sum<NT>(s_cnt, mine, turn);
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    kmin = __reduce_min_sync(0xffffffffu, kmin);
+    kmax = __reduce_max_sync(0xffffffffu, kmax);
+    most = warp_max(most);
+    if (lane == 0) {
+      s_count[warp] = mine;
+      s_low[warp] = kmin;
+      s_high[warp] = kmax;
+      s_red[warp] = most;
+    }
+    __syncthreads();
+    const int eligible = __reduce_add_sync(0xffffffffu, lane < NWARP ? s_count[lane] : 0);
     if (r <= 0) {
       take = 0xffffffffu;  // no competing page fits; no key is this large
     } else if (eligible > r) {
-      kmin = __reduce_min_sync(0xffffffffu, kmin);
-      kmax = __reduce_max_sync(0xffffffffu, kmax);
-      if (lane == 0) {
-        atomicMin(&s_ends[0], kmin);
-        atomicMax(&s_ends[1], kmax);
-      }
-      // the largest sum of magnitudes of the row
-      float most = 0.f;
-      const int tiles = (n + p.tile_pages - 1) / p.tile_pages;
-      for (int i = tid; i < tiles; i += NT)
-        most = fmaxf(most, p.magnitude[(long long)row * p.tiles + i]);
-      most = warp_max(most);
-      if (lane == 0) s_red[warp] = most;
-      __syncthreads();
+      kmin = __reduce_min_sync(0xffffffffu, lane < NWARP ? s_low[lane] : 0xffffffffu);
+      kmax = __reduce_max_sync(0xffffffffu, lane < NWARP ? s_high[lane] : 0u);
       most = warp_max(lane < NWARP ? s_red[lane] : 0.f);
       // histogram of the keys over [kmin, kmax], each bin 2^shift keys wide
-      kmin = s_ends[0];
-      kmax = s_ends[1];
       const int shift = max(0, 32 - __clz(kmax - kmin) - 11);
-#pragma unroll 2
+#pragma unroll 4
       for (int at = tid; at < last; at += NT) {
         const unsigned k = at >= first ? K[at] : 0u;
         if (k) atomicAdd(&s_bins[(k - kmin) >> shift], 1);
@@ -651,8 +696,11 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p, 
       // the bin of the r-th largest: a thread's bins, from the top, then the scan
       constexpr int BPT = kBins / NT;
       int in_bins = 0;
-#pragma unroll 1
-      for (int i = 0; i < BPT; ++i) in_bins += s_bins[kBins - 1 - (tid * BPT + i)];
+#pragma unroll
+      for (int i = 0; i < BPT / 4; ++i) {
+        const int4 v = reinterpret_cast<const int4*>(s_bins)[(kBins - (tid + 1) * BPT) / 4 + i];
+        in_bins += v.x + v.y + v.z + v.w;
+      }
       int upto = in_bins;  // keys in this warp's bins down to this thread's
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -684,7 +732,7 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p, 
       // in shared memory too
       unsigned* far_page = p.near_page + (long long)row * p.max_blocks;
       int above = 0;
-#pragma unroll 2
+#pragma unroll 4
       for (int at = tid; at < last; at += NT) {
         const unsigned k = at >= first ? K[at] : 0u;
         above += k > near_hi;
@@ -701,43 +749,11 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p, 
         const bool few = near <= kNearCap;
         const unsigned* lp = few ? s_near_page : far_page;
         unsigned long long* lk = few ? s_near_key : p.near_key + (long long)row * p.max_blocks;
-        const T* q =
-            static_cast<const T*>(p.q) + ((long long)b * p.Hq + (long long)h * p.GS) * p.D;
 #pragma unroll 1
         for (int i = warp; i < near; i += NWARP) {
           const int e = __ldg(p.block_tables + (long long)b * p.max_blocks + lp[i]);
-          const T* lo = static_cast<const T*>(p.bounds) + ((long long)e * p.Hkv + h) * 2 * p.D;
-          T l[8], u[8];  // D <= 256
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int d = lane + 32 * k;
-            l[k] = d < p.D ? lo[d] : from_float<T>(0.f);
-            u[k] = d < p.D ? lo[p.D + d] : from_float<T>(0.f);
-          }
-          double best = -INFINITY;
-#pragma unroll 1
-          for (int x0 = 0; x0 < p.GS; x0 += 4) {  // four heads' sums side by side
-            double s[4] = {};
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const int d = lane + 32 * k;
-              T qx[4];  // all four loads before their use
-#pragma unroll
-              for (int x = 0; x < 4; ++x)
-                qx[x] = d < p.D ? q[(long long)min(x0 + x, p.GS - 1) * p.D + d]
-                                : from_float<T>(0.f);
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                const float qd = p.sign * tame(to_float<T>(qx[x]), top);
-                s[x] = fma((double)qd, (double)to_float<T>(qd > 0.f ? u[k] : l[k]), s[x]);
-              }
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-              for (int x = 0; x < 4; ++x) s[x] += __shfl_xor_sync(0xffffffffu, s[x], o);
-            best = fmax(best, fmax(fmax(s[0], s[1]), fmax(s[2], s[3])));
-          }
+          const double best = p.D <= 128 ? score64<T, 4>(p, b, h, e, lane)
+                                         : score64<T, 8>(p, b, h, e, lane);
           if (lane == 0) lk[i] = key_of(best);
         }
         __syncthreads();
@@ -783,23 +799,43 @@ __global__ void __launch_bounds__(NT, 1) pa_select_kernel(const SelectParams p, 
     const unsigned k = K[at];
     return at < first || at >= last ? k != 0u : k >= take;
   };
+  // lane l: which of the pages at + 32 l .. + 31 are kept
+  auto mask_at = [&](int at) {
+    unsigned own = 0u;
+    const int words = min(32, (stop - at + 31) >> 5);
+#pragma unroll 4
+    for (int j = 0; j < words; ++j) {
+      const unsigned m = __ballot_sync(0xffffffffu, kept(at + 32 * j + lane));
+      if (lane == j) own = m;
+    }
+    return own;
+  };
+  unsigned own = 0u;
   int count = 0;
-#pragma unroll 2
-  for (int at = begin; at < stop; at += 32)
-    count += __popc(__ballot_sync(0xffffffffu, kept(at + lane)));
-  if (lane == 0) s_count[warp] = count;
+#pragma unroll 1
+  for (int at = begin; at < stop; at += 1024) {
+    own = mask_at(at);
+    count += __reduce_add_sync(0xffffffffu, __popc(own));
+  }
+  if (lane == 0) s_total[warp] = count;
   __syncthreads();
-  int to = __reduce_add_sync(0xffffffffu, lane < warp ? s_count[lane] : 0);
-  const int done = __reduce_add_sync(0xffffffffu, lane < NWARP ? s_count[lane] : 0);
+  int to = __reduce_add_sync(0xffffffffu, lane < warp ? s_total[lane] : 0);
+  const int done = __reduce_add_sync(0xffffffffu, lane < NWARP ? s_total[lane] : 0);
   int* tab = p.sel_tables + (long long)row * p.copies * p.width * p.sub;
   int* order = p.order ? p.order + (long long)row * p.width : tab;
   int* pages = p.sel_pages ? p.sel_pages + (long long)row * p.keep : nullptr;
-#pragma unroll 2
-  for (int base = begin; base < stop; base += 32) {
-    const bool in = kept(base + lane);
-    const unsigned m = __ballot_sync(0xffffffffu, in);
-    if (in) order[to + __popc(m & ((1u << lane) - 1u))] = base + lane;
-    to += __popc(m);
+#pragma unroll 1
+  for (int at = begin; at < stop; at += 1024) {
+    unsigned m = run <= 1024 ? own : mask_at(at);
+    int upto = __popc(m);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    int mine = to + upto - __popc(m);
+    to += __shfl_sync(0xffffffffu, upto, 31);
+    for (; m; m &= m - 1u) order[mine++] = at + 32 * lane + __ffs(m) - 1;
   }
   __syncthreads();
   // page indices -> per-head page ids, all table reads at once
