@@ -82,12 +82,19 @@ int rows_call(bool write, void* key, void* value, void* kc, void* vc, const int6
 // XPA_Q4_ITEMS_PER_SM items per SM, but not below 8, nor below sqrt(tiles / 2):
 // with few rows, a shorter partition saves its own time and costs as much in
 // the merge of the longer list of partials (2 rows of 3254 tiles, D = 256: 8
-// tiles 47 us, 64 tiles 23).
+// tiles 47 us, 64 tiles 23). Finer steps (3/4, 2/3) gain where lengths differ
+// and lose as much where they do not (16 sequences, 8 KV heads: 4-8K tokens 38
+// -> 32 us, 8K each 39 -> 45). Rows that one partition holds whole need no merge
+// and stay whole from XPA_Q4_WHOLE_PER_SM of them per SM on (512 rows of 64
+// tiles, with their selection: whole 53 us, in two 57).
 #ifndef XPA_Q4_PART_TILES
 #define XPA_Q4_PART_TILES 128
 #endif
 #ifndef XPA_Q4_ITEMS_PER_SM
 #define XPA_Q4_ITEMS_PER_SM 4
+#endif
+#ifndef XPA_Q4_WHOLE_PER_SM
+#define XPA_Q4_WHOLE_PER_SM 3
 #endif
 #ifndef XPA_Q4_MIN_TILES
 #define XPA_Q4_MIN_TILES 8
@@ -97,7 +104,9 @@ Plan q4_plan(int B, int Hq, int D, int Hkv, int max_blocks, int bs, int nsm) {
   const long long tiles = std::max(1LL, (long long)max_blocks * spp);
   const long long rows = (long long)B * Hkv, want = (long long)XPA_Q4_ITEMS_PER_SM * nsm;
   long long pt = XPA_Q4_PART_TILES;
-  while (pt > XPA_Q4_MIN_TILES && pt * pt > tiles && rows * ceil_div(tiles, pt) < want) pt >>= 1;
+  if (tiles > pt || rows < (long long)XPA_Q4_WHOLE_PER_SM * nsm)
+    while (pt > XPA_Q4_MIN_TILES && pt * pt > tiles && rows * ceil_div(tiles, pt) < want)
+      pt >>= 1;
   while (ceil_div(tiles, pt) > 8192) pt <<= 1;
   Plan pl;
   pl.part_pages = (int)std::max(1LL, pt / spp);
