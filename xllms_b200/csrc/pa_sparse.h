@@ -64,8 +64,16 @@ struct SelectParams {
 // Pages of one magnitude entry and of one score CTA. The tensor-core kernel
 // takes tiles of 16, 128 pages a CTA (8 sequences of 32-128K tokens: 64 pages
 // 80 us with the selection, 128 74, 32 91), fewer while that leaves the GPU
-// without three CTAs per SM; the scalar one, whose warps take a page at a time, 32.
-constexpr int kScoreTile = 16, kScoreChunkScalar = 32, kScoreWarps = 4;
+// without three CTAs per SM; the scalar one, whose warps take a page at a time,
+// 32 to 4 in the same way (whole sparse call, 60 rows of up to
+// 49 pages: 24 us with 32, 20 with 4).
+constexpr int kScoreTile = 16, kScoreChunkScalar = 32, kScoreChunkLeast = 4, kScoreWarps = 4;
+inline int score_chunk_scalar(long long rows, int max_blocks, int sms) {
+  int chunk = kScoreChunkScalar;
+  while (chunk > kScoreChunkLeast && rows * ((max_blocks + chunk - 1) / chunk) < 3LL * sms)
+    chunk >>= 1;
+  return chunk;
+}
 inline int score_chunk(int B, int Hkv, int max_blocks, int sms) {
   const long long cols = (long long)B * ((Hkv + kScoreWarps - 1) / kScoreWarps);
   int chunk = 128;

@@ -149,7 +149,7 @@ Layout layout_of(long long rows, int GS, int D, int max_blocks, int bs, int ds, 
   };
   const size_t scored = max_blocks > keep ? (size_t)rows * max_blocks : 0;
   l.keys = take(scored * sizeof(unsigned));
-  l.magnitude = take(scored ? (size_t)rows * ceil_div(max_blocks, xpa::kScoreTile) * sizeof(float) : 0);
+  l.magnitude = take(scored ? (size_t)rows * ceil_div(max_blocks, xpa::kScoreChunkLeast) * sizeof(float) : 0);
   l.near_page = take(scored * sizeof(unsigned));
   l.near_key = take(scored * sizeof(unsigned long long));
   l.order = take(sub > 1 ? (size_t)rows * l.width * sizeof(int) : 0);
@@ -262,8 +262,8 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
   p.sign = c.scale > 0.f ? 1.f : c.scale < 0.f ? -1.f : 0.f;
   p.vec = c.ds == 2 && c.D % 8 == 0 && aligned(c.q, 16) && aligned(c.bounds, 16);
   p.chunk_pages = p.vec ? xpa::score_chunk(c.B, c.Hkv, c.max_blocks, sm_count_of(dev))
-                        : xpa::kScoreChunkScalar;
-  p.tile_pages = p.vec ? xpa::kScoreTile : xpa::kScoreChunkScalar;
+                        : xpa::score_chunk_scalar(rows, c.max_blocks, sm_count_of(dev));
+  p.tile_pages = p.vec ? xpa::kScoreTile : p.chunk_pages;
   p.chunks = ceil_div(c.max_blocks, p.chunk_pages);
   p.tiles = ceil_div(c.max_blocks, p.tile_pages);
   const cudaError_t e = xpa::launch_select(p, c.ds, st);
