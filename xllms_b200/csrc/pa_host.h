@@ -52,6 +52,9 @@ struct Plan {
 Plan make_plan(int B, int Hq, int D, int Hkv, int max_blocks, int nsm, int kv_es = 2,
                int min_items = 0, int min_pages = 4);
 
+// Plan of the kernels that take an item in 16-token tiles (4-bit, fp16 pages).
+Plan tile_plan(int B, int Hq, int D, int Hkv, int max_blocks, int bs, int nsm);
+
 // nxt_paged_attention_ex with these floors; `ws` holds at least
 // make_plan(...).ws_bytes of the same floors.
 int attention_planned(void* out, const void* q, const void* k, const void* v, const int* bt,

@@ -506,30 +506,6 @@ struct Q4Units {
   int head_chunks;  // CTAs per group of query heads
 };
 
-constexpr int kGridY = 32768;
-
-// Partition blockIdx.x of row (sequence, KV head).
-__device__ __forceinline__ ItemKind q4_item(const Params& p, int row, Item& it) {
-  it.part = blockIdx.x;
-  it.b = row / p.Hkv;
-  it.kvh = row - it.b * p.Hkv;
-  int L = __ldg(p.seq_lens + it.b);
-  const long long cap = (long long)p.max_blocks * p.block_size;
-  if (L < 0 || L > cap) {
-    if (it.part == 0 && it.kvh == 0 && threadIdx.x == 0) raise_status(p, kDevSeqClamped);
-    L = L < 0 ? 0 : (int)cap;
-  }
-  it.L = L;
-  it.slot0 = 0;
-  const long long part_tokens = (long long)p.part_pages * p.block_size;
-  it.direct = L <= part_tokens;
-  if (L == 0) return it.part == 0 ? kItemZero : kItemNone;
-  if (it.part * part_tokens >= L) return kItemNone;
-  it.page_begin = it.part * p.part_pages;
-  it.page_end = it.page_begin + p.part_pages;
-  return kItemWork;
-}
-
 template <int D, int NT, int NW, int STAGES, int U, int MINB>
 __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, const Q4Units q) {
   using C = Q4Cfg<D, NT, NW, STAGES, U>;
@@ -544,7 +520,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, co
   const int col = blockIdx.y + blockIdx.z * kGridY;
   if (col >= p.B * p.Hkv * q.head_chunks) return;
   const int row = q.head_chunks == 1 ? col : col / q.head_chunks;
-  const ItemKind kind = q4_item(p, row, it);
+  const ItemKind kind = part_item(p, row, it);
   if (kind == kItemNone) return;
   const int h0 = (col - row * q.head_chunks) * C::kHeads;
   const int nh = min(p.GS - h0, C::kHeads);
@@ -850,51 +826,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, co
       }
     }
   __syncthreads();
-  const int nc = D / 8;
-  for (int idx = threadIdx.x; idx < nh * nc; idx += NW * 32) {
-    const int head = idx / nc, d0 = (idx - head * nc) * 8;
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) M = fmaxf(M, sml[(w * C::kHeads + head) * 2]);
-    float num[8] = {}, den = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float mw = sml[(w * C::kHeads + head) * 2];
-      // a warp without a score above -inf holds zeros, or NaN to pass on
-      const float wt = mw == M ? 1.f : ex2(mw - M);
-      den = fmaf(wt, sml[(w * C::kHeads + head) * 2 + 1], den);
-      const float4* src =
-          reinterpret_cast<const float4*>(so + (size_t)(w * C::kHeads + head) * C::kRow + d0);
-      const float4 a = src[0], b = src[1];
-      num[0] = fmaf(wt, a.x, num[0]);
-      num[1] = fmaf(wt, a.y, num[1]);
-      num[2] = fmaf(wt, a.z, num[2]);
-      num[3] = fmaf(wt, a.w, num[3]);
-      num[4] = fmaf(wt, b.x, num[4]);
-      num[5] = fmaf(wt, b.y, num[5]);
-      num[6] = fmaf(wt, b.z, num[6]);
-      num[7] = fmaf(wt, b.w, num[7]);
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) num[k] *= p.v_scale;
-    if (it.direct) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) num[k] = den == 0.f ? 0.f : num[k] / den;
-      if (p.vec8) {
-        store_out8<__half>(p, row0 + head, d0, num);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) store_out<__half>(p, row0 + head, d0 + k, num[k]);
-      }
-    } else {
-      const long long pr = (row0 + head) * p.slots + it.slot0 + it.part;
-      // D is a multiple of 16: the partials' rows start on 16-byte boundaries
-      float4* dst = reinterpret_cast<float4*>(p.part_o + pr * D + d0);
-      dst[0] = make_float4(num[0], num[1], num[2], num[3]);
-      dst[1] = make_float4(num[4], num[5], num[6], num[7]);
-      if (d0 == 0) reinterpret_cast<float2*>(p.part_ml)[pr] = make_float2(M, den);
-    }
-  }
+  merge_warps<NW, C::kHeads, C::kRow>(p, it, so, sml, row0, nh, D);
 }
 
 // ── launchers ─────────────────────────────────────────────────────────────

@@ -13,6 +13,50 @@
 
 using namespace xpa::host;
 
+namespace xpa {
+namespace host {
+
+// Partitions of a call, in 16-token tiles rounded to whole pages: at
+// most XPA_Q4_PART_TILES, halved while the grid would hold fewer than
+// XPA_Q4_ITEMS_PER_SM items per SM, but not below 8, nor below sqrt(tiles / 2):
+// with few rows, a shorter partition saves its own time and costs as much in
+// the merge of the longer list of partials (2 rows of 3254 tiles, D = 256: 8
+// tiles 47 us, 64 tiles 23). Finer steps (3/4, 2/3) gain where lengths differ
+// and lose as much where they do not (16 sequences, 8 KV heads: 4-8K tokens 38
+// -> 32 us, 8K each 39 -> 45). Rows that one partition holds whole need no merge
+// and stay whole from XPA_Q4_WHOLE_PER_SM of them per SM on (512 rows of 64
+// tiles, with their selection: whole 53 us, in two 57).
+#ifndef XPA_Q4_PART_TILES
+#define XPA_Q4_PART_TILES 128
+#endif
+#ifndef XPA_Q4_ITEMS_PER_SM
+#define XPA_Q4_ITEMS_PER_SM 4
+#endif
+#ifndef XPA_Q4_WHOLE_PER_SM
+#define XPA_Q4_WHOLE_PER_SM 3
+#endif
+#ifndef XPA_Q4_MIN_TILES
+#define XPA_Q4_MIN_TILES 8
+#endif
+Plan tile_plan(int B, int Hq, int D, int Hkv, int max_blocks, int bs, int nsm) {
+  const int spp = bs / 16;
+  const long long tiles = std::max(1LL, (long long)max_blocks * spp);
+  const long long rows = (long long)B * Hkv, want = (long long)XPA_Q4_ITEMS_PER_SM * nsm;
+  long long pt = XPA_Q4_PART_TILES;
+  if (tiles > pt || rows < (long long)XPA_Q4_WHOLE_PER_SM * nsm)
+    while (pt > XPA_Q4_MIN_TILES && pt * pt > tiles && rows * ceil_div(tiles, pt) < want)
+      pt >>= 1;
+  while (ceil_div(tiles, pt) > 8192) pt <<= 1;
+  Plan pl;
+  pl.part_pages = (int)std::max(1LL, pt / spp);
+  pl.max_parts = ceil_div(max_blocks > 0 ? max_blocks : 1, pl.part_pages);
+  pl.ws_bytes = pl.max_parts > 1 ? partial_bytes((long long)B * Hq * pl.max_parts, D) : 0;
+  return pl;
+}
+
+}  // namespace host
+}  // namespace xpa
+
 namespace {
 
 int map_cuda(cudaError_t e) { return e == cudaSuccess ? NXT_PA_OK : NXT_PA_ECUDA; }
@@ -77,44 +121,6 @@ int rows_call(bool write, void* key, void* value, void* kc, void* vc, const int6
   return map_cuda(write ? xpa::launch_q4_write(a, st) : xpa::launch_q4_read(a, st));
 }
 
-// Partitions of a 4-bit call, in 16-token tiles rounded to whole pages: at
-// most XPA_Q4_PART_TILES, halved while the grid would hold fewer than
-// XPA_Q4_ITEMS_PER_SM items per SM, but not below 8, nor below sqrt(tiles / 2):
-// with few rows, a shorter partition saves its own time and costs as much in
-// the merge of the longer list of partials (2 rows of 3254 tiles, D = 256: 8
-// tiles 47 us, 64 tiles 23). Finer steps (3/4, 2/3) gain where lengths differ
-// and lose as much where they do not (16 sequences, 8 KV heads: 4-8K tokens 38
-// -> 32 us, 8K each 39 -> 45). Rows that one partition holds whole need no merge
-// and stay whole from XPA_Q4_WHOLE_PER_SM of them per SM on (512 rows of 64
-// tiles, with their selection: whole 53 us, in two 57).
-#ifndef XPA_Q4_PART_TILES
-#define XPA_Q4_PART_TILES 128
-#endif
-#ifndef XPA_Q4_ITEMS_PER_SM
-#define XPA_Q4_ITEMS_PER_SM 4
-#endif
-#ifndef XPA_Q4_WHOLE_PER_SM
-#define XPA_Q4_WHOLE_PER_SM 3
-#endif
-#ifndef XPA_Q4_MIN_TILES
-#define XPA_Q4_MIN_TILES 8
-#endif
-Plan q4_plan(int B, int Hq, int D, int Hkv, int max_blocks, int bs, int nsm) {
-  const int spp = bs / 16;
-  const long long tiles = std::max(1LL, (long long)max_blocks * spp);
-  const long long rows = (long long)B * Hkv, want = (long long)XPA_Q4_ITEMS_PER_SM * nsm;
-  long long pt = XPA_Q4_PART_TILES;
-  if (tiles > pt || rows < (long long)XPA_Q4_WHOLE_PER_SM * nsm)
-    while (pt > XPA_Q4_MIN_TILES && pt * pt > tiles && rows * ceil_div(tiles, pt) < want)
-      pt >>= 1;
-  while (ceil_div(tiles, pt) > 8192) pt <<= 1;
-  Plan pl;
-  pl.part_pages = (int)std::max(1LL, pt / spp);
-  pl.max_parts = ceil_div(max_blocks > 0 ? max_blocks : 1, pl.part_pages);
-  pl.ws_bytes = pl.max_parts > 1 ? partial_bytes((long long)B * Hq * pl.max_parts, D) : 0;
-  return pl;
-}
-
 int attention_call(void* out, const void* q, const void* k, const void* v, const int* bt,
                    const int* sl, int B, int Hq, int D, int Hkv, float scale, int max_blocks,
                    int bs, float ks, float vs, long long kbs, long long khs, long long num_blocks,
@@ -128,7 +134,7 @@ int attention_call(void* out, const void* q, const void* k, const void* v, const
   if (ws && !workspace_aligned(ws)) return NXT_PA_EINVAL;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return NXT_PA_ECUDA;
-  const Plan pl = q4_plan(B, Hq, D, Hkv, max_blocks, bs, sm_count_of(dev));
+  const Plan pl = tile_plan(B, Hq, D, Hkv, max_blocks, bs, sm_count_of(dev));
   // one CTA per partition and 8 query heads (16 of a larger group) at least
   if ((long long)B * Hkv * pl.max_parts > INT_MAX || (long long)B * Hq > INT_MAX)
     return NXT_PA_EINVAL;
@@ -237,7 +243,7 @@ size_t nxt_paged_attention_q4_workspace_size(int num_seqs, int num_heads, int he
     return 0;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) dev = -1;
-  return q4_plan(num_seqs, num_heads, head_size, num_kv_heads, max_num_blocks_per_seq, block_size,
+  return tile_plan(num_seqs, num_heads, head_size, num_kv_heads, max_num_blocks_per_seq, block_size,
                  sm_count_of(dev))
       .ws_bytes;
 }

@@ -83,4 +83,9 @@ inline int score_chunk(int B, int Hkv, int max_blocks, int sms) {
 
 cudaError_t launch_select(const SelectParams& p, int dtype_size, cudaStream_t st);
 
+// Decode attention over fp16 pages (pa_pages.cu): D and block_size multiples of
+// 16, rows on 16-byte boundaries, the query on 4-byte ones. Params as for the
+// other attention kernels; part_pages / max_parts / slots as tile_plan has them.
+cudaError_t launch_pages(const Params& p, cudaStream_t st);
+
 }  // namespace xpa

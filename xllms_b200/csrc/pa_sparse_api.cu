@@ -8,6 +8,7 @@
 
 #include "operator_api.h"
 #include "pa_host.h"
+#include "pa_launch.h"
 #include "pa_sparse.h"
 
 using namespace xpa::host;
@@ -103,6 +104,12 @@ bool tma_shape(int D, int bs, int ds) {
   return ds == 2 && bs == 16 && (D == 64 || D == 128 || D == 256);
 }
 
+// Heads of a group that the TMA kernel reads a page for.
+int tma_heads(int D) { return D == 256 ? 8 : 16; }
+
+// What attends to a row's kept pages.
+enum Path { kPathDecode, kPathPages, kPathQ4 };
+
 // Parts that a KV head's group of query heads is taken in. The tensor-core
 // decode kernel of fp16 pools reads a page for up to 16 heads (8 at head size
 // 256), and re-reading it from L2 for the next part costs less than the
@@ -110,9 +117,8 @@ bool tma_shape(int D, int bs, int ds) {
 // D = 128, 64 pages: 302 -> 57 us; 48 over 3, D = 256, 18 pages: 116 -> 40).
 // The CUDA-core kernel goes over a page once per `most` heads, so CTAs of that
 // many side by side read no more.
-int head_parts(int GS, int D, int bs, int ds, bool q4) {
-  if (q4) return 1;
-  const int tma = !tma_shape(D, bs, ds) ? 0 : D == 256 ? 8 : 16;
+int head_parts(int GS, int D, int bs, int ds) {
+  const int tma = tma_shape(D, bs, ds) ? tma_heads(D) : 0;
   const int most = D <= 64 ? 16 : D <= 128 ? 8 : 4;
   int parts = 1;
   for (int s = 1; s <= 8; ++s) {
@@ -121,6 +127,14 @@ int head_parts(int GS, int D, int bs, int ds, bool q4) {
     if (GS / parts > most) parts = s;
   }
   return parts;
+}
+
+// fp16 shapes of the pages kernel: those that the decode kernel, with a page in
+// `sub` pieces, takes to its CUDA-core form.
+bool pages_shape(int GS, int D, int bs, int ds, int sub) {
+  if (ds != 2 || D % 16 || bs % 16) return false;
+  return !(tma_shape(D, bs / sub, ds) &&
+           GS / head_parts(GS, D, bs / sub, ds) <= tma_heads(D));
 }
 
 // Shortest partition of the attention, in pages: 64 tokens.
@@ -136,8 +150,8 @@ struct Layout {
 };
 
 // sub: the attention takes a page as this many of bs / sub tokens.
-Layout layout_of(long long rows, int GS, int D, int max_blocks, int bs, int ds, int keep, bool q4,
-                 bool attention, int sms, int sub) {
+Layout layout_of(long long rows, int GS, int D, int max_blocks, int bs, int ds, int keep,
+                 Path path, bool attention, int sms, int sub) {
   Layout l{};
   l.parts = 1;
   l.width = attention ? std::max(1, std::min(keep, max_blocks)) : keep;
@@ -154,14 +168,15 @@ Layout layout_of(long long rows, int GS, int D, int max_blocks, int bs, int ds, 
   l.near_key = take(scored * sizeof(unsigned long long));
   l.order = take(sub > 1 ? (size_t)rows * l.width * sizeof(int) : 0);
   if (attention) {
-    l.parts = head_parts(GS, D, bs / sub, ds, q4);
+    if (path == kPathDecode) l.parts = head_parts(GS, D, bs / sub, ds);
     const long long n = rows * l.parts;
     l.tables = take((size_t)n * l.width * sub * sizeof(int));
     l.lens = take((size_t)n * sizeof(int));
-    l.part_bytes = q4 ? nxt_paged_attention_q4_workspace_size((int)n, GS, D, 1, l.width, bs)
-                      : make_plan((int)n, GS / l.parts, D, 1, l.width * sub, sms, ds,
-                                  XPA_SPARSE_ITEMS_PER_SM, min_pages(bs / sub))
-                            .ws_bytes;
+    l.part_bytes = path != kPathDecode
+                       ? tile_plan((int)n, GS, D, 1, l.width, bs, sms).ws_bytes
+                       : make_plan((int)n, GS / l.parts, D, 1, l.width * sub, sms, ds,
+                                   XPA_SPARSE_ITEMS_PER_SM, min_pages(bs / sub))
+                             .ws_bytes;
     l.part = take(l.part_bytes);
   }
   l.total = at;
@@ -210,6 +225,15 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
     sub = c.bs / 16;
     sub_ids = page_stride / piece;
   }
+  // What the TMA kernel's boxes and heads do not fit goes to the kernel of plain
+  // copies where rows start on 16-byte boundaries, else to the CUDA-core kernel.
+  Path path = c.q4 ? kPathQ4 : kPathDecode;
+  if (attention && !c.q4 && pages_shape(GS, c.D, c.bs, c.ds, sub) && aligned(c.k, 16) &&
+      aligned(c.v, 16) && page_stride % 8 == 0 && aligned(c.q, 4)) {
+    path = kPathPages;
+    sub = 1;
+    sub_ids = 1;
+  }
 
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return NXT_PA_ECUDA;
@@ -219,7 +243,7 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
     if (rc != NXT_PA_OK) return rc;
   }
   const Layout l =
-      layout_of(rows, GS, c.D, c.max_blocks, c.bs, c.ds, c.keep, c.q4, attention,
+      layout_of(rows, GS, c.D, c.max_blocks, c.bs, c.ds, c.keep, path, attention,
                 sm_count_of(dev), sub);
   std::unique_lock<std::mutex> lk;
   if (ws) {
@@ -278,6 +302,38 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
                                      GS, c.D, 1, c.scale, l.width, c.bs, c.k_scale,
                                      c.v_scale, page_stride, c.khs, nb, part, l.part_bytes, status,
                                      st);
+  if (path == kPathPages) {
+    const Plan pl = tile_plan((int)rows, GS, c.D, 1, l.width, c.bs, sm_count_of(dev));
+    xpa::Params a{};
+    a.out = c.out;
+    a.q = c.q;
+    a.k = c.k;
+    a.v = c.v;
+    a.block_tables = p.sel_tables;
+    a.seq_lens = p.sel_lens;
+    a.part_o = static_cast<float*>(part);
+    a.part_ml = part ? reinterpret_cast<float*>(
+                           static_cast<char*>(part) +
+                           part_ml_offset_bytes(rows * GS * pl.max_parts, c.D))
+                     : nullptr;
+    a.status = status;
+    a.kv_block_stride = page_stride;
+    a.num_blocks = nb;
+    a.B = (int)rows;
+    a.Hq = a.GS = GS;
+    a.Hkv = 1;
+    a.D = c.D;
+    a.max_blocks = l.width;
+    a.block_size = c.bs;
+    a.part_pages = pl.part_pages;
+    a.max_parts = a.slots = pl.max_parts;
+    a.scale_log2 = c.scale * 1.4426950408889634f;
+    a.v_scale = 1.f;
+    a.vec8 = aligned(c.out, 16) ? 1 : 0;
+    cudaError_t err = xpa::launch_pages(a, st);
+    if (err == cudaSuccess && pl.max_parts > 1) err = xpa::launch_reduce(a, 2, st);
+    return map_cuda(err);
+  }
   if (sub > 1) nb = c.num_blocks * head_pages * sub_ids;
   return attention_planned(c.out, c.q, c.k, c.v, p.sel_tables, p.sel_lens, (int)rows * l.parts,
                            GS / l.parts, c.D, 1, c.scale, l.width * sub, c.bs / sub, c.ds,
@@ -379,14 +435,16 @@ size_t nxt_paged_attention_sparse_workspace_size(int num_seqs, int num_heads, in
   const int sms = sm_count_of(dev);
   // the largest of what a call may take: 4-bit pools, pages whole or in pieces
   size_t most = 0;
-  auto add = [&](bool q4, int sub) {
+  auto add = [&](Path path, int sub) {
     most = std::max(most, layout_of(rows, GS, head_size, max_num_blocks_per_seq, block_size,
-                                    dtype_size, max_pages, q4, true, sms, sub)
+                                    dtype_size, max_pages, path, true, sms, sub)
                               .total);
   };
-  add(false, 1);
-  add(true, 1);
-  if (block_size % 16 == 0) add(false, block_size / 16);
+  add(kPathDecode, 1);
+  if (block_size % 16 == 0) {
+    add(kPathQ4, 1);  // and kPathPages
+    add(kPathDecode, block_size / 16);
+  }
   return most;
 }
 
