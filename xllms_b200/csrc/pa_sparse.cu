@@ -530,7 +530,9 @@ __global__ void __launch_bounds__(128) pa_score_kernel(const SelectParams p) {
 // 2^-14 of the sum of a score's terms' magnitudes, whose largest of the row the
 // score kernel has left.
 // A row is read once and the code runs through once: what counts is the latency
-// of its dozen barriers and of fetching the code, so loops stay loops.
+// of its barriers, of its few dependent reads and of fetching the code, so loops
+// stay loops and reads are issued together (6144 pages a row, 512 threads: 16.6
+// us; rows of 64-512 pages, 128 threads: 11.5 us).
 // ════════════════════════════════════════════════════════════════════════
 constexpr int kBins = 2048;
 constexpr int kNearCap = 1024;  // near pages that are ranked in shared memory

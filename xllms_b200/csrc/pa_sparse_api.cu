@@ -95,7 +95,8 @@ struct SparseCall {
 
 // Items per SM below which the attention over the kept pages splits its rows
 // further. A row holds few pages here, so the partials of a finer split cost
-// more than an idle SM (64 rows of 256 pages, whole sparse call: 3 90 us, 8 95).
+// more than an idle SM (64 rows of 256 pages, whole sparse call: 8 items took 5
+// us more than 3).
 #ifndef XPA_SPARSE_ITEMS_PER_SM
 #define XPA_SPARSE_ITEMS_PER_SM 3
 #endif
@@ -114,7 +115,7 @@ enum Path { kPathDecode, kPathPages, kPathQ4 };
 // decode kernel of fp16 pools reads a page for up to 16 heads (8 at head size
 // 256), and re-reading it from L2 for the next part costs less than the
 // CUDA-core kernel (whole sparse call, 8 sequences: 192 heads over 8 KV heads,
-// D = 128, 64 pages: 302 -> 57 us; 48 over 3, D = 256, 18 pages: 116 -> 40).
+// D = 128, 64 pages: 302 -> 53 us; 48 over 3, D = 256, 18 pages: 116 -> 39).
 // The CUDA-core kernel goes over a page once per `most` heads, so CTAs of that
 // many side by side read no more.
 int head_parts(int GS, int D, int bs, int ds) {
@@ -130,7 +131,9 @@ int head_parts(int GS, int D, int bs, int ds) {
 }
 
 // fp16 shapes of the pages kernel: those that the decode kernel, with a page in
-// `sub` pieces, takes to its CUDA-core form.
+// `sub` pieces, takes to its CUDA-core form. At the TMA kernel's shapes it is the
+// slower one from a few dozen pages a row on (64 rows of 256 pages, whole sparse
+// call: 98 against 85 us).
 bool pages_shape(int GS, int D, int bs, int ds, int sub) {
   if (ds != 2 || D % 16 || bs % 16) return false;
   return !(tma_shape(D, bs / sub, ds) &&
