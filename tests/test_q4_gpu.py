@@ -467,3 +467,21 @@ def test_more_blocks_than_the_pools_have_are_refused(cuda):
         assert (PA.paged_attention_q4(*args, KS, VS, num_blocks=few) == want).all()
     with pytest.raises(PA.PagedAttentionError):
         PA.paged_attention_q4(*args, KS, VS, num_blocks=nb + 1)
+
+
+def test_read_back_into_either_or_both_rows(cuda):
+    import torch
+    hkv, D, T = 2, 64, 21
+    rng = np.random.default_rng(76)
+    pool = _t(rng.integers(0, 0x70, PA.q4_pool_shape(3, hkv, 16, D)).astype(np.uint8), cuda)
+    slots = _t(_slots(rng, T, 3, 16), cuda)
+    want = PA.read_cache_q4(pool, pool, slots, KS, VS)
+    for given in (("key",), ("value",), ("key", "value")):
+        wide = torch.zeros(T, hkv * D + 8, dtype=torch.float16, device=cuda)
+        rows = {name: wide.clone()[:, :hkv * D].view(T, hkv, D) for name in given}
+        got = PA.read_cache_q4(pool, pool, slots, KS, VS, **rows)
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+        assert all(got["key value".split().index(n)] is r for n, r in rows.items())
+        assert got[0].stride() == got[1].stride()
+    with pytest.raises(PA.PagedAttentionError):
+        PA.read_cache_q4(pool, pool, slots, KS, VS, key=want[0], value=wide[:, 8:].view(T, hkv, D))

@@ -673,10 +673,13 @@ def read_cache_q4(key_cache, value_cache, slot_mapping, k_scale, v_scale, *, key
     st, leave = _launch_on(device, stream)
     try:
         if key is None:
-            key = torch.empty((T, hkv, d), dtype=torch.float16, device=key_cache.device)
-        if value is None:
+            if value is None:
+                value = key_cache.new_empty((T, hkv, d), dtype=torch.float16)
+            key = torch.empty_strided(value.shape, value.stride(), dtype=torch.float16,
+                                      device=value.device)
+        elif value is None:
             value = torch.empty_strided(key.shape, key.stride(), dtype=torch.float16,
-                                        device=key_cache.device)
+                                        device=key.device)
         ts = _row_stride(where, key, value, slot_mapping, hkv, d, device)
         if key.shape[0] != T:
             _refuse(where, "one row per slot")
