@@ -499,3 +499,30 @@ def test_more_new_tokens_than_a_cache_can_hold(cuda):
                          num_new_tokens=2 ** 31 - 1)
     np.testing.assert_array_equal(got.cpu().numpy(),
                                   S.bounds(k, table, lens, 0, old, np.float16))
+
+
+def test_host_workspaces_and_status_words_are_refused(cuda):
+    import torch
+    q, k, v, table, lens = _case(91, [300], 8, 2, 64, 16)
+    bnd = _bounds_of(k, table, lens, np.float16)
+    args = [_t(x, cuda) for x in (q, k, v, bnd, table, lens)]
+    pool = torch.zeros(PA.q4_pool_shape(len(k), 2, 16, 64), dtype=torch.uint8, device=cuda)
+    host = torch.zeros(1 << 20, dtype=torch.uint8)
+    word = torch.zeros(1, dtype=torch.int32)
+    for bad in (dict(workspace=host), dict(device_status=word),
+                dict(device_status=word.to(cuda).float())):
+        with pytest.raises(PA.PagedAttentionError):
+            PA.paged_attention_sparse(*args, 4, **bad)
+        with pytest.raises(PA.PagedAttentionError):
+            PA.paged_attention_q4(args[0], pool, pool, args[4], args[5], KS, VS, **bad)
+        if "device_status" not in bad:
+            continue
+        with pytest.raises(PA.PagedAttentionError):
+            PA.select_pages(args[0], args[1], *args[3:], 4, **bad)
+        with pytest.raises(PA.PagedAttentionError):
+            PA.page_bounds(args[1], args[4], args[5], args[3], **bad)
+        rows = torch.zeros(1, 2, 64, dtype=torch.float16, device=cuda)
+        slots = torch.zeros(1, dtype=torch.int64, device=cuda)
+        with pytest.raises(PA.PagedAttentionError):
+            PA.paged_attention_q4_append(args[0], pool, pool, args[4], args[5], rows, rows, slots,
+                                         KS, VS, **bad)

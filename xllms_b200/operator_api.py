@@ -720,8 +720,21 @@ def _check_q4_step(where, query, key_cache, value_cache, block_tables, seq_lens,
     return B, Hq, dims
 
 
-def _workspace(t):
-    return (None, 0) if t is None else (t.data_ptr(), t.numel() * t.element_size())
+def _workspace(where, t, device):
+    if t is None:
+        return None, 0
+    if not t.is_contiguous() or t.get_device() != device:
+        _refuse(where, "workspace must be contiguous, on the query's device")
+    return t.data_ptr(), t.numel() * t.element_size()
+
+
+def _status(where, t, device):
+    import torch
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.numel() < 1 or t.get_device() != device:
+        _refuse(where, "device_status must be an int32 tensor on the call's device")
+    return t.data_ptr()
 
 
 def paged_attention_q4(query, key_cache, value_cache, block_tables, seq_lens, k_scale, v_scale, *,
@@ -730,9 +743,10 @@ def paged_attention_q4(query, key_cache, value_cache, block_tables, seq_lens, k_
     """Decode attention over 4-bit pools (q4_pool_shape); query and output fp16
     [B, Hq, D], any number of query heads per KV head."""
     import torch
+    where = "paged_attention_q4"
     device = query.get_device()
     B, Hq, (nb, hkv, bs, d, page, head) = _check_q4_step(
-        "paged_attention_q4", query, key_cache, value_cache, block_tables, seq_lens, out, device)
+        where, query, key_cache, value_cache, block_tables, seq_lens, out, device)
     st, leave = _launch_on(device, stream)
     try:
         if out is None:
@@ -741,8 +755,8 @@ def paged_attention_q4(query, key_cache, value_cache, block_tables, seq_lens, k_
                      key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
                      seq_lens.data_ptr(), B, Hq, d, hkv, d ** -0.5 if scale is None else scale,
                      block_tables.shape[1], bs, k_scale, v_scale, page, head,
-                     _known_blocks("paged_attention_q4", num_blocks, nb), *_workspace(workspace),
-                     _opt_ptr(device_status), st)
+                     _known_blocks(where, num_blocks, nb), *_workspace(where, workspace, device),
+                     _status(where, device_status, device), st)
     finally:
         if leave is not None:
             leave.close()
@@ -779,7 +793,8 @@ def paged_attention_q4_append(query, key_cache, value_cache, block_tables, seq_l
                      seq_lens.data_ptr(), new_key.data_ptr(), new_value.data_ptr(),
                      slot_mapping.data_ptr(), B, Hq, d, hkv, d ** -0.5 if scale is None else scale,
                      block_tables.shape[1], bs, k_scale, v_scale, page, head,
-                     _known_blocks(where, num_blocks, nb), _opt_ptr(device_status), st)
+                     _known_blocks(where, num_blocks, nb), _status(where, device_status, device),
+                     st)
     finally:
         if leave is not None:
             leave.close()
@@ -836,7 +851,7 @@ def page_bounds(key_cache, block_tables, seq_lens, bounds, *, num_new_tokens=0, 
         _native_call(name, bounds.data_ptr(), key_cache.data_ptr(), block_tables.data_ptr(),
                      seq_lens.data_ptr(), B, hkv, d, block_tables.shape[1], bs, kind, page, head,
                      _known_blocks(where, num_blocks, nb), num_new_tokens,
-                     _opt_ptr(device_status), st)
+                     _status(where, device_status, device), st)
     finally:
         if leave is not None:
             leave.close()
@@ -879,7 +894,7 @@ def select_pages(query, key_cache, bounds, block_tables, seq_lens, max_pages, *,
                      seq_lens.data_ptr(), B, Hq, d, hkv, d ** -0.5 if scale is None else scale,
                      block_tables.shape[1], bs, query.element_size(), page, head,
                      _known_blocks("select_pages", num_blocks, nb), max_pages, sink_pages,
-                     recent_pages, None, 0, _opt_ptr(device_status), st)
+                     recent_pages, None, 0, _status("select_pages", device_status, device), st)
     finally:
         if leave is not None:
             leave.close()
@@ -920,7 +935,8 @@ def paged_attention_sparse(query, key_cache, value_cache, bounds, block_tables, 
                      seq_lens.data_ptr(), _opt_ptr(selected), B, Hq, d, hkv,
                      d ** -0.5 if scale is None else scale, block_tables.shape[1], bs, *kind, page,
                      head, _known_blocks(where, num_blocks, nb), max_pages, sink_pages,
-                     recent_pages, *_workspace(workspace), _opt_ptr(device_status), st)
+                     recent_pages, *_workspace(where, workspace, device),
+                     _status(where, device_status, device), st)
     finally:
         if leave is not None:
             leave.close()
