@@ -16,24 +16,25 @@ using namespace xpa::host;
 namespace xpa {
 namespace host {
 
-// Partitions of a call, in 16-token tiles rounded to whole pages: at
-// most XPA_Q4_PART_TILES, halved while the grid would hold fewer than
-// XPA_Q4_ITEMS_PER_SM items per SM, but not below 8, nor below sqrt(tiles / 2):
-// with few rows, a shorter partition saves its own time and costs as much in
-// the merge of the longer list of partials (2 rows of 3254 tiles, D = 256: 8
-// tiles 47 us, 64 tiles 23). Finer steps (3/4, 2/3) gain where lengths differ
-// and lose as much where they do not (16 sequences, 8 KV heads: 4-8K tokens 38
-// -> 32 us, 8K each 39 -> 45). Rows that one partition holds whole need no merge
-// and stay whole from XPA_Q4_WHOLE_PER_SM of them per SM on (512 rows of 64
-// tiles, with their selection: whole 53 us, in two 57).
+// Partitions of a call, in 16-token tiles rounded to whole pages: at most
+// XPA_Q4_PART_TILES, halved while the grid would hold fewer than
+// XPA_Q4_ITEMS_PER_SM items per SM (8 sequences of 2048 tokens, 8 KV heads: 3
+// 11.1 us, 4 13.9; 512 rows of 64 tiles with their selection 53 and 57), but not
+// below 8, nor below sqrt(tiles / 2): with few rows, a shorter partition saves
+// its own time and costs as much in the merge of the longer list of partials
+// (2 rows of 3254 tiles, D = 256: 8 tiles 47 us, 64 tiles 23). Rows of at most
+// XPA_Q4_WHOLE_TILES stay whole, without a merge (48 rows of 32 tiles 5.4 us,
+// in four parts 6.8; 8 rows 6.8 and 6.0). Finer steps (3/4, 2/3) gain where
+// lengths differ and lose as much where they do not (16 sequences, 8 KV heads:
+// 4-8K tokens 38 -> 32 us, 8K each 39 -> 45).
 #ifndef XPA_Q4_PART_TILES
 #define XPA_Q4_PART_TILES 128
 #endif
 #ifndef XPA_Q4_ITEMS_PER_SM
-#define XPA_Q4_ITEMS_PER_SM 4
+#define XPA_Q4_ITEMS_PER_SM 3
 #endif
-#ifndef XPA_Q4_WHOLE_PER_SM
-#define XPA_Q4_WHOLE_PER_SM 3
+#ifndef XPA_Q4_WHOLE_TILES
+#define XPA_Q4_WHOLE_TILES 32
 #endif
 #ifndef XPA_Q4_MIN_TILES
 #define XPA_Q4_MIN_TILES 8
@@ -43,7 +44,7 @@ Plan tile_plan(int B, int Hq, int D, int Hkv, int max_blocks, int bs, int nsm) {
   const long long tiles = std::max(1LL, (long long)max_blocks * spp);
   const long long rows = (long long)B * Hkv, want = (long long)XPA_Q4_ITEMS_PER_SM * nsm;
   long long pt = XPA_Q4_PART_TILES;
-  if (tiles > pt || rows < (long long)XPA_Q4_WHOLE_PER_SM * nsm)
+  if (tiles > XPA_Q4_WHOLE_TILES)
     while (pt > XPA_Q4_MIN_TILES && pt * pt > tiles && rows * ceil_div(tiles, pt) < want)
       pt >>= 1;
   while (ceil_div(tiles, pt) > 8192) pt <<= 1;
