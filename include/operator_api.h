@@ -479,7 +479,8 @@ int nxt_select_pages(
     nxt_stream_t stream);
 
 /* Selection and attention in one call. sel_pages as above (may be NULL);
- * workspace and device_status as for nxt_paged_attention_ex. */
+ * device_status as for nxt_paged_attention_ex, workspace (or NULL) as for
+ * nxt_paged_attention_q4_ex. */
 int nxt_paged_attention_sparse_ex(
     void *out, const void *query,
     const void *key_cache, const void *value_cache, const void *bounds,
