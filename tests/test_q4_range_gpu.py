@@ -1,0 +1,105 @@
+"""The 4-bit cache, and attention over fp16 pages, at the ends of their range
+and in narrow calls, against statements in 64 bits."""
+
+import numpy as np
+import pytest
+
+import _q4ref as R
+from xllms_b200 import operator_api as PA
+
+pytestmark = pytest.mark.gpu
+
+
+def _t(x, dev):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(x)).to(dev)
+
+
+def _paged(rng, lens, bs):
+    """(table, number of blocks): shuffled pages for these lengths."""
+    lens = np.asarray(lens)
+    pages = -(-lens // bs)
+    nb = int(pages.sum()) + 2
+    table = np.full((len(lens), max(1, int(pages.max()))), -1, np.int32)
+    table[np.arange(table.shape[1])[None] < pages[:, None]] = rng.permutation(nb)[:pages.sum()]
+    return table, nb
+
+
+def _rows_of(pool, table, n, h, bs):
+    """Rows [n, D] of one sequence and KV head from values [nb, Hkv, bs, D]."""
+    at = np.arange(n)
+    return pool[table[at // bs], h, at % bs]
+
+
+def _softmax_av(s, v, extra=0.0):
+    """(out, bound) of exact scores s [n] and values v [n, D]. The kernels hold a
+    weight as two fp16 terms: 2^-22 of it, and where the second is subnormal
+    half of 2^-24, 2^-32 of the largest weight, which is at least 2^7. Its
+    exponent is a difference of scores times a factor of three roundings, in
+    one fused step: 2^-22 of the difference, and the exponential's 2^-22.
+    Products and sums are fp32, a matrix step or a merge off by 2^-22 of the sum
+    of magnitudes, and the output is rounded to fp16 once."""
+    d = s - s.max()
+    p = np.exp(d)
+    p /= p.sum()
+    out = p @ v
+    ds = 2.0 ** -22 + 1.5 * 2.0 ** -22 * np.abs(d)
+    bound = (p * (np.expm1(2 * ds) + 2.0 ** -21 + (len(s) / 16 + 16) * 2.0 ** -22 + extra)) @ np.abs(v)
+    bound += 2.0 ** -32 * p.max() * np.abs(v).sum(0)
+    return out, bound + 2.0 ** -11 * np.abs(out) + 2.0 ** -25
+
+
+def _worst(out, ref, bound):
+    x = out.double().cpu().numpy()
+    assert np.isfinite(x).all()
+    worst = np.max(np.abs(x - ref) / bound)
+    assert worst <= 1.0, worst
+
+
+# ── 4-bit pools with chosen keys ──────────────────────────────────────────
+def _q4_pools(rng, k_codes, k_scale_byte):
+    """(pools, values) of these key codes, one scale byte for all, random values."""
+    nb, hkv, bs, D = k_codes.shape
+    kb = np.full((nb, hkv, bs, D // 16), k_scale_byte, np.uint8)
+    vc = rng.integers(0, 16, k_codes.shape).astype(np.uint8)
+    vb = rng.integers(40, 60, kb.shape).astype(np.uint8)
+    pools = R.pack(k_codes, kb, True), R.pack(vc, vb, False)
+    return pools, (R.values(k_codes, kb, 1.0), R.values(vc, vb, 0.5))
+
+
+def _q4_call(cuda, q, pools, table, lens, scale):
+    return PA.paged_attention_q4(_t(q, cuda), _t(pools[0], cuda), _t(pools[1], cuda),
+                                 _t(table, cuda), _t(np.asarray(lens, np.int32), cuda), 1.0, 0.5,
+                                 scale=scale)
+
+
+def _check_rows(out, q, k, v, table, lens, scale, bs, exact=True):
+    hkv = k.shape[1]
+    group = q.shape[1] // hkv
+    ref, bound = np.zeros(q.shape), np.zeros(q.shape)
+    for b, n in enumerate(lens):
+        for x in range(q.shape[1]):
+            kk, vv = (_rows_of(y, table[b], n, x // group, bs) for y in (k, v))
+            s = kk @ q[b, x].astype(np.float64) * scale
+            # equal keys have equal scores, whatever the sums round to
+            s = s if exact else np.zeros(n)
+            ref[b, x], bound[b, x] = _softmax_av(s, vv)
+    _worst(out, ref, bound)
+
+
+Q4_SHAPES = [(8, 2, 128, 16), (3, 1, 112, 16), (16, 1, 64, 32), (2, 1, 256, 16), (9, 1, 80, 16)]
+
+
+@pytest.mark.parametrize("hq,hkv,D,bs", Q4_SHAPES + [(20, 2, 128, 16), (10, 1, 240, 16)])
+def test_q4_weights_keep_22_bits(cuda, hq, hkv, D, bs):
+    """Whole-number queries and keys of half units, whose scores are exact: what
+    is off is the weights' and the sums' own rounding, and it stays within the
+    bound of two fp16 terms a weight."""
+    rng = np.random.default_rng(hq * D)
+    lens = [1, 17, 300, 2500]
+    table, nb = _paged(rng, lens, bs)
+    pools, (k, v) = _q4_pools(rng, rng.integers(0, 16, (nb, hkv, bs, D)).astype(np.uint8), 0x38)
+    q = rng.integers(-2, 3, (len(lens), hq, D)).astype(np.float16)
+    for scale in (1 / 16, 1 / 64):
+        out = _q4_call(cuda, q, pools, table, lens, scale)
+        _check_rows(out, q, k, v, table, lens, scale, bs)
