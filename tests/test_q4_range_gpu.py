@@ -1,5 +1,6 @@
 """The 4-bit cache, and attention over fp16 pages, at the ends of their range
 and in narrow calls, against statements in 64 bits."""
+import math
 
 import numpy as np
 import pytest
@@ -87,7 +88,106 @@ def _check_rows(out, q, k, v, table, lens, scale, bs, exact=True):
     _worst(out, ref, bound)
 
 
+HUGE = [65504.0, -65504.0, 30000.0]
 Q4_SHAPES = [(8, 2, 128, 16), (3, 1, 112, 16), (16, 1, 64, 32), (2, 1, 256, 16), (9, 1, 80, 16)]
+
+
+@pytest.mark.parametrize("value", HUGE)
+@pytest.mark.parametrize("hq,hkv,D,bs", Q4_SHAPES)
+def test_q4_equal_keys_weigh_the_same_at_any_score(cuda, hq, hkv, D, bs, value):
+    """The largest queries against the largest keys: one token's weight is 1,
+    many tokens of one key get equal weights."""
+    rng = np.random.default_rng(D)
+    lens = [1, 40, 700, 5000]
+    table, nb = _paged(rng, lens, bs)
+    codes = np.broadcast_to(rng.integers(0, 16, (1, hkv, 1, D)), (nb, hkv, bs, D)).astype(np.uint8)
+    for scale_byte in (0x7e, 0x38):  # 448 and 1
+        pools, (k, v) = _q4_pools(rng, codes, scale_byte)
+        q = np.full((len(lens), hq, D), value, np.float16)
+        q[:, ::2, ::3] *= np.float16(0.5)
+        for scale in (1 / math.sqrt(D), -3.0):
+            out = _q4_call(cuda, q, pools, table, lens, scale)
+            _check_rows(out, q, k, v, table, lens, scale, bs, exact=False)
+
+
+def _rising(rng, n, steps):
+    """Offsets of n tokens: some runs of rising ones, then any."""
+    d = rng.integers(0, len(steps), n)
+    d[:n // 2] = np.sort(d[:n // 2])
+    return d
+
+
+@pytest.mark.parametrize("scale", [1.0, -1.0, 0.25])
+@pytest.mark.parametrize("D", [64, 128, 112, 256])
+def test_q4_differences_of_large_scores(cuda, D, scale):
+    """Scores of 12.6 million whose differences of a few units decide the
+    weights; every sum is a whole number below 2^24, so fp32 holds it exactly."""
+    rng = np.random.default_rng(D)
+    hq, hkv, bs, lens = 2, 1, 16, [3, 64, 700, 5000]
+    table, nb = _paged(rng, lens, bs)
+    codes = np.zeros((nb, hkv, bs, D), np.uint8)
+    codes[..., 0] = 7  # 6 * 64 * 32768
+    for b, n in enumerate(lens):
+        at = np.arange(n)
+        codes[table[b, at // bs], 0, at % bs, 1] = _rising(rng, n, R.LEVELS)
+    pools, (k, v) = _q4_pools(rng, codes, 0x68)  # 64
+    q = np.zeros((len(lens), hq, D), np.float16)
+    q[:, :, 0] = 32768 * np.sign(scale)
+    q[:, 0, 1] = 1 / 32  # 32 code units / 32: whole numbers
+    q[:, 1, 1] = -1 / 32
+    out = _q4_call(cuda, q, pools, table, lens, scale)
+    _check_rows(out, q, k, v, table, lens, scale, bs)
+
+
+def _pages_case(rng, lens, hkv, D, bs):
+    table, nb = _paged(rng, lens, bs)
+    return table, nb, rng.standard_normal((nb, hkv, bs, D)).astype(np.float16)
+
+
+def _keep_all(cuda, q, k, v, table, lens, scale, **kw):
+    """Sparse attention that keeps every page (bounds are not read)."""
+    bnd = np.zeros((len(k), k.shape[1], 2, k.shape[3]), np.float16)
+    return PA.paged_attention_sparse(*(_t(x, cuda) for x in (q, k, v, bnd, table)),
+                                     _t(np.asarray(lens, np.int32), cuda), table.shape[1],
+                                     scale=scale, **kw)
+
+
+# shapes of the kernel of plain page copies: its head sizes, a group of 13
+PAGE_SHAPES = [(20, 5, 112, 16), (3, 1, 80, 32), (13, 1, 256, 16), (2, 2, 208, 48)]
+
+
+@pytest.mark.parametrize("value", HUGE)
+@pytest.mark.parametrize("hq,hkv,D,bs", PAGE_SHAPES)
+def test_pages_equal_keys_weigh_the_same_at_any_score(cuda, hq, hkv, D, bs, value):
+    rng = np.random.default_rng(D)
+    lens = [1, 40, 900, 3000]
+    table, nb, v = _pages_case(rng, lens, hkv, D, bs)
+    k = np.broadcast_to(rng.choice([65504.0, 30000.0, -9.5], (1, hkv, 1, D)), v.shape).astype(np.float16)
+    q = np.full((len(lens), hq, D), value, np.float16)
+    q[:, ::2, ::3] *= np.float16(0.5)
+    for scale in (1 / math.sqrt(D), -3.0):
+        out = _keep_all(cuda, q, k, v, table, lens, scale)
+        _check_rows(out, q, k.astype(np.float64), v.astype(np.float64), table, lens, scale, bs,
+                    exact=False)
+
+
+@pytest.mark.parametrize("scale", [1.0, -1.0, 0.25])
+@pytest.mark.parametrize("hq,hkv,D,bs", PAGE_SHAPES)
+def test_pages_differences_of_large_scores(cuda, hq, hkv, D, bs, scale):
+    """As for 4-bit pools: scores of 2^23 and whole differences."""
+    rng = np.random.default_rng(D)
+    lens = [3, 64, 900, 3000]
+    table, nb, v = _pages_case(rng, lens, hkv, D, bs)
+    k = np.zeros(v.shape, np.float16)
+    k[..., 0] = 2048
+    for b, n in enumerate(lens):
+        at = np.arange(n)
+        k[table[b, at // bs], :, at % bs, 1] = _rising(rng, n, range(13))[:, None]
+    q = np.zeros((len(lens), hq, D), np.float16)
+    q[:, :, 0] = 4096 * np.sign(scale)
+    q[:, :, 1] = rng.choice([1, -1], hq)
+    out = _keep_all(cuda, q, k, v, table, lens, scale)
+    _check_rows(out, q, k.astype(np.float64), v.astype(np.float64), table, lens, scale, bs)
 
 
 @pytest.mark.parametrize("hq,hkv,D,bs", Q4_SHAPES + [(20, 2, 128, 16), (10, 1, 240, 16)])

@@ -25,7 +25,7 @@ struct Params {
   const int* block_tables;  // [B][max_blocks]
   const int* seq_lens;      // [B]
   float* part_o;   // [B][Hq][slots][D] unnormalised partial outputs
-  float* part_ml;  // [B][Hq][slots][2] (max in log2 units, sum of exp2)
+  float* part_ml;  // [B][Hq][slots][2] (max, see ml_unit; sum of exp2)
   int* status;     // device status word (NXT_PA_DEV_* bits), may be null
   long long kv_block_stride;
   long long kv_head_stride;
@@ -73,6 +73,10 @@ struct Params {
   // scale_log2; v_scale multiplies V (generic path) or O (fast path).
   int kv_fmt;
   float v_scale;
+  // What a partial's max is in: log2 units (1), or units whose differences times
+  // this are. A max of raw scores times a scale is rounded by more than a whole
+  // log2 unit from 2^25 on, a difference of raw scores is not.
+  float ml_unit = 1.f;
 };
 
 constexpr int kKvE4M3 = 1;
@@ -523,7 +527,9 @@ __device__ __forceinline__ void merge_row_warp(const Params& p, long long row, i
   float mx = mine.x;
   for (int i = lane + 32; i < nslots; i += 32) mx = fmaxf(mx, __ldcg(&ml[i].x));
   const float M = warp_max(mx);
-  auto weight = [M](float m) { return (M == -INFINITY || m == -INFINITY) ? 0.f : ex2(m - M); };
+  auto weight = [M, &p](float m) {
+    return (M == -INFINITY || m == -INFINITY) ? 0.f : ex2((m - M) * p.ml_unit);
+  };
   const float wm = weight(mine.x);
   sw[lane] = wm;
   float den = wm * mine.y;

@@ -7,6 +7,7 @@
 #include <stddef.h>
 
 #include <atomic>
+#include <cmath>
 #include <mutex>
 
 namespace xpa {
@@ -51,6 +52,12 @@ struct Plan {
 // shortest partition, in pages.
 Plan make_plan(int B, int Hq, int D, int Hkv, int max_blocks, int nsm, int kv_es = 2,
                int min_items = 0, int min_pages = 4);
+
+// Params::ml_unit of the same kernels: they handle scores as q . k times this,
+// with the scale's sign in Q (a scale of 0 is a Q of 0).
+inline float score_unit(float scale_log2) {
+  return scale_log2 == 0.f ? 1.f : std::fabs(scale_log2);
+}
 
 // Plan of the kernels that take an item in 16-token tiles (4-bit, fp16 pages).
 Plan tile_plan(int B, int Hq, int D, int Hkv, int max_blocks, int bs, int nsm);

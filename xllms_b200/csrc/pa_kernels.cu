@@ -776,7 +776,9 @@ __global__ void __launch_bounds__(128) pa_reduce_wide_kernel(const Params p) {
   if (lane == 0) s_max[warp] = mx;
   __syncthreads();
   const float M = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-  auto weight = [M](float m) { return (M == -INFINITY || m == -INFINITY) ? 0.f : ex2(m - M); };
+  auto weight = [M, &p](float m) {
+    return (M == -INFINITY || m == -INFINITY) ? 0.f : ex2((m - M) * p.ml_unit);
+  };
 
   const float* po = p.part_o + row * p.slots * p.D;
   float den = 0.f;

@@ -9,8 +9,9 @@
 // conflict. Per tile, with mma.sync m16n8k16 (fp16 in, fp32 sums):
 //   S^T(16 tokens x 8 heads) = K . Q^T,  O^T(D x 8 heads) += V^T . P^T
 // The weights go in as two fp16 terms (22 bits). The reference point of the
-// softmax moves when a score passes it by more than 8 in the exp2 domain. Rows
-// past the end, or of pages that are not there, are filled with zeros.
+// softmax moves when a score passes it by more than 8 in the exp2 domain, and
+// exponents are formed from the distance to it, as in the 4-bit kernel. Rows past
+// the end, or of pages that are not there, are filled with zeros.
 // Bound by the latency of short items: 4 D bytes a token against 4 D flop per
 // head and token leave HBM the limit, and the kept pages of a row are few.
 // 43 sequences, 20 heads over 5 of 112, 28 pages each (43 MB): 17 us, where the
@@ -70,8 +71,8 @@ __global__ void __launch_bounds__(kWarps * 32) pa_pages_kernel(const Params p, i
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
 
-  // Scores are q . k times a positive factor: its sign goes into Q.
-  const float sl = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+  // scores are q . k times sl; see score_unit
+  const float sl = p.ml_unit;
   const float sign = p.scale_log2 > 0.f ? 1.f : p.scale_log2 < 0.f ? -1.f : 0.f;
   const float slack = fminf(kRaiseBy / sl, 1e30f);
   // head g: channels 16 s + 2 t, + 1 and + 8, + 9
@@ -126,9 +127,8 @@ __global__ void __launch_bounds__(kWarps * 32) pa_pages_kernel(const Params p, i
   };
 
   float o[NGM][4] = {};
-  // heads 2 t, 2 t + 1: reference point in units of q . k, the same less
-  // kShiftBy in the exp2 domain, and the weights' sum
-  float m[2] = {-INFINITY, -INFINITY}, moff[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
+  // heads 2 t, 2 t + 1: reference point in units of q . k, and the weights' sum
+  float m[2] = {kNoScore, kNoScore}, l[2] = {0.f, 0.f};
   // rows 0-7, 8-15, then the next 8 values; transposed: tokens 0-7, then 8-15
   const uint32_t kfrag = (lane & 15) * pitch + (lane >> 4) * 16;
   const uint32_t vfrag =
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kWarps * 32) pa_pages_kernel(const Params p, i
       x[c] += y[c];
       if (g + 8 * (c >> 1) >= here) x[c] = -INFINITY;
     }
-    const bool raise = fmaxf(x[0], x[2]) > m[0] + slack || fmaxf(x[1], x[3]) > m[1] + slack;
+    const bool raise = fmaxf(x[0], x[2]) - m[0] > slack || fmaxf(x[1], x[3]) - m[1] > slack;
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -167,9 +167,8 @@ __global__ void __launch_bounds__(kWarps * 32) pa_pages_kernel(const Params p, i
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
         mx = fmaxf(mx, m[c]);
-        const float f = m[c] == -INFINITY ? 0.f : ex2((m[c] - mx) * sl);
+        const float f = ex2((m[c] - mx) * sl);
         m[c] = mx;
-        moff[c] = mx == -INFINITY ? 0.f : fmaf(mx, sl, -kShiftBy);
         l[c] *= f;
 #pragma unroll
         for (int s = 0; s < NGM; ++s) {
@@ -180,7 +179,7 @@ __global__ void __launch_bounds__(kWarps * 32) pa_pages_kernel(const Params p, i
     }
     float w[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) w[c] = ex2(fmaf(x[c], sl, -moff[c & 1]));
+    for (int c = 0; c < 4; ++c) w[c] = ex2(fmaf(x[c] - m[c & 1], sl, kShiftBy));
     l[0] += w[0] + w[2];
     l[1] += w[1] + w[3];
     uint32_t hi[2], lo[2];
@@ -221,7 +220,7 @@ __global__ void __launch_bounds__(kWarps * 32) pa_pages_kernel(const Params p, i
 #pragma unroll
     for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
     if (g == 0) {
-      sml[(warp * HEADS + head) * 2] = m[c] == -INFINITY ? -INFINITY : moff[c];
+      sml[(warp * HEADS + head) * 2] = m[c] == kNoScore ? -INFINITY : m[c];
       sml[(warp * HEADS + head) * 2 + 1] = sum;
     }
   }

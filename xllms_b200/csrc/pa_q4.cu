@@ -227,9 +227,11 @@ __global__ void __launch_bounds__(128) pa_q4_read_kernel(const Q4RowsParams a) {
 // 2 t + 8, 2 t + 9 are channels 16 j + 4 t .. + 3 (Q's fragments follow); V
 // row tile 4 w + i holds channels 8 (g W + w) + 2 i (row g) and + 1 (row g + 8).
 //
-// Softmax: scores live in the exp2 domain. The reference point m of a head
-// moves only when a score exceeds it by more than 8, so most steps need one
-// vote and no shuffles. The weights p = 2^(x - m + 7) <= 2^15 go into the
+// Softmax: the reference point m of a head moves only when a score exceeds it
+// by more than 8 in the exp2 domain, so most steps need one vote and no
+// shuffles. Exponents are formed from x - m: the distance is all but exact
+// where it matters, while x or m times the scale is rounded by more than a whole
+// unit from 2^25 on. The weights p = 2^(x - m + 7) <= 2^15 go into the
 // product as two fp16 terms, p rounded and what that leaves: 22 bits, like the
 // other decode kernels' (2^-22 of a weight at most, 2^-32 of the largest where
 // the second term is subnormal). The rounded weight alone takes a tenth less
@@ -534,9 +536,8 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
 
-  // Scores are handled as q . k times a positive factor: its sign goes into Q
-  // (a factor of 0 is a Q of 0).
-  const float sl = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+  // scores are q . k times sl; see score_unit
+  const float sl = p.ml_unit;
   const float sign = p.scale_log2 > 0.f ? 1.f : p.scale_log2 < 0.f ? -1.f : 0.f;
   const float slack = fminf(kRaise / sl, 1e30f);  // kRaise in units of q . k
 
@@ -624,15 +625,14 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, co
   };
 
   float o[4 * W][NT][4] = {};
-  // Heads 2 t, 2 t + 1 of each tile: the reference point m in units of q . k
-  // and the same less kShift in the exp2 domain, and the weights' sum.
-  float m[NT][2], moff[NT][2], l[NT][2];
+  // Heads 2 t, 2 t + 1 of each tile: the reference point m in units of q . k,
+  // and the weights' sum.
+  float m[NT][2], l[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      m[nt][c] = -INFINITY;
-      moff[nt][c] = 0.f;
+      m[nt][c] = kNoScore;
       l[nt][c] = 0.f;
     }
 
@@ -713,7 +713,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, co
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c)
-        raise |= top(nt, c) > m[nt][c] + slack;
+        raise |= top(nt, c) - m[nt][c] > slack;
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -723,9 +723,8 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, co
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
           mx = fmaxf(mx, m[nt][c]);
-          const float f = m[nt][c] == -INFINITY ? 0.f : ex2((m[nt][c] - mx) * sl);
+          const float f = ex2((m[nt][c] - mx) * sl);
           m[nt][c] = mx;
-          moff[nt][c] = mx == -INFINITY ? 0.f : fmaf(mx, sl, -kShift);
           l[nt][c] *= f;
 #pragma unroll
           for (int mt = 0; mt < 4 * W; ++mt) {
@@ -741,8 +740,8 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, co
       for (int nt = 0; nt < NT; ++nt) {
         float e[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)  // a masked score is -inf and its weight 0, whatever moff is
-          e[c] = ex2(fmaf(x[u][nt][c], sl, -moff[nt][c & 1]));
+        for (int c = 0; c < 4; ++c)  // a masked score is -inf and its weight 0, whatever m is
+          e[c] = ex2(fmaf(x[u][nt][c] - m[nt][c & 1], sl, kShift));
         l[nt][0] += e[0] + e[2];
         l[nt][1] += e[1] + e[3];
 #pragma unroll
@@ -827,8 +826,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, co
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
       if (g == 0) {
-        // any common offset of the reference points leaves the merges as they are
-        sml[(warp * C::kHeads + head) * 2] = m[nt][c] == -INFINITY ? -INFINITY : moff[nt][c];
+        sml[(warp * C::kHeads + head) * 2] = m[nt][c] == kNoScore ? -INFINITY : m[nt][c];
         sml[(warp * C::kHeads + head) * 2 + 1] = s;
       }
     }

@@ -23,6 +23,8 @@
 // Every token's row is its own bytes, so tokens are written independently.
 #pragma once
 
+#include <cfloat>
+
 #include "pa_device.cuh"
 
 namespace xpa {
@@ -105,6 +107,9 @@ __device__ __forceinline__ void cp_async_wait() {
 
 // ── partitions and their merge over a CTA's warps ───────────────────────
 constexpr int kGridY = 32768;
+// A warp's reference point before any score above -inf: below every score, and
+// finite, so that a score's distance from it is never NaN.
+constexpr float kNoScore = -FLT_MAX;
 
 // Partition blockIdx.x of row (sequence, KV head).
 __device__ __forceinline__ ItemKind part_item(const Params& p, int row, Item& it) {
@@ -130,7 +135,8 @@ __device__ __forceinline__ ItemKind part_item(const Params& p, int row, Item& it
 
 // Merges the warps' states and stores the item: the output itself, or a partial.
 // so: [NW][HEADS][ROW] sums of weights times V; sml: [NW][HEADS] reference point
-// (-inf: no score above -inf) and sum of the weights. D is a multiple of 16.
+// in units of q . k, p.ml_unit of the exp2 domain each (-inf: no score above
+// -inf), and sum of the weights. D is a multiple of 16.
 template <int NW, int HEADS, int ROW>
 __device__ __forceinline__ void merge_warps(const Params& p, const Item& it, const float* so,
                                             const float* sml, long long row0, int nh, int D) {
@@ -145,7 +151,7 @@ __device__ __forceinline__ void merge_warps(const Params& p, const Item& it, con
     for (int w = 0; w < NW; ++w) {
       const float mw = sml[(w * HEADS + head) * 2];
       // a warp without a score above -inf holds zeros, or NaN to pass on
-      const float wt = mw == M ? 1.f : ex2(mw - M);
+      const float wt = mw == M ? 1.f : ex2((mw - M) * p.ml_unit);
       den = fmaf(wt, sml[(w * HEADS + head) * 2 + 1], den);
       const float4* src =
           reinterpret_cast<const float4*>(so + (size_t)(w * HEADS + head) * ROW + d0);

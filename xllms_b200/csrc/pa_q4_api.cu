@@ -189,6 +189,7 @@ int attention_call(void* out, const void* q, const void* k, const void* v, const
   p.max_parts = pl.max_parts;
   p.slots = pl.max_parts;
   p.scale_log2 = scale * ks * 1.4426950408889634f;
+  p.ml_unit = score_unit(p.scale_log2);
   p.v_scale = vs;
   p.vec8 = aligned(out, 16) ? 1 : 0;
   cudaError_t e = xpa::launch_q4_attention(p, st);

@@ -331,6 +331,7 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
     a.part_pages = pl.part_pages;
     a.max_parts = a.slots = pl.max_parts;
     a.scale_log2 = c.scale * 1.4426950408889634f;
+    a.ml_unit = score_unit(a.scale_log2);
     a.v_scale = 1.f;
     a.vec8 = aligned(c.out, 16) ? 1 : 0;
     cudaError_t err = xpa::launch_pages(a, st);
