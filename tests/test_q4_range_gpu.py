@@ -203,3 +203,59 @@ def test_q4_weights_keep_22_bits(cuda, hq, hkv, D, bs):
     for scale in (1 / 16, 1 / 64):
         out = _q4_call(cuda, q, pools, table, lens, scale)
         _check_rows(out, q, k, v, table, lens, scale, bs)
+
+
+# ── NaN ───────────────────────────────────────────────────────────────────
+def test_a_nan_query_gives_zeros_however_a_row_is_split(cuda):
+    """As in the framework's other decode calls: a head whose scores are NaN has
+    no sum above 0 and its output is 0, in one partition or many; the others'
+    outputs are off by no more than their rounding (the reference points of a
+    warp's heads move together, so not every bit need be the same)."""
+    rng = np.random.default_rng(6)
+    hq, hkv, D, bs, lens = 8, 2, 128, 16, [40, 1, 6000, 4097]
+    table, nb = _paged(rng, lens, bs)
+    q = rng.standard_normal((len(lens), hq, D)).astype(np.float16)
+    bad = q.copy()
+    bad[:, 1, 5] = np.nan
+    bad[:, 6] = np.nan
+    others = [0, 2, 3, 4, 5, 7]
+    kv = rng.standard_normal((2, nb, hkv, bs, D)).astype(np.float16)
+    pools, (_, v4) = _q4_pools(rng, rng.integers(0, 16, (nb, hkv, bs, D)).astype(np.uint8), 0x38)
+    lt = _t(np.asarray(lens, np.int32), cuda)
+    calls = {
+        "fp16": lambda x: PA.paged_attention(_t(x, cuda), _t(kv[0], cuda), _t(kv[1], cuda),
+                                             _t(table, cuda), lt),
+        "q4": lambda x: _q4_call(cuda, x, pools, table, lens, 0.1),
+    }
+    def check(good, out, top, name):
+        assert not out[:, [1, 6]].any(), name
+        # one fp16 step, and twice the sums' bound
+        tol = good.abs().double() * 2.0 ** -10 + top * 2 * 2.0 ** -22 * (
+            _t(np.asarray(lens) / 16 + 20.0, cuda))[:, None, None]
+        assert ((out.double() - good.double()).abs() <= tol)[:, others].all(), name
+
+    for name, call in calls.items():
+        check(call(q), call(bad), 8.0 if name == "fp16" else float(abs(v4).max()), name)
+    k = rng.standard_normal((nb, hkv, bs, 112)).astype(np.float16)
+    q, bad = q[..., :112], bad[..., :112]
+    check(*(_keep_all(cuda, x, k, k, table, lens, 0.1) for x in (q, bad)), 8.0, "pages")
+
+
+@pytest.mark.parametrize("at", [0, 33, "last"])
+@pytest.mark.parametrize("hq,hkv,D,bs", PAGE_SHAPES)
+def test_a_nan_key_gives_zeros_however_a_row_is_split(cuda, hq, hkv, D, bs, at):
+    """Also where the NaN is the only token of the row's last partition."""
+    rng = np.random.default_rng(7)
+    lens = [64, 500, 2049, 4097]
+    table, nb, v = _pages_case(rng, lens, hkv, D, bs)
+    k = rng.standard_normal(v.shape).astype(np.float16)
+    for b, n in enumerate(lens):
+        tok = n - 1 if at == "last" else at
+        k[table[b, tok // bs], 0, tok % bs, 2] = np.nan
+    q = rng.standard_normal((len(lens), hq, D)).astype(np.float16)
+    out = _keep_all(cuda, q, k, v, table, lens, 0.1)
+    group = hq // hkv
+    assert not out[:, :group].any()
+    if hkv > 1:
+        clean = np.nan_to_num(k)
+        assert (out[:, group:] == _keep_all(cuda, q, clean, v, table, lens, 0.1)[:, group:]).all()

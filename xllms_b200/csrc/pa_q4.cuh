@@ -134,6 +134,8 @@ __device__ __forceinline__ ItemKind part_item(const Params& p, int row, Item& it
 }
 
 // Merges the warps' states and stores the item: the output itself, or a partial.
+// A row whose weights' sum is not above 0 (nothing valid, or a NaN score) is 0,
+// as in every other kernel here and however the row is split.
 // so: [NW][HEADS][ROW] sums of weights times V; sml: [NW][HEADS] reference point
 // in units of q . k, p.ml_unit of the exp2 domain each (-inf: no score above
 // -inf), and sum of the weights. D is a multiple of 16.
@@ -150,7 +152,7 @@ __device__ __forceinline__ void merge_warps(const Params& p, const Item& it, con
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
       const float mw = sml[(w * HEADS + head) * 2];
-      // a warp without a score above -inf holds zeros, or NaN to pass on
+      // a warp without a score above -inf holds zeros, or NaN sums to pass on
       const float wt = mw == M ? 1.f : ex2((mw - M) * p.ml_unit);
       den = fmaf(wt, sml[(w * HEADS + head) * 2 + 1], den);
       const float4* src =
@@ -169,7 +171,7 @@ __device__ __forceinline__ void merge_warps(const Params& p, const Item& it, con
     for (int k = 0; k < 8; ++k) num[k] *= p.v_scale;
     if (it.direct) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) num[k] = den == 0.f ? 0.f : num[k] / den;
+      for (int k = 0; k < 8; ++k) num[k] = den > 0.f ? num[k] / den : 0.f;
       if (p.vec8) {
         store_out8<__half>(p, row0 + head, d0, num);
       } else {
@@ -182,7 +184,10 @@ __device__ __forceinline__ void merge_warps(const Params& p, const Item& it, con
       float4* dst = reinterpret_cast<float4*>(p.part_o + pr * D + d0);
       dst[0] = make_float4(num[0], num[1], num[2], num[3]);
       dst[1] = make_float4(num[4], num[5], num[6], num[7]);
-      if (d0 == 0) reinterpret_cast<float2*>(p.part_ml)[pr] = make_float2(M, den);
+      // the merge of partials leaves out one without a score above -inf: NaN
+      // sums are not to be lost with it
+      if (d0 == 0)
+        reinterpret_cast<float2*>(p.part_ml)[pr] = make_float2(isnan(den) ? 0.f : M, den);
     }
   }
 }
