@@ -1,11 +1,16 @@
 """The 4-bit cache, and attention over fp16 pages, at the ends of their range
 and in narrow calls, against statements in 64 bits."""
 import math
+import os
+import subprocess
+import sys
+import threading
 
 import numpy as np
 import pytest
 
 import _q4ref as R
+from xllms_b200 import _native
 from xllms_b200 import operator_api as PA
 
 pytestmark = pytest.mark.gpu
@@ -259,3 +264,86 @@ def test_a_nan_key_gives_zeros_however_a_row_is_split(cuda, hq, hkv, D, bs, at):
     if hkv > 1:
         clean = np.nan_to_num(k)
         assert (out[:, group:] == _keep_all(cuda, q, clean, v, table, lens, 0.1)[:, group:]).all()
+
+
+# ── another thread's capture ──────────────────────────────────────────────
+def test_an_eager_call_on_a_new_stream_leaves_another_threads_capture_alone(cuda):
+    """While one thread captures, another makes its stream's first call (which
+    allocates that stream's scratch) and a larger one (which replaces it)."""
+    import torch
+    rng = np.random.default_rng(5)
+    cases = []
+    for lens in ([6000, 5000], [9000] * 6):
+        table, nb = _paged(rng, lens, 16)
+        pools, _ = _q4_pools(rng, rng.integers(0, 16, (nb, 8, 16, 128)).astype(np.uint8), 0x38)
+        q = rng.standard_normal((len(lens), 32, 128)).astype(np.float16)
+        args = [_t(x, cuda) for x in (q, *pools, table, np.asarray(lens, np.int32))]
+        want = PA.paged_attention_q4(*args, 1.0, 0.5)
+        cases.append((args, want, torch.empty_like(want), torch.empty_like(want)))
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    # every stream's scratch is gone: the next call on each is its first
+    assert _native.xpa().nxt_paged_attention_release_workspaces() == _native.NXT_PA_OK
+    failed = []
+
+    def eager():
+        try:
+            for args, _, out, _ in cases:
+                PA.paged_attention_q4(*args, 1.0, 0.5, out=out, stream=other)
+        except Exception as exc:  # looked at by the test's own thread
+            failed.append(exc)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        PA.paged_attention_q4(*cases[0][0], 1.0, 0.5, out=cases[0][3])
+        thread = threading.Thread(target=eager)
+        thread.start()
+        thread.join()
+        PA.paged_attention_q4(*cases[1][0], 1.0, 0.5, out=cases[1][3])
+    assert not failed, failed
+    graph.replay()
+    torch.cuda.synchronize()
+    for _, want, out, captured in cases:
+        assert torch.equal(out, want) and torch.equal(captured, want)
+
+
+FIRST_CALL = """
+import sys, threading
+import torch
+from xllms_b200 import operator_api as PA
+dev = torch.device("cuda:0")
+q = torch.randn(2, 8, 128, device=dev).half()
+pool = torch.zeros(PA.q4_pool_shape(200, 2, 16, 128), dtype=torch.uint8, device=dev)
+pool.view(-1)[::5] = 0x31
+table = torch.arange(200, dtype=torch.int32, device=dev).view(2, 100)
+lens = torch.tensor([1600, 1500], dtype=torch.int32, device=dev)
+outs = [torch.zeros_like(q) for _ in range(2)]
+side, other = torch.cuda.Stream(), torch.cuda.Stream()
+call = lambda out, st: PA.paged_attention_q4(q, pool, pool, table, lens, 1.0, 1.0, out=out, stream=st)
+x = torch.zeros(4, device=dev)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=side):
+    x.add_(1)
+    if sys.argv[1] == "beside":
+        thread = threading.Thread(target=call, args=(outs[0], other))
+        thread.start()
+        thread.join()
+    else:
+        call(outs[0], None)
+graph.replay()
+torch.cuda.synchronize()
+call(outs[1], None)
+torch.cuda.synchronize()
+assert outs[1].any() and torch.equal(*outs) and (x == 1).all() and PA.device_status() == 0
+print("first call ok")
+"""
+
+
+@pytest.mark.parametrize("where", ["beside", "inside"])
+def test_the_devices_first_call_beside_or_inside_a_capture(cuda, where):
+    """A process of its own, whose first library call allocates the status word."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL, where], cwd=root, capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0 and "first call ok" in r.stdout, r.stderr[-2000:]

@@ -64,15 +64,60 @@ struct Workspace {
 // Keyed by (device, stream) so calls on different streams never share partials.
 std::map<std::pair<int, uintptr_t>, Workspace> g_ws;
 
-// Scratch of the 4-bit and sparse entry points (acquire_scratch).
+// Device memory for the library. An allocation is no part of a capture: in the
+// default mode one would fail while any thread captures, and end that capture.
+class OutsideCaptures {
+ public:
+  OutsideCaptures() { ok_ = cudaThreadExchangeStreamCaptureMode(&mode_) == cudaSuccess; }
+  ~OutsideCaptures() {
+    if (ok_) cudaThreadExchangeStreamCaptureMode(&mode_);
+  }
+  OutsideCaptures(const OutsideCaptures&) = delete;
+  OutsideCaptures& operator=(const OutsideCaptures&) = delete;
+  bool ok() const { return ok_; }
+
+ private:
+  cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
+  bool ok_;
+};
+
+int device_alloc(size_t bytes, void** out) {
+  OutsideCaptures outside;
+  if (!outside.ok()) return NXT_PA_ECUDA;
+  const cudaError_t e = cudaMalloc(out, bytes);
+  if (e == cudaSuccess) return NXT_PA_OK;
+  cudaGetLastError();
+  return e == cudaErrorMemoryAllocation ? NXT_PA_ENOMEM : NXT_PA_ECUDA;
+}
+
+// The same, filled with zeros on a stream of its own.
+int device_alloc_zeros(size_t bytes, void** out) {
+  const int rc = device_alloc(bytes, out);
+  if (rc != NXT_PA_OK) return rc;
+  OutsideCaptures outside;
+  cudaStream_t st = nullptr;
+  bool ok = outside.ok() && cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) == cudaSuccess;
+  ok = ok && cudaMemsetAsync(*out, 0, bytes, st) == cudaSuccess &&
+       cudaStreamSynchronize(st) == cudaSuccess;
+  if (st) cudaStreamDestroy(st);
+  if (ok) return NXT_PA_OK;
+  cudaGetLastError();
+  cudaFree(*out);
+  *out = nullptr;
+  return NXT_PA_ECUDA;
+}
+
+// Scratch of the 4-bit and sparse entry points (acquire_scratch) on one stream.
+// Its lock is held while a call enqueues; other streams' calls do not wait.
 struct Scratch {
-  Workspace eager;     // of calls that run at once
-  Workspace captured;  // of the calls in one stream capture
+  std::mutex mu;
+  Workspace eager;         // of calls that run at once
+  std::vector<void*> old;  // outgrown ones
+  Workspace captured;      // of the calls in one stream capture
   unsigned long long capture = 0;  // which
 };
-std::mutex g_scratch_mu;
-std::map<std::pair<int, uintptr_t>, Scratch> g_scratch;
-std::vector<std::pair<int, void*>> g_scratch_old;  // outgrown buffers, by device
+std::mutex g_scratch_mu;  // the map; entries are never erased
+std::map<std::pair<int, uintptr_t>, std::unique_ptr<Scratch>> g_scratch;
 
 // A captured call's buffer belongs to its graph and comes back here when the
 // graph and what was instantiated from it are gone. That happens on a thread
@@ -109,14 +154,8 @@ int buffer_of_graph(int dev, cudaGraph_t graph, size_t bytes, Workspace* out) {
       }
   }
   if (!b->ptr) {
-    // an allocation is no part of the capture
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return NXT_PA_ECUDA;
-    const cudaError_t e = cudaMalloc(&b->ptr, bytes);
-    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess || e != cudaSuccess) {
-      cudaGetLastError();
-      return NXT_PA_ENOMEM;
-    }
+    const int rc = device_alloc(bytes, &b->ptr);
+    if (rc != NXT_PA_OK) return rc;
   }
   const Workspace w{b->ptr, b->bytes};
   cudaUserObject_t obj;
@@ -163,11 +202,8 @@ int device_state_locked(int dev, DeviceState** out) {
   }
   if (!d.status) {
     void* p = nullptr;
-    if (cudaMalloc(&p, 256) != cudaSuccess) return NXT_PA_ENOMEM;
-    if (cudaMemset(p, 0, 256) != cudaSuccess) {
-      cudaFree(p);
-      return NXT_PA_ECUDA;
-    }
+    const int rc = device_alloc_zeros(256, &p);
+    if (rc != NXT_PA_OK) return rc;
     d.status = static_cast<int*>(p);
   }
   *out = &d;
@@ -211,8 +247,15 @@ int acquire_scratch(int dev, cudaStream_t st, size_t bytes, void** out,
     cudaGetLastError();
     return NXT_PA_ECUDA;
   }
-  lk = std::unique_lock<std::mutex>(g_scratch_mu);
-  Scratch& s = g_scratch[{dev, stream_key(st)}];
+  Scratch* entry;
+  {
+    std::lock_guard<std::mutex> map_lock(g_scratch_mu);
+    std::unique_ptr<Scratch>& slot = g_scratch[{dev, stream_key(st)}];
+    if (!slot) slot.reset(new Scratch);
+    entry = slot.get();
+  }
+  lk = std::unique_lock<std::mutex>(entry->mu);
+  Scratch& s = *entry;
   if (capturing == cudaStreamCaptureStatusActive) {
     if (s.capture != id || s.captured.bytes < bytes) {
       const int rc = buffer_of_graph(dev, graph, bytes, &s.captured);
@@ -226,14 +269,12 @@ int acquire_scratch(int dev, cudaStream_t st, size_t bytes, void** out,
   if (w.bytes < bytes) {
     // at least doubled, so that what is kept of old buffers stays below the newest
     const size_t want = std::max(bytes, 2 * w.bytes);
-    if (w.ptr) g_scratch_old.reserve(g_scratch_old.size() + 1);
+    if (w.ptr) s.old.reserve(s.old.size() + 1);
     void* p = nullptr;
-    if (cudaMalloc(&p, want) != cudaSuccess) {
-      cudaGetLastError();
-      return NXT_PA_ENOMEM;
-    }
+    const int rc = device_alloc(want, &p);
+    if (rc != NXT_PA_OK) return rc;
     // its last calls may still run
-    if (w.ptr) g_scratch_old.emplace_back(dev, w.ptr);
+    if (w.ptr) s.old.push_back(w.ptr);
     w.ptr = p;
     w.bytes = want;
   }
@@ -251,16 +292,21 @@ int release_scratch() {
   auto drop = [&rc](int dev, void* p) {
     if (p && (cudaSetDevice(dev) != cudaSuccess || cudaFree(p) != cudaSuccess)) rc = NXT_PA_ECUDA;
   };
-  for (auto& kv : g_scratch) drop(kv.first.first, kv.second.eager.ptr);
-  for (auto& o : g_scratch_old) drop(o.first, o.second);
+  for (auto& kv : g_scratch) {
+    Scratch& x = *kv.second;
+    std::lock_guard<std::mutex> one(x.mu);
+    drop(kv.first.first, x.eager.ptr);
+    for (void* o : x.old) drop(kv.first.first, o);
+    x.old.clear();
+    x.eager = x.captured = Workspace{};  // captured: the graph's
+    x.capture = 0;
+  }
   std::vector<GraphBuffer> back;
   {
     std::lock_guard<std::mutex> lb(g_back_mu);
     back.swap(g_back);
   }
   for (auto& o : back) drop(o.dev, o.ptr);  // those of living graphs stay theirs
-  g_scratch.clear();
-  g_scratch_old.clear();
   if (have_prev) cudaSetDevice(prev);
   return rc;
 }

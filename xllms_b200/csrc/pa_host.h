@@ -108,10 +108,11 @@ int status_word(int dev, int** out);
 // Library-owned scratch of the 4-bit and sparse entry points: one buffer per
 // (device, stream) for calls that run at once, and one per stream capture for
 // captured calls, which the graph owns, so that graphs may be replayed at the
-// same time as each other and as eager calls. `lk` holds the pool's lock on
+// same time as each other and as eager calls. `lk` holds the stream's lock on
 // return: keep it until the call's kernels are enqueued, so that no other
 // thread on the same stream can hand out the buffer in between. A buffer that
-// has to grow is replaced, and the old one kept until release_scratch().
+// has to grow is replaced, and the old one kept until release_scratch(). No
+// thread's capture is disturbed.
 // EINVAL / ECUDA / ENOMEM / OK.
 int acquire_scratch(int dev, cudaStream_t st, size_t bytes, void** out,
                     std::unique_lock<std::mutex>& lk);
