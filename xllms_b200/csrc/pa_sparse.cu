@@ -435,12 +435,15 @@ __global__ void __launch_bounds__(kScoreWarps * 32) pa_score_mma_kernel(const Se
       }
       __syncwarp();  // the stage may be filled again
       st ^= stage_bytes;
-      // heads h0 + 2 t, + 1 of pages g and g + 8: the largest over the group
+      // heads h0 + 2 t, + 1 of pages g and g + 8: the largest over the group.
+      // Rows of pages that are not there hold another page's bounds, and those
+      // widen no error bound.
+      const int e0 = __shfl_sync(0xffffffffu, e, g), e1 = __shfl_sync(0xffffffffu, e, g + 8);
       float most = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         x[0][k] += x[1][k];
-        most = fmaxf(most, y[0][k] + y[1][k]);
+        most = fmaxf(most, (k < 2 ? e0 : e1) < 0 ? 0.f : y[0][k] + y[1][k]);
       }
       const bool c0 = h0 + 2 * t < p.GS, c1 = h0 + 2 * t + 1 < p.GS;
       float s0 = fmaxf(c0 ? x[0][0] : -INFINITY, c1 ? x[0][1] : -INFINITY);
@@ -450,7 +453,6 @@ __global__ void __launch_bounds__(kScoreWarps * 32) pa_score_mma_kernel(const Se
       s0 = fmaxf(s0, __shfl_xor_sync(0xffffffffu, s0, 2));
       s1 = fmaxf(s1, __shfl_xor_sync(0xffffffffu, s1, 2));
       most = warp_max(most);
-      const int e0 = __shfl_sync(0xffffffffu, e, g), e1 = __shfl_sync(0xffffffffu, e, g + 8);
       e = next;
       // lane 0 of a quad stores page g, lane 1 page g + 8
       if (t < 2 && p0 + g + 8 * t < page_end) {
