@@ -266,6 +266,45 @@ def test_a_nan_key_gives_zeros_however_a_row_is_split(cuda, hq, hkv, D, bs, at):
         assert (out[:, group:] == _keep_all(cuda, q, clean, v, table, lens, 0.1)[:, group:]).all()
 
 
+# ── narrow calls ──────────────────────────────────────────────────────────
+def test_one_tokens_rows_of_any_outer_strides(cuda):
+    """With one token, or one head, the strides that no address uses may differ:
+    a view of a fused projection's row beside a dense one."""
+    import torch
+    D, bs = 64, 16
+    rng = np.random.default_rng(3)
+    for T, hkv in ((1, 2), (1, 1), (5, 1)):
+        width = 3 * hkv * D + 8
+        fused = _t(rng.standard_normal((T, width)).astype(np.float16), cuda)
+        if T > 1:  # rows of one head: any head stride beside the same token stride
+            key = fused.as_strided((T, 1, D), (width, 7, 1), 8)
+            value = fused.as_strided((T, 1, D), (width, D, 1), 8 + D)
+        else:
+            key = fused.as_strided((1, hkv, D), (width, D, 1), 8)
+            value = _t(rng.standard_normal((1, hkv, D)).astype(np.float16), cuda)
+        assert key.stride() != value.stride()
+        slots = _t(rng.permutation(32)[:T].astype(np.int64), cuda)
+        pools = torch.zeros((4,) + PA.q4_pool_shape(2, hkv, bs, D), dtype=torch.uint8, device=cuda)
+        PA.reshape_and_cache_q4(key, value, pools[0], pools[1], slots, 0.01, 0.02)
+        PA.reshape_and_cache_q4(key.clone(memory_format=torch.contiguous_format),
+                                value.clone(memory_format=torch.contiguous_format), pools[2],
+                                pools[3], slots, 0.01, 0.02)
+        assert torch.equal(pools[:2], pools[2:]) and pools[0].any()
+        want = PA.read_cache_q4(pools[0], pools[1], slots, 0.01, 0.02)
+        got = PA.read_cache_q4(pools[0], pools[1], slots, 0.01, 0.02, key=key, value=value)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_rows_of_two_tokens_still_need_one_stride(cuda):
+    import torch
+    rows = torch.zeros(2, 300, dtype=torch.float16, device=cuda)
+    key, dense = rows[:, :128].view(2, 2, 64), torch.zeros(2, 2, 64, dtype=torch.float16, device=cuda)
+    pool = torch.zeros(PA.q4_pool_shape(2, 2, 16, 64), dtype=torch.uint8, device=cuda)
+    slots = torch.arange(2, device=cuda)
+    with pytest.raises(PA.PagedAttentionError):
+        PA.reshape_and_cache_q4(key, dense, pool, pool.clone(), slots, 1.0, 1.0)
+
+
 # ── another thread's capture ──────────────────────────────────────────────
 def test_an_eager_call_on_a_new_stream_leaves_another_threads_capture_alone(cuda):
     """While one thread captures, another makes its stream's first call (which

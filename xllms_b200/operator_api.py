@@ -627,18 +627,20 @@ def _q4_dims(where, key_cache, value_cache, device):
 
 
 def _row_stride(where, key, value, slots, heads, dim, device):
+    """Token stride of key and value rows [T, Hkv, D]. Strides of a dimension of
+    one element reach no address and may be anything."""
     import torch
     T = key.shape[0] if key.dim() == 3 else -1
-    ks = key.stride()
     if (key.shape != (T, heads, dim) or value.shape != key.shape or key.dtype != torch.float16
-            or value.dtype != torch.float16 or value.stride() != ks
-            or (T and (ks[2] != 1 or (heads > 1 and ks[1] != dim)
-                       or (T > 1 and ks[0] < heads * dim)))
-            or slots.dtype != torch.int64 or slots.numel() < T or not slots.is_contiguous()
-            or device < 0 or key.get_device() != device or value.get_device() != device
-            or slots.get_device() != device):
-        _refuse(where, "rows must be fp16 [T, Hkv, D] with dense heads and slot_mapping int64 [T], "
-                "on the pools' CUDA device")
+            or value.dtype != torch.float16 or slots.dtype != torch.int64 or slots.numel() < T
+            or not slots.is_contiguous() or device < 0 or key.get_device() != device
+            or value.get_device() != device or slots.get_device() != device):
+        _refuse(where, "rows must be fp16 [T, Hkv, D] and slot_mapping int64 [T], on the pools' "
+                "CUDA device")
+    ks, vs = key.stride(), value.stride()
+    if T and (ks[2] != 1 or vs[2] != 1 or (heads > 1 and (ks[1] != dim or vs[1] != dim))
+              or (T > 1 and (ks[0] != vs[0] or ks[0] < heads * dim))):
+        _refuse(where, "rows must have dense heads, and key and value one token stride")
     return ks[0] if T > 1 else heads * dim
 
 
