@@ -4,11 +4,12 @@ calls take."""
 import numpy as np
 import pytest
 
-from test_sparse_gpu import _t
+from test_sparse_gpu import _case, _t
 from xllms_b200 import _native
 from xllms_b200 import operator_api as PA
 
 pytestmark = pytest.mark.gpu
+KS, VS = 0.011, 0.0073
 
 
 @pytest.mark.parametrize("kind", ["tensor cores", "scalar"])
@@ -44,3 +45,25 @@ def test_pages_that_are_not_there_widen_no_error_bound(cuda, kind):
         seen.append((int((words != sentinel).sum()), pages.cpu().numpy().tolist()))
     PA.device_status(clear=True)
     assert all(s == seen[0] for s in seen[1:]), [s[0] for s in seen]
+
+
+def test_selected_tables_of_4_bit_pools(cuda):
+    """select_pages over a 4-bit pool: the tables of its pages, per KV head."""
+    import torch
+    hq, hkv, D, bs, keep = 8, 2, 64, 32, 7
+    q, k, v, table, lens = _case(41, [900, 0, 77], hq, hkv, D, bs)
+    kc = torch.zeros(PA.q4_pool_shape(len(k), hkv, bs, D), dtype=torch.uint8, device=cuda)
+    vc = torch.zeros_like(kc)
+    rows = lambda x: _t(x.transpose(0, 2, 1, 3).reshape(-1, hkv, D), cuda)
+    PA.reshape_and_cache_q4(rows(k), rows(v), kc, vc, torch.arange(len(k) * bs, device=cuda), KS, VS)
+    qt, tt, lt = _t(q, cuda), _t(table, cuda), _t(lens, cuda)
+    bnd = PA.page_bounds(kc, tt, lt, torch.zeros(len(k), hkv, 2, D, dtype=torch.float16,
+                                                 device=cuda), k_scale=KS)
+    kept = torch.empty(3, hkv, keep, dtype=torch.int32, device=cuda)
+    want = PA.paged_attention_sparse(qt, kc, vc, bnd, tt, lt, keep, selected=kept, k_scale=KS,
+                                     v_scale=VS)
+    tables, slens, pages = PA.select_pages(qt, kc, bnd, tt, lt, keep)
+    assert torch.equal(pages, kept)
+    one = lambda x: x.view(len(k) * hkv, 1, bs // 16, 9 * D)
+    got = PA.paged_attention_q4(qt.view(3 * hkv, hq // hkv, D), one(kc), one(vc), tables, slens, KS, VS)
+    assert torch.equal(got.view_as(want), want)

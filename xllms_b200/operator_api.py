@@ -879,14 +879,16 @@ def _check_sparse(where, query, key_cache, value_cache, bounds, block_tables, se
 def select_pages(query, key_cache, bounds, block_tables, seq_lens, max_pages, *, sink_pages=0,
                  recent_pages=1, scale=None, num_blocks=None, device_status=None, stream=None):
     """The pages that sparse attention keeps: (tables int32 [B * Hkv,
-    max_pages], lens int32 [B * Hkv], pages int32 [B, Hkv, max_pages]). With
-    key_cache.view(NB * Hkv, 1, P, D), query.view(B * Hkv, G, D), tables and
+    max_pages], lens int32 [B * Hkv], pages int32 [B, Hkv, max_pages]).
+    key_cache is an fp16 or fp32 pool, or a 4-bit one (q4_pool_shape). With
+    key_cache.view(NB * Hkv, 1, ...), query.view(B * Hkv, G, D), tables and
     lens are the inputs of any attention call over the pool."""
     import torch
     device = query.get_device()
+    q4 = key_cache.dtype == torch.uint8
     B, Hq, (nb, hkv, bs, d, page, head) = _check_sparse(
         "select_pages", query, key_cache, key_cache, bounds, block_tables, seq_lens, None, device,
-        False)
+        q4)
     st, leave = _launch_on(device, stream)
     try:
         new = lambda *s: torch.empty(s, dtype=torch.int32, device=query.device)
