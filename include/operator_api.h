@@ -495,7 +495,9 @@ int nxt_paged_attention_sparse_ex(
     int *device_status,
     nxt_stream_t stream);
 
-/* The same over 4-bit pools. */
+/* The same over 4-bit pools; with num_blocks known, pools are refused whose
+ * kv_head_stride (kv_block_stride with one KV head) as the page stride would
+ * take them past the addresses of nxt_paged_attention_q4_ex. */
 int nxt_paged_attention_q4_sparse_ex(
     void *out, const void *query,
     const void *key_cache, const void *value_cache, const void *bounds,

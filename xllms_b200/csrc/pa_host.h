@@ -5,6 +5,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
+#include <stdint.h>
 
 #include <atomic>
 #include <cmath>
@@ -78,6 +79,13 @@ bool encode_pool(CUtensorMap* m, const void* base, int D, int Hkv, long long num
 // Pool alignment and stride order the TMA path needs.
 bool fast_layout_ok(const void* k, const void* v, int D, int Hkv, long long kbs, long long khs,
                     int es = 2);
+
+// What every call on 4-bit pools needs of them: NXT_PA_OK or NXT_PA_EINVAL.
+int check_q4_pools(const void* k, const void* v, int Hkv, int D, int bs, float k_scale,
+                   float v_scale, int64_t kbs, int64_t khs);
+// The 4-bit kernels address tiles by 32 bits of the largest unit that divides a
+// page and a tile. False: pools that are known (num_blocks > 0) to be larger.
+bool q4_addresses_ok(int D, int bs, int64_t kbs, int64_t num_blocks);
 
 // NXT_PA_OK or NXT_PA_EINVAL for the argument set of one call.
 int check_args(const void* out, const void* q, const void* k, const void* v, const int* bt,

@@ -60,11 +60,38 @@ Plan tile_plan(int B, int Hq, int D, int Hkv, int max_blocks, int bs, int nsm) {
 
 namespace {
 
-int map_cuda(cudaError_t e) { return e == cudaSuccess ? NXT_PA_OK : NXT_PA_ECUDA; }
-
 bool scale_ok(float s) { return s > 0.f && std::isfinite(s); }
 
 bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+}  // namespace
+
+namespace xpa {
+namespace host {
+
+// What every call on 4-bit pools needs of them.
+int check_q4_pools(const void* k, const void* v, int Hkv, int D, int bs, float ks, float vs,
+                   int64_t kbs, int64_t khs) {
+  if (!k || !v || !aligned(k, 16) || !aligned(v, 16)) return NXT_PA_EINVAL;
+  if (Hkv <= 0 || D <= 0 || D > 256 || D % 16 || bs <= 0 || bs % 16) return NXT_PA_EINVAL;
+  if (!scale_ok(ks) || !scale_ok(vs)) return NXT_PA_EINVAL;
+  if (kbs < 0 || kbs > INT_MAX || khs < 0 || kbs % 16 || khs % 16) return NXT_PA_EINVAL;
+  return NXT_PA_OK;
+}
+
+bool q4_addresses_ok(int D, int bs, int64_t kbs, int64_t num_blocks) {
+  if (num_blocks <= 0 || kbs <= 0) return true;
+  const long long unit = std::gcd((long long)kbs, 9LL * D);
+  const long long last = 0xfffffffeLL - (bs / 16) * (9LL * D / unit);
+  return last >= 0 && num_blocks - 1 <= last / (kbs / unit);
+}
+
+}  // namespace host
+}  // namespace xpa
+
+namespace {
+
+int map_cuda(cudaError_t e) { return e == cudaSuccess ? NXT_PA_OK : NXT_PA_ECUDA; }
 
 // 1 / s for the kernel's corrected quotient, which needs a significand that is
 // not all ones and room at both ends of the range; 0: divide.
@@ -75,22 +102,12 @@ float inverse_of(float s) {
   return ones || s < 0x1p-60f || s > 0x1p60f ? 0.f : 1.f / s;
 }
 
-// What every call on 4-bit pools needs of them.
-int check_pools(const void* k, const void* v, int Hkv, int D, int bs, float ks, float vs,
-                int64_t kbs, int64_t khs) {
-  if (!k || !v || !aligned(k, 16) || !aligned(v, 16)) return NXT_PA_EINVAL;
-  if (Hkv <= 0 || D <= 0 || D > 256 || D % 16 || bs <= 0 || bs % 16) return NXT_PA_EINVAL;
-  if (!scale_ok(ks) || !scale_ok(vs)) return NXT_PA_EINVAL;
-  if (kbs < 0 || kbs > INT_MAX || khs < 0 || kbs % 16 || khs % 16) return NXT_PA_EINVAL;
-  return NXT_PA_OK;
-}
-
 int rows_call(bool write, void* key, void* value, void* kc, void* vc, const int64_t* slots, int T,
               int Hkv, int D, int bs, float ks, float vs, int64_t kbs, int64_t khs,
               int64_t token_stride, int64_t num_blocks, cudaStream_t st) {
   if (T < 0) return NXT_PA_EINVAL;
   if (T == 0) return NXT_PA_OK;
-  const int rc = check_pools(kc, vc, Hkv, D, bs, ks, vs, kbs, khs);
+  const int rc = check_q4_pools(kc, vc, Hkv, D, bs, ks, vs, kbs, khs);
   if (rc != NXT_PA_OK) return rc;
   if (!key || !value || !slots || token_stride < (int64_t)Hkv * D) return NXT_PA_EINVAL;
   if (!aligned(key, 2) || !aligned(value, 2)) return NXT_PA_EINVAL;
@@ -129,9 +146,10 @@ int attention_call(void* out, const void* q, const void* k, const void* v, const
                    bool check_only = false) {
   int rc = check_args(out, q, k, v, bt, sl, B, Hq, D, Hkv, max_blocks, bs, 2, kbs, khs);
   if (rc != NXT_PA_OK || B == 0) return rc;
-  rc = check_pools(k, v, Hkv, D, bs, ks, vs, kbs, khs);
+  rc = check_q4_pools(k, v, Hkv, D, bs, ks, vs, kbs, khs);
   if (rc != NXT_PA_OK) return rc;
-  if (!aligned(q, 2) || !aligned(out, 2)) return NXT_PA_EINVAL;
+  if (!aligned(q, 2) || !aligned(out, 2) || !q4_addresses_ok(D, bs, kbs, num_blocks))
+    return NXT_PA_EINVAL;
   if (ws && !workspace_aligned(ws)) return NXT_PA_EINVAL;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return NXT_PA_ECUDA;
@@ -139,13 +157,6 @@ int attention_call(void* out, const void* q, const void* k, const void* v, const
   // one CTA per partition and 8 query heads (16 of a larger group) at least
   if ((long long)B * Hkv * pl.max_parts > INT_MAX || (long long)B * Hq > INT_MAX)
     return NXT_PA_EINVAL;
-  // the kernels address tiles by 32 bits of the largest unit that divides a
-  // page and a tile; pools that are known to be larger are refused
-  if (num_blocks > 0 && kbs > 0) {
-    const long long unit = std::gcd(kbs, 9LL * D);
-    if ((num_blocks - 1) * (kbs / unit) + (bs / 16) * (9LL * D / unit) > 0xfffffffeLL)
-      return NXT_PA_EINVAL;
-  }
   if (check_only) return NXT_PA_OK;
   int* status = dev_status;
   if (!status) {

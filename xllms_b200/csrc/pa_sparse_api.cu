@@ -205,10 +205,6 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
     return NXT_PA_EINVAL;
   if (std::isnan(c.scale)) return NXT_PA_EINVAL;
   if (c.Hkv > 1 && (c.khs <= 0 || c.kbs % c.khs || c.kbs / c.khs < c.Hkv)) return NXT_PA_EINVAL;
-  if (c.q4 && (c.D % 16 || c.bs % 16 || !(c.k_scale > 0.f) || !(c.v_scale > 0.f) ||
-               !std::isfinite(c.k_scale) || !std::isfinite(c.v_scale) || !aligned(c.k, 16) ||
-               !aligned(c.v, 16) || c.kbs % 16 || c.khs % 16 || !aligned(c.out, 2)))
-    return NXT_PA_EINVAL;
   if (ws && !workspace_aligned(ws)) return NXT_PA_EINVAL;
   const long long rows = (long long)c.B * c.Hkv;
   const int GS = c.Hq / c.Hkv;
@@ -217,6 +213,16 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
     return NXT_PA_EINVAL;
   const long long head_pages = c.Hkv > 1 ? c.kbs / c.khs : 1;
   const int64_t page_stride = c.Hkv > 1 ? c.khs : c.kbs;
+  // pages of the pool with one KV head, -1: unknown; ids are ints
+  int64_t nb = c.num_blocks > 0 ? c.num_blocks : -1;
+  if (nb > 0) nb = nb > INT_MAX / head_pages ? INT_MAX : nb * head_pages;
+  // all that the attention would refuse, before the selection is launched
+  if (c.q4) {
+    rc = check_q4_pools(c.k, c.v, 1, c.D, c.bs, c.k_scale, c.v_scale, page_stride, c.khs);
+    if (rc != NXT_PA_OK) return rc;
+    if (!aligned(c.q, 2) || !aligned(c.out, 2) || !q4_addresses_ok(c.D, c.bs, page_stride, nb))
+      return NXT_PA_EINVAL;
+  }
   // Longer pages go to the tensor-core kernel as pages of 16 tokens, where ids
   // of those fit
   int sub = 1;
@@ -297,8 +303,6 @@ int sparse_call(const SparseCall& c, int* sel_tables, int* sel_lens, void* ws, s
   if (e != cudaSuccess) return map_cuda(e);
   if (!attention) return NXT_PA_OK;
 
-  int64_t nb = c.num_blocks > 0 ? c.num_blocks : -1;
-  if (nb > 0) nb = nb > INT_MAX / head_pages ? INT_MAX : nb * head_pages;
   void* part = l.part_bytes ? base + l.part : nullptr;
   if (c.q4)
     return nxt_paged_attention_q4_ex(c.out, c.q, c.k, c.v, p.sel_tables, p.sel_lens, (int)rows,
