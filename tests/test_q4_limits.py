@@ -41,3 +41,14 @@ def test_pools_within_the_addresses_are_not_refused():
 @pytest.mark.parametrize("nb", [(2 ** 32 - 2 - 36) // 73 + 2, 2 ** 40, 2 ** 62])
 def test_dense_calls_refuse_the_same(nb):
     assert _dense(nb) == _native.NXT_PA_EINVAL
+
+
+@pytest.mark.parametrize("rows,heads,D,tiles,split", [
+    (1, 8, 128, 24, False), (1, 8, 128, 25, True), (1, 8, 128, 32, True), (6, 8, 128, 32, True),
+    (6, 8, 64, 48, False), (1, 1, 64, 49, True), (1, 8, 256, 24, False), (1, 8, 256, 32, True),
+    (1, 8, 16, 48, False), (16, 8, 128, 32, False), (16, 8, 128, 48, False), (16, 8, 128, 49, True),
+    (48, 8, 256, 48, False)])
+def test_short_rows_are_split_only_where_they_are_few(rows, heads, D, tiles, split):
+    """A call whose rows all stay whole asks for no workspace."""
+    need = _native.xpa().nxt_paged_attention_q4_workspace_size(rows, heads, D, heads, tiles, 16)
+    assert (need > 0) == split

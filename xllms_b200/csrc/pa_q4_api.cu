@@ -22,9 +22,18 @@ namespace host {
 // 11.1 us, 4 13.9; 512 rows of 64 tiles with their selection 53 and 57), but not
 // below 8, nor below sqrt(tiles / 2): with few rows, a shorter partition saves
 // its own time and costs as much in the merge of the longer list of partials
-// (2 rows of 3254 tiles, D = 256: 8 tiles 47 us, 64 tiles 23). Rows of at most
-// XPA_Q4_WHOLE_TILES stay whole, without a merge (48 rows of 32 tiles 5.4 us,
-// in four parts 6.8; 8 rows 6.8 and 6.0). Finer steps (3/4, 2/3) gain where
+// (2 rows of 3254 tiles, D = 256: 8 tiles 47 us, 64 tiles 23).
+// Short rows stay whole, without a merge. That costs the tiles that a warp then
+// takes one after the other, by head size up to 128 (the few bytes of smaller ones
+// than 64 and the longer steps of larger ones are no part of it), and saves
+// the merge, whose time grows with the rows: XPA_Q4_WHOLE_TILES at D = 128, and
+// XPA_Q4_WHOLE_TILES_MANY at any from half as many rows as SMs on. Whole / split:
+//   rows   D = 64: 24, 32, 48, 64 tiles        D = 128: 16, 24, 32, 48
+//      8   4.8/6.2 5.5/5.6 6.8/6.6 8.0/6.2     5.4/6.6 6.1/7.0 7.2/6.4 9.0/7.2
+//     48   5.0/6.8 5.6/6.4 7.0/7.2 8.2/7.6     5.8/6.8 6.4/7.6 7.6/7.2 9.5/8.6
+//    128   5.1/7.8 5.8/7.4 7.0/10.9 8.3/8.9    5.8/7.8 6.6/9.1 7.8/8.8 9.7/12.6
+// and D = 256: 16, 24, 32 tiles  8 rows 9.3/11.1 10.5/12.1 12.3/10.9, 128 rows
+// 10.5/12.7 11.5/19.8 13.6/19.7 us. Finer steps (3/4, 2/3) gain where
 // lengths differ and lose as much where they do not (16 sequences, 8 KV heads:
 // 4-8K tokens 38 -> 32 us, 8K each 39 -> 45).
 #ifndef XPA_Q4_PART_TILES
@@ -34,7 +43,10 @@ namespace host {
 #define XPA_Q4_ITEMS_PER_SM 3
 #endif
 #ifndef XPA_Q4_WHOLE_TILES
-#define XPA_Q4_WHOLE_TILES 32
+#define XPA_Q4_WHOLE_TILES 24
+#endif
+#ifndef XPA_Q4_WHOLE_TILES_MANY
+#define XPA_Q4_WHOLE_TILES_MANY 48
 #endif
 #ifndef XPA_Q4_MIN_TILES
 #define XPA_Q4_MIN_TILES 8
@@ -44,7 +56,9 @@ Plan tile_plan(int B, int Hq, int D, int Hkv, int max_blocks, int bs, int nsm) {
   const long long tiles = std::max(1LL, (long long)max_blocks * spp);
   const long long rows = (long long)B * Hkv, want = (long long)XPA_Q4_ITEMS_PER_SM * nsm;
   long long pt = XPA_Q4_PART_TILES;
-  if (tiles > XPA_Q4_WHOLE_TILES)
+  const bool whole = tiles * std::clamp(D, 64, 128) <= XPA_Q4_WHOLE_TILES * 128 ||
+                     (2 * rows >= nsm && tiles <= XPA_Q4_WHOLE_TILES_MANY);
+  if (!whole)
     while (pt > XPA_Q4_MIN_TILES && pt * pt > tiles && rows * ceil_div(tiles, pt) < want)
       pt >>= 1;
   while (ceil_div(tiles, pt) > 8192) pt <<= 1;
