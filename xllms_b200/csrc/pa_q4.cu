@@ -954,17 +954,25 @@ cudaError_t launch_rows(void (*one)(Q4RowsParams), void (*four)(Q4RowsParams),
 
 }  // namespace
 
+// The head sizes that attention has swizzles of its own for have their address
+// arithmetic folded here too (8192 tokens x 8 heads stored and read back, folded /
+// not: D = 64 17.9 / 21.3 us, 128 32.0 / 38.2; 4096 tokens, 256 31.4 / 38.3).
 cudaError_t launch_q4_write(const Q4RowsParams& a, cudaStream_t st) {
-  // head size 128, where most rows come from, with its address arithmetic folded
-  if (a.D == 128)
-    return launch_rows(pa_q4_write_kernel<1, 128>, pa_q4_write_kernel<4, 128>, a, st);
-  return launch_rows(pa_q4_write_kernel<1, 0>, pa_q4_write_kernel<4, 0>, a, st);
+  switch (a.D) {
+    case 64: return launch_rows(pa_q4_write_kernel<1, 64>, pa_q4_write_kernel<4, 64>, a, st);
+    case 128: return launch_rows(pa_q4_write_kernel<1, 128>, pa_q4_write_kernel<4, 128>, a, st);
+    case 256: return launch_rows(pa_q4_write_kernel<1, 256>, pa_q4_write_kernel<4, 256>, a, st);
+    default: return launch_rows(pa_q4_write_kernel<1, 0>, pa_q4_write_kernel<4, 0>, a, st);
+  }
 }
 
 cudaError_t launch_q4_read(const Q4RowsParams& a, cudaStream_t st) {
-  if (a.D == 128)
-    return launch_rows(pa_q4_read_kernel<1, 128>, pa_q4_read_kernel<4, 128>, a, st);
-  return launch_rows(pa_q4_read_kernel<1, 0>, pa_q4_read_kernel<4, 0>, a, st);
+  switch (a.D) {
+    case 64: return launch_rows(pa_q4_read_kernel<1, 64>, pa_q4_read_kernel<4, 64>, a, st);
+    case 128: return launch_rows(pa_q4_read_kernel<1, 128>, pa_q4_read_kernel<4, 128>, a, st);
+    case 256: return launch_rows(pa_q4_read_kernel<1, 256>, pa_q4_read_kernel<4, 256>, a, st);
+    default: return launch_rows(pa_q4_read_kernel<1, 0>, pa_q4_read_kernel<4, 0>, a, st);
+  }
 }
 
 }  // namespace xpa
