@@ -542,8 +542,8 @@ __global__ void __launch_bounds__(NW * 32, MINB) pa_q4_kernel(const Params p, co
   const float slack = fminf(kRaise / sl, 1e30f);  // kRaise in units of q . k
 
   // ── Q fragments: head g of tile nt, channels 16 j + 4 t .. + 3 ──────────
-  // Groups go in pairs, a missing one as 0: with the second half of a word's
-  // conversions unused, the compiler's conversions of the first came out wrong.
+  // Groups go in pairs, a missing one as 0, so that both halves of a word of codes
+  // are used (q4x8_to_h2).
   constexpr int NGP = NG + NG % 2;
   uint32_t qf[NGP][NT][2];
   {

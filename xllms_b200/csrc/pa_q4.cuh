@@ -45,6 +45,12 @@ __device__ __forceinline__ int q4_v_scale_off(int D, int tok, int grp) {
 
 // ── decoding ────────────────────────────────────────────────────────────
 // The eight codes of a word -> four fp16x2 (byte i: low nibble in the low half).
+// Callers use outputs of both 16-bit halves of the word (0 or 1, and 2 or 3): where
+// those of one half alone are used, what ptxas 12.9.86 makes of this gives wrong
+// values. Tried on a B200 over all 65536 values of a half: outputs {0, 1}, {2, 3}
+// and each by itself are wrong, {0, 2}, {1, 3}, any three and all four right.
+// Bytes taken apart by way of 16-bit registers, or one to a statement, are wrong at
+// output 2 even with all four in use.
 __device__ __forceinline__ void q4x8_to_h2(uint32_t w, uint32_t (&h)[4]) {
   asm("{\n\t.reg .b8 p, q, r, s;\n\tmov.b32 {p, q, r, s}, %4;\n\t"
       "cvt.rn.f16x2.e2m1x2 %0, p;\n\tcvt.rn.f16x2.e2m1x2 %1, q;\n\t"
