@@ -867,15 +867,26 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t
 #define XPA_Q4_MIN_CTAS_ODD 2
 #endif
 
+#ifndef XPA_Q4_MIN_CTAS_LARGE
+#define XPA_Q4_MIN_CTAS_LARGE 3
+#endif
+
 template <int D, int NT>
 cudaError_t launch_q4_t(const Params& p, cudaStream_t st) {
   constexpr bool EXACT = Q4Stage<D>::EXACT;
   constexpr int NW = XPA_Q4_WARPS;
   // two tiles a step against one and a ring of four, 64 sequences of 1-8K tokens:
-  // D = 96 74 against 77 us, 160 109 / 115, 240 206 / 226
+  // D = 64 59 against 61 us, 96 85 / 90, 128 88 / 94, 160 122 / 149, 240 222 / 243
   constexpr int U = XPA_Q4_TILES, STAGES = XPA_Q4_STAGES;
-  // the head sizes without a swizzle of their own take more registers
-  constexpr int MINB = D <= 128 && NT == 1 ? (EXACT ? XPA_Q4_MIN_CTAS : XPA_Q4_MIN_CTAS_ODD) : 1;
+  // Resident CTAs per SM that the registers are held down for. Head sizes without a
+  // swizzle of their own take more: four of them at 80 to 112 gain 2-3 % there and
+  // lose 5 % on short ragged rows. From 144 to 192 three CTAs take 129, 122, 147, 127
+  // us (144, 160, 176, 192; as above), two 143, 134, 161, 141.
+  constexpr int MINB = NT > 1     ? 1
+                       : EXACT && D <= 128 ? XPA_Q4_MIN_CTAS
+                       : D <= 128 ? XPA_Q4_MIN_CTAS_ODD
+                       : D <= 192 ? XPA_Q4_MIN_CTAS_LARGE
+                                  : 1;
   using C = Q4Cfg<D, NT, NW, STAGES, U>;
   auto kern = pa_q4_kernel<D, NT, NW, STAGES, U, MINB>;
   static std::atomic<unsigned long long> done{0};
