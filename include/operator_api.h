@@ -363,10 +363,12 @@ int nxt_read_cache_q4(
 
 /* Paged decode attention over 4-bit pools: the result of
  * nxt_paged_attention_ex over the dequantised cache, for any number of query
- * heads per KV head. Masking, clamping, status bits and workspace as there; a
+ * heads per KV head; a head with a NaN score gives zeros here as there. Masking, clamping, status bits and workspace as there; a
  * caller-owned workspace needs nxt_paged_attention_q4_workspace_size bytes.
  * The library's own workspace is one per (device, stream), and for captured
- * calls one per capture, which lives as long as the graph. With num_blocks
+ * calls one per capture, which lives as long as the graph: graphs may be
+ * replayed beside each other and beside eager calls, but not two executables
+ * of one graph, nor copies of it, at the same time. With num_blocks
  * unknown (<= 0), a page that reaches 2^32 times the largest common divisor of
  * kv_block_stride and 9 * head_size bytes into the pool is masked like one
  * outside it; with num_blocks known, such pools are refused. */
@@ -412,7 +414,9 @@ int nxt_paged_attention_q4_append_ex(
  * bounds, the lowest and highest key per channel:
  *   score = max over the KV head's query heads q of
  *           sum_d max(q_d * lo_d, q_d * hi_d),
- * which no q . k of the page exceeds (of q . k times the sign of `scale`). The
+ * which no q . k of the page exceeds (of q . k times the sign of `scale`; for
+ * 4-bit pools q . k of the keys that nxt_read_cache_q4 returns, 2^-11 at most of
+ * each product from those that attention multiplies). The
  * first sink_pages and the last recent_pages pages of a sequence are always
  * kept, the rest of max_pages goes to the best others, in the exact order of
  * the scores, ties to the earlier page. A sequence of at most max_pages pages

@@ -18,12 +18,14 @@ namespace {
 // K before V; a lane takes a piece, neighbouring lanes a 16-channel group, and
 // a warp P times 32 pieces, whose reads are all in flight together: four where
 // that still leaves the GPU warps enough, one for the few tokens of a decode
-// step, whose time is the chain of one piece. HBM is not the bound: storing 8192
-// tokens x 8 heads x 128 and reading them back (43 MB each) takes 32 us, where the
-// bytes alone take 13, with 80 % of the issue slots used: the corrected
-// quotients, conversions and addresses are 30 instructions a channel to write
-// and 18 to read. A quotient by the reciprocal alone would be off by an ulp,
-// and a code by a step wherever that crosses a midpoint.
+// step, whose time is the chain of one piece. Instruction issue is the bound:
+// storing 8192 tokens x 8 heads x 128 and reading them back (43 MB each) takes 32
+// us with the rows and pools in L2 (40 from HBM, where the bytes alone take 13),
+// 70-75 % of the issue slots used: the corrected quotients, conversions and
+// addresses are 31 instructions a channel to write and 18 to read, the addresses of
+// two 2-byte codes and a scale byte for only 8 channels a large part of them. A
+// quotient by the reciprocal alone would be off by an ulp, and a code by a step
+// wherever that crosses a midpoint.
 // ════════════════════════════════════════════════════════════════════════
 
 struct RowAt {
@@ -239,14 +241,14 @@ __global__ void __launch_bounds__(128) pa_q4_read_kernel(const Q4RowsParams a) {
 // as the output's own rounding.
 //
 // Bound and measured, 32 heads over 8 of 128: 12 sequences of 64K tokens (906
-// MB) take 174 us, 0.79 of the copy rate, 64 of 1-8K (336 MB) 78 us, 0.65, as
+// MB) take 198 us, 0.70 of the copy rate, 64 of 1-8K (336 MB) 88 us, 0.58, as
 // the items of a ragged batch end apart (shorter items, or the short ones last,
-// were no faster); 62 us if nothing is computed, 81 if nothing is copied (two
-// fp16 terms then). At the copy rate there are 3.1 issue slots for 32 elements
-// and the kernel uses 2.2, half an instruction each of them for conversions and
-// scalings; the long case has the issue slots 65 % busy, the conversions'
-// half-rate pipe 54 %, the tensor pipe 29 %, and a warp waits for its turn, a
-// fixed latency or a pipe. So the shape that counts is the one with the fewest
+// were no faster); 61 us if nothing is computed, 75 if nothing is copied. At the
+// copy rate there are 3.1 issue slots for 32 elements and the kernel uses 2.4,
+// half an instruction each of them for conversions and scalings; the long case
+// has the issue slots 62 % busy, the conversions' half-rate pipe 49 %, the tensor
+// pipe 38 %, and a warp waits for its turn, a fixed latency or a pipe. So the
+// shape that counts is the one with the fewest
 // instructions per element: K and V go through mma.sync straight from
 // registers, where tcgen05 would want the unpacked fp16 operands written to
 // shared memory first (3.6 times the bytes that were read) and the few rows of
@@ -866,7 +868,6 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t
 #ifndef XPA_Q4_MIN_CTAS_ODD
 #define XPA_Q4_MIN_CTAS_ODD 2
 #endif
-
 #ifndef XPA_Q4_MIN_CTAS_LARGE
 #define XPA_Q4_MIN_CTAS_LARGE 3
 #endif
@@ -882,11 +883,11 @@ cudaError_t launch_q4_t(const Params& p, cudaStream_t st) {
   // swizzle of their own take more: four of them at 80 to 112 gain 2-3 % there and
   // lose 5 % on short ragged rows. From 144 to 192 three CTAs take 129, 122, 147, 127
   // us (144, 160, 176, 192; as above), two 143, 134, 161, 141.
-  constexpr int MINB = NT > 1     ? 1
+  constexpr int MINB = NT > 1              ? 1
                        : EXACT && D <= 128 ? XPA_Q4_MIN_CTAS
-                       : D <= 128 ? XPA_Q4_MIN_CTAS_ODD
-                       : D <= 192 ? XPA_Q4_MIN_CTAS_LARGE
-                                  : 1;
+                       : D <= 128          ? XPA_Q4_MIN_CTAS_ODD
+                       : D <= 192          ? XPA_Q4_MIN_CTAS_LARGE
+                                           : 1;
   using C = Q4Cfg<D, NT, NW, STAGES, U>;
   auto kern = pa_q4_kernel<D, NT, NW, STAGES, U, MINB>;
   static std::atomic<unsigned long long> done{0};

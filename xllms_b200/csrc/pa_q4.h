@@ -32,7 +32,7 @@ cudaError_t launch_q4_read(const Q4RowsParams& a, cudaStream_t st);
 
 // Decode attention over 4-bit pools; Params as for the other attention
 // kernels, with the pool strides in bytes. p.part_pages / max_parts / slots
-// as planned by q4_plan.
+// as planned by host::tile_plan, p.ml_unit from host::score_unit.
 cudaError_t launch_q4_attention(const Params& p, cudaStream_t st);
 
 }  // namespace xpa

@@ -19,10 +19,10 @@ namespace host {
 // Partitions of a call, in 16-token tiles rounded to whole pages: at most
 // XPA_Q4_PART_TILES, halved while the grid would hold fewer than
 // XPA_Q4_ITEMS_PER_SM items per SM (8 sequences of 2048 tokens, 8 KV heads: 3
-// 11.1 us, 4 13.9; 512 rows of 64 tiles with their selection 53 and 57), but not
+// 11.5 us, 4 14.4; 512 rows of 64 tiles with their selection 56 and 59), but not
 // below 8, nor below sqrt(tiles / 2): with few rows, a shorter partition saves
 // its own time and costs as much in the merge of the longer list of partials
-// (2 rows of 3254 tiles, D = 256: 8 tiles 47 us, 64 tiles 23).
+// (2 rows of 3254 tiles, D = 256: 8 tiles 55 us, 64 tiles 26).
 // Short rows stay whole, without a merge. That costs the tiles that a warp then
 // takes one after the other, by head size up to 128 (the few bytes of smaller ones
 // than 64 and the longer steps of larger ones are no part of it), and saves
@@ -34,8 +34,8 @@ namespace host {
 //    128   5.1/7.8 5.8/7.4 7.0/10.9 8.3/8.9    5.8/7.8 6.6/9.1 7.8/8.8 9.7/12.6
 // and D = 256: 16, 24, 32 tiles  8 rows 9.3/11.1 10.5/12.1 12.3/10.9, 128 rows
 // 10.5/12.7 11.5/19.8 13.6/19.7 us. Finer steps (3/4, 2/3) gain where
-// lengths differ and lose as much where they do not (16 sequences, 8 KV heads:
-// 4-8K tokens 38 -> 32 us, 8K each 39 -> 45).
+// lengths differ and lose as much where they do not (16 sequences, 8 KV heads, a
+// tenth less than now: 4-8K tokens 38 -> 32 us, 8K each 39 -> 45).
 #ifndef XPA_Q4_PART_TILES
 #define XPA_Q4_PART_TILES 128
 #endif

@@ -4,8 +4,8 @@
 // A page's bounds are, per KV head and channel, the lowest and the highest of
 // its keys. For a query head q the page's score is
 //   sum_d max(q_d lo_d, q_d hi_d) = sum_d (q_d^+ hi_d + q_d^- lo_d),
-// no less than any q . k of the page; the score of a KV head is the largest
-// over its query heads. The best pages are kept, in the exact order of the
+// no less than any q . k of the page (4-bit keys: of the keys rounded to fp16, as
+// their bounds are); the score of a KV head is the largest over its query heads. The best pages are kept, in the exact order of the
 // scores, ties to the earlier page.
 #include <algorithm>
 #include <cfloat>

@@ -55,7 +55,7 @@ struct SelectParams {
   int copies;  // of every row's tables, for attention that takes its heads in parts
   int sub;     // entries per kept page: page id * sub_ids + 0 .. sub - 1, for attention
   int sub_ids; // that takes a page in pieces of 16 tokens (sub > 1 needs order)
-  int chunks, chunk_pages;  // score CTAs per row (or 8 rows), pages of each
+  int chunks, chunk_pages;  // score CTAs per row (or kScoreWarps rows), pages of each
   int tiles, tile_pages;    // entries of a row's magnitude, pages of each
   float sign;  // of the score scale: -1, 0 or 1
   int vec;     // fp16, D % 8 == 0, q and bounds on 16-byte boundaries
@@ -85,7 +85,8 @@ cudaError_t launch_select(const SelectParams& p, int dtype_size, cudaStream_t st
 
 // Decode attention over fp16 pages (pa_pages.cu): D and block_size multiples of
 // 16, rows on 16-byte boundaries, the query on 4-byte ones. Params as for the
-// other attention kernels; part_pages / max_parts / slots as tile_plan has them.
+// other attention kernels; part_pages / max_parts / slots as tile_plan has them,
+// ml_unit as score_unit does.
 cudaError_t launch_pages(const Params& p, cudaStream_t st);
 
 }  // namespace xpa
